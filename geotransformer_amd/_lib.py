@@ -17,7 +17,7 @@ c_ptr = ctypes.c_void_p
 c_size = ctypes.c_size_t
 c_int = ctypes.c_int
 
-ABI_VERSION = 8  # geotr_abi_version() of the library this package's ctypes mirrors (native.py, kernels.py) were written against
+ABI_VERSION = 9  # geotr_abi_version() of the library this package's ctypes mirrors (native.py, kernels.py) were written against
 
 # name -> (restype, argtypes); must list every symbol include/geotr.h declares (tests check this)
 SIGNATURES = {
@@ -129,6 +129,12 @@ SIGNATURES = {
     'geotr_apply_transform': (c_int, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
     'geotr_pairwise_distance': (c_int, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_ptr, c_ptr]),
     'geotr_index_select': (c_int, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
+    'geotr_rotary': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_i64, c_i64, c_i64, c_i64, c_int, c_ptr, c_int, c_i64, c_i64, c_i64, c_ptr, c_ptr,
+                             c_f32, c_int, c_ptr]),
+    'geotr_diff_attn_workspace_bytes': (c_size, [c_ptr]),  # struct pointers; typed in geotransformer_amd/kernels.py
+    'geotr_diff_attn_forward': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
+    'geotr_diff_attn_backward_workspace_bytes': (c_size, [c_ptr]),
+    'geotr_diff_attn_backward': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
     'geotr_lgr': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_f32, c_int, c_f32, c_i64,
                           c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
 }

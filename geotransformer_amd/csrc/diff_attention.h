@@ -1,0 +1,919 @@
+// diff_attention.h -- kernels of the differential attention (geotr_diff_attn_*, include/geotr.h), instantiated per type in
+// diff_attention_{f32,bf16,f16}.hip.
+//
+//   out_h = sum_j (P1_ij - lam_h P2_ij) v_j,   Pa_ij = softmax_j(s q_a,i . k_a,j),   heads 2h and 2h + 1 of q and k are the two maps.
+//
+// One pass over the keys with a running maximum and sum for each map and two accumulators (O1 and O2 share every fragment of V):
+//   4 D + 4 Dv products per (row, key).  Joining the weights first would need the sums before the pass: one V product less, but every
+//   score and exponential twice.
+// Backward, from lse_a = log2 of the sums and del_a = dO . O_a (attention output of map a):
+//   dP = dO V^T;  dS1 = P1 (dP - del1);  dS2 = -lam P2 (dP - del2);  dQa = s dSa Ka;  dKa = s dSa^T Qa;  dV = (P1 - lam P2)^T dO;
+//   dlam = - sum_ij P2 dP.  Two kernels, one that owns query rows (dQ, dlam) and one that owns keys (dK, dV): the scores are computed
+//   twice, and no sum depends on the order of atomics.
+//
+// Layout of the matrix work (32 x 32 MFMA, a wave = 32 rows of one kind): scores are computed TRANSPOSED to how they are consumed, so the
+// accumulator a lane holds (16 of 32 contraction indices of ONE row) is the B operand of the next product as it stands: no exchange
+// between lanes and no LDS round trip for P and dS.  The other operand of that product is read transposed from LDS (ds_read_b64_tr_b16;
+// 32-bit: ds_read_b32 along the row), contraction indices in the same order: 8 (r / 4) + 4 half + r % 4 for accumulator register r.
+// A row of a head group: with g query heads to a key head the g heads of a query are g consecutive rows r = i g + h of the tile, so they
+// share every K and V fragment, and one query row over a long cache still fills g rows of the tile.
+// Tiles go global -> LDS by 16-byte buffer loads (no registers), rows that do not exist or are masked and channels beyond D / Dv at an
+// offset past the buffer's end: the hardware writes zeros, so what a masked row holds (NaN included) never enters a product.  The chunk
+// order inside a row is permuted by the row (swizzle): row reads and transposed reads both spread over all banks.
+#pragma once
+#include "common.h"
+
+namespace geotr {
+namespace dattn {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+#define GEOTR_LDS __attribute__((address_space(3)))
+
+struct Args {
+  geotr_heads q, k, v, dout;             // dout: backward only
+  void *out, *o2, *gq, *gk, *gv;         // contiguous (rows, heads, channels)
+  float *lse, *del, *part, *drow;        // (hk, 2, nq, g), (hk, 2, nq, g), split partials, (hk, nq, g)
+  const float* amax;                     // 16-bit floats of narrow range: largest |dout| (backward), else null
+  const float* lam;
+  const int64_t *q_len, *k_len;
+  const uint8_t* masks;                  // (nk) 1 = ignored key
+  int64_t nq, nk;                        // all rows
+  int batch, stacked, n, m;              // batch mode: n, m rows per sequence
+  int hk, g, d, dv, causal, splits;
+  float scale, scale_log2;
+};
+
+// ---- types: E elements in 16 bytes, a contraction step of 2 E, one 16-byte fragment per lane and step -----------------------------------
+template <typename T>
+struct Ops;
+template <>
+struct Ops<__bf16> {
+  using Frag = __attribute__((ext_vector_type(8))) __bf16;
+  static __device__ __forceinline__ void mma(f32x16& c, Frag a, Frag b) { c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Ops<_Float16> {
+  using Frag = __attribute__((ext_vector_type(8))) _Float16;
+  static __device__ __forceinline__ void mma(f32x16& c, Frag a, Frag b) { c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Ops<float> {
+  using Frag = f32x4;
+  static __device__ __forceinline__ void mma(f32x16& c, Frag a, Frag b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+  }
+};
+
+template <typename T>
+constexpr int kE = 16 / sizeof(T);         // elements of a fragment
+template <typename T>
+constexpr int kStep = 2 * kE<T>;           // channels (row reads) or contraction indices of one step
+template <typename T>
+constexpr int kPSteps = 32 / kStep<T>;     // steps of a 32-deep product
+
+// fragment t of the accumulator's 32 contraction indices: registers E t .. E t + E - 1 (rounded to T: the one rounding of P and dS)
+template <typename T>
+__device__ __forceinline__ typename Ops<T>::Frag pack(const f32x16& p, int t) {
+  typename Ops<T>::Frag f;
+#pragma unroll
+  for (int i = 0; i < kE<T>; ++i) f[i] = (T)p[kE<T> * t + i];
+  return f;
+}
+
+// ---- LDS tiles ------------------------------------------------------------------------------------------------------------------------
+// A tile of `rows` rows of C 16-byte chunks; chunk c of row r lies at position c ^ swz(r).  256 bytes (all banks) hold RP = 16 / C rows.
+template <int C>
+__device__ __forceinline__ int swz(int row) {
+  constexpr int RP = C >= 16 ? 1 : 16 / C, M = (C >= 16 ? 16 : C) - 1;
+  const int x = row / RP;
+  return (((x << 1) & 14) | ((x >> 3) & 1)) & M;
+}
+// fragment of row `row`: channels of chunk `chunk` (C-operand order of a row read: lane % 32 = row, half h reads chunk 2 s + h)
+template <typename T, int C>
+__device__ __forceinline__ typename Ops<T>::Frag row_frag(const char* tile, int row, int chunk) {
+  return *(const typename Ops<T>::Frag*)(tile + (row * C + (chunk ^ swz<C>(row))) * 16);
+}
+// transposed fragment: lane % 32 = channel col0 + lane % 32, contraction indices = rows row0 + (order of accumulator registers, step t)
+template <typename T, int C>
+__device__ __forceinline__ typename Ops<T>::Frag col_frag(const char* tile, int row0, int t, int col0, int lane) {
+  typename Ops<T>::Frag f;
+  if constexpr (sizeof(T) == 2) {
+    const int row = row0 + 16 * t + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int chunk = col0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const char* a = tile + (row * C + (chunk ^ swz<C>(row))) * 16 + (lane & 1) * 8;
+    const char* b = tile + ((row + 8) * C + (chunk ^ swz<C>(row + 8))) * 16 + (lane & 1) * 8;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GEOTR_LDS s16x4*)a);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GEOTR_LDS s16x4*)b);
+    const auto z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    f = __builtin_bit_cast(typename Ops<T>::Frag, z);
+  } else {
+    const int chunk = col0 / 4 + ((lane & 31) >> 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + 8 * t + 4 * (lane >> 5) + i;
+      f[i] = *(const float*)(tile + (row * C + (chunk ^ swz<C>(row))) * 16 + (lane & 3) * 4);
+    }
+  }
+  return f;
+}
+
+constexpr int kNumRecords = 0x40000000, kOutside = 0x7fffff00;  // a chunk at kOutside lies past every buffer: zeros
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, kNumRecords, 0x00020000);
+}
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, char* lds, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (GEOTR_LDS void*)lds, 16, offset, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ typename Ops<T>::Frag load_frag(__amdgpu_buffer_rsrc_t r, int offset) {
+  return __builtin_bit_cast(typename Ops<T>::Frag, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
+}
+
+// ROWS rows of NM maps of `width` channels (bucket DB) into `tile`, dealt over the SHARE waves that use it (wave w of them).  src(row)
+// gives the byte offset of a row or kOutside.
+template <typename T, int ROWS, int NM, int DB, int SHARE, class Src>
+__device__ __forceinline__ void stage(char* tile, __amdgpu_buffer_rsrc_t r, int width, int map_bytes, int w, int lane, Src src) {
+  constexpr int CM = DB * (int)sizeof(T) / 16, C = NM * CM, N = ROWS * C / 64;
+  static_assert(ROWS * C % 64 == 0, "whole wave loads");
+#pragma unroll
+  for (int it = 0; it < (N + SHARE - 1) / SHARE; ++it) {
+    const int i = it * SHARE + w;
+    if (N % SHARE != 0 && i >= N) break;
+    const int p = i * 64 + lane, row = p / C, c = (p % C) ^ swz<C>(row);
+    const int map = NM == 1 ? 0 : c / CM, cc = NM == 1 ? c : c % CM;
+    const int o = src(row);
+    load_lds(r, tile + i * 1024, (o == kOutside || cc * kE<T> >= width) ? kOutside : o + map * map_bytes + cc * 16);
+  }
+}
+
+// ---- sequences ------------------------------------------------------------------------------------------------------------------------
+struct Seq {
+  int b;             // address index of the batch (0 in stack mode)
+  int64_t q0, k0;    // first row in all rows
+  int n, m, tile;    // tile < 0: behind the last sequence
+  int spare, spares; // index and number of the blocks behind the last sequence
+  int64_t q_end, k_end;
+};
+constexpr int kMostRows = 1 << 30;
+__device__ __forceinline__ int clamp_len(int64_t v, int64_t most) { return (int)(v < 0 ? 0 : v > most ? most : v); }
+__device__ __forceinline__ int add_sat(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)kMostRows); }
+
+// Sequence and tile (TILE packed query rows, or keys when KEYS) of block `t`.  Stack mode: lengths on the device, one scan of 64 clouds at
+// a time by every wave; sums are held at 2^30 and rows clamped to what exists, so lengths that do not fit never address past the arrays.
+template <int TILE, bool KEYS>
+__device__ __forceinline__ Seq find_seq(const Args& a, int b, int t, int tiles) {
+  Seq s;
+  s.spare = 0, s.spares = 1, s.q_end = a.nq, s.k_end = a.nk;
+  if (!a.stacked) {
+    s.b = b, s.q0 = (int64_t)b * a.n, s.k0 = (int64_t)b * a.m, s.tile = t;
+    s.n = a.q_len ? clamp_len(a.q_len[b], a.n) : a.n;
+    s.m = a.k_len ? clamp_len(a.k_len[b], a.m) : a.m;
+    return s;
+  }
+  const int lane = lane_id();
+  int qs = 0, ks = 0, ts = 0;
+  s.b = 0, s.tile = -1, s.n = s.m = 0, s.q0 = s.k0 = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int i = b0 + lane;
+    int ql = i < a.batch ? clamp_len(a.q_len[i], a.nq) : 0, kl = i < a.batch ? clamp_len(a.k_len[i], a.nk) : 0;
+    const int ql0 = ql, kl0 = kl;
+    int tl = KEYS ? (kl + TILE - 1) / TILE : (int)(((int64_t)ql * a.g + TILE - 1) / TILE);
+    const int tl0 = tl;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(ql, o, 64), y = __shfl_up(kl, o, 64), z = __shfl_up(tl, o, 64);
+      if (lane >= o) ql = add_sat(ql, x), kl = add_sat(kl, y), tl = add_sat(tl, z);
+    }
+    ql = add_sat(ql, qs), kl = add_sat(kl, ks), tl = add_sat(tl, ts);
+    const uint64_t hit = __ballot(tl > t && tl - tl0 <= t && tl0 > 0);
+    if (hit && s.tile < 0) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      const int qe = __shfl(ql, l, 64), ke = __shfl(kl, l, 64), te = __shfl(tl, l, 64);
+      const int qn = __shfl(ql0, l, 64), kn = __shfl(kl0, l, 64), tn = __shfl(tl0, l, 64);
+      s.q0 = qe - qn, s.k0 = ke - kn, s.tile = t - (te - tn);
+      s.n = (int)(s.q0 < a.nq ? (s.q0 + qn > a.nq ? a.nq - s.q0 : qn) : 0);
+      s.m = (int)(s.k0 < a.nk ? (s.k0 + kn > a.nk ? a.nk - s.k0 : kn) : 0);
+      s.tile = __builtin_amdgcn_readfirstlane(s.tile);
+      s.n = __builtin_amdgcn_readfirstlane(s.n), s.m = __builtin_amdgcn_readfirstlane(s.m);
+      s.q0 = __builtin_amdgcn_readfirstlane((int)s.q0), s.k0 = __builtin_amdgcn_readfirstlane((int)s.k0);
+      return s;
+    }
+    qs = __shfl(ql, 63, 64), ks = __shfl(kl, 63, 64), ts = __shfl(tl, 63, 64);
+  }
+  s.spare = t - ts, s.spares = max(1, tiles - ts);
+  s.q_end = min((int64_t)qs, a.nq), s.k_end = min((int64_t)ks, a.nk);
+  return s;
+}
+
+// keys key0 .. key0 + 63 that exist and are not masked
+__device__ __forceinline__ uint64_t key_bits(const Args& a, const Seq& s, int key0, int end, int lane) {
+  if (a.masks) {
+    const int j = key0 + lane;
+    return __ballot(j < end && !a.masks[s.k0 + j]);
+  }
+  const int left = end - key0;
+  return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+}
+
+__device__ __forceinline__ float swap_max(float x) {
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
+__device__ __forceinline__ float swap_add(float x) {
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// Scores beyond 2^20 (in powers of two): s c - b with a product of its own.  An fma keeps the exact product, whose distance from the
+// rounded maximum b grows with it until the exponential overflows; rounded alike, the largest score gives exactly 0.
+constexpr float kHuge = 1048576.f;
+__device__ __forceinline__ float exponent(float s, float c, float b, bool huge) { return huge ? s * c - b : fmaf(s, c, -b); }
+
+// One packed query row of a lane: its query, head within the group, and whether it exists
+struct Row {
+  int i, h;
+  bool in;
+};
+__device__ __forceinline__ Row row_of(const Args& a, const Seq& s, int r) {
+  Row x;
+  x.i = a.g == 1 ? r : r / a.g;
+  x.h = a.g == 1 ? 0 : r - x.i * a.g;
+  x.in = r < s.n * a.g;
+  return x;
+}
+__device__ __forceinline__ int64_t stat_at(const Args& a, int kvh, int map, int64_t row, int h) {
+  return (((int64_t)kvh * 2 + map) * a.nq + row) * a.g + h;
+}
+
+// four consecutive channels of an output row
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float x, float y, float z, float w) {
+  struct alignas(4 * sizeof(T)) V { T v[4]; };
+  *(V*)p = V{{(T)x, (T)y, (T)z, (T)w}};
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------------------------------
+// NW waves.  KEYS = false: wave w owns packed rows 32 w .. of the block's 32 NW, all waves share the staged tile of BN keys.
+// KEYS = true (few rows): all waves own the same 32 rows and every wave streams key tiles of its own (no barrier), joined at the end; with
+// a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next launch.
+template <typename T, int DB, int DVB, int NW, bool KEYS>
+__global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
+  using Frag = typename Ops<T>::Frag;
+  constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>;
+  constexpr int kTileBytes64 = 64 * (CK + CV) * 16;
+  constexpr int BN = KEYS ? 32 : (kTileBytes64 <= 40960 ? 64 : 32);
+  constexpr int kTile = BN * (CK + CV) * 16;
+  constexpr int kJoin = KEYS ? (NW / 2) * 64 * (2 * NT * 16 + 4) * 4 : 0;
+  constexpr int kSmem = KEYS ? (kTile * NW > kJoin ? kTile * NW : kJoin) : 2 * kTile;
+  __shared__ __attribute__((aligned(1024))) char smem[kSmem];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+  constexpr int TILE = KEYS ? 32 : 32 * NW;
+  const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
+  const int t = a.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y;  // causal: the longest rows first
+  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
+  T* const out = (T*)a.out;
+  T* const o2 = (T*)a.o2;
+  if (s.tile < 0) {  // rows behind the last sequence: zero results
+    const int64_t rows = s.q_end < a.nq ? a.nq - s.q_end : 0, per = (int64_t)a.g * a.dv;
+    if (a.splits > 1) {  // no keys: the join writes zeros
+      const int w = a.dv + 4;
+      for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * a.g; e += (int64_t)s.spares * (NW * 64)) {
+        float* p = a.part + (((int64_t)blockIdx.z * a.nq + s.q_end + e / a.g) * a.hk * a.g + kvh * a.g + e % a.g) * 2 * w;
+        p[0] = p[w] = -INFINITY, p[1] = p[w + 1] = 0.f;
+      }
+      return;
+    }
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * per; e += (int64_t)s.spares * (NW * 64)) {
+      const int64_t i = e / per, o = ((s.q_end + i) * a.hk + kvh) * per + (e - i * per);
+      out[o] = (T)0.f;
+      if (o2) o2[o] = (T)0.f;
+    }
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; a.lse && e < rows * a.g; e += (int64_t)s.spares * (NW * 64)) {
+      const int64_t at = stat_at(a, kvh, 0, s.q_end, 0) + e;
+      a.lse[at] = a.lse[at + a.nq * a.g] = INFINITY;
+    }
+    return;
+  }
+  const int row_base = s.tile * TILE;
+  const int rows_here = a.stacked ? s.n : a.n;  // batch mode: rows beyond the length get zeros
+  if (row_base >= rows_here * a.g) return;
+  const int r = row_base + (KEYS ? 0 : 32 * wave) + col;
+  const Row row = row_of(a, s, r);
+
+  // Q: B operand, lane = row, straight from global memory
+  Frag q1[QS], q2[QS];
+  {
+    const auto rq = buffer((const T*)a.q.data + s.b * a.q.batch_stride + (a.stacked ? s.q0 : 0) * a.q.row_stride +
+                           (int64_t)kvh * 2 * a.g * a.q.head_stride + (int64_t)(row_base / a.g) * a.q.row_stride);
+    const int o = (int)(((row.i - row_base / a.g) * a.q.row_stride + 2 * row.h * a.q.head_stride) * (int)sizeof(T));
+    const int hs = (int)(a.q.head_stride * sizeof(T));
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      const int c = (2 * i + half) * kE<T>;
+      const bool in = row.in && c < a.d;
+      q1[i] = load_frag<T>(rq, in ? o + c * (int)sizeof(T) : kOutside);
+      q2[i] = load_frag<T>(rq, in ? o + hs + c * (int)sizeof(T) : kOutside);
+    }
+  }
+  f32x16 acc1[NT], acc2[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc1[i] = zero16(), acc2[i] = zero16();
+  float m1 = -INFINITY, m2 = -INFINITY, l1 = 0.f, l2 = 0.f;
+  bool huge = false;
+
+  const T* const kp = (const T*)a.k.data + s.b * a.k.batch_stride + (a.stacked ? s.k0 : 0) * a.k.row_stride + (int64_t)kvh * 2 * a.k.head_stride;
+  const T* const vp = (const T*)a.v.data + s.b * a.v.batch_stride + (a.stacked ? s.k0 : 0) * a.v.row_stride + (int64_t)kvh * a.v.head_stride;
+  const int off = s.m - s.n;                         // causal: key j for query i iff j <= i + off
+  const int limit = a.causal ? row.i + off : 0x7fffffff;
+  int end = s.m;
+  if (a.causal) {  // no key beyond the last row's limit
+    const int last = min(row_base + TILE, s.n * a.g) - 1;
+    end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
+  }
+  int begin = 0;
+  if (a.splits > 1) {
+    const int tiles = (end + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
+    begin = min(end, (int)blockIdx.z * per * 32);
+    end = min(end, begin + per * 32);
+  }
+
+  constexpr int SHARE = KEYS ? 1 : NW;
+  const int w = KEYS ? 0 : wave;
+  auto fill = [&](char* tile, int key0, uint64_t bits) {
+    const auto rk = buffer(kp + (int64_t)key0 * a.k.row_stride);
+    const auto rv = buffer(vp + (int64_t)key0 * a.v.row_stride);
+    const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
+    stage<T, BN, 2, DB, SHARE>(tile, rk, a.d, (int)(a.k.head_stride * sizeof(T)), w, lane,
+                        [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
+    stage<T, BN, 1, DVB, SHARE>(tile + BN * CK * 16, rv, a.dv, 0, w, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
+  };
+
+  // 32 keys of a staged tile
+  auto consume = [&](const char* tile, int sub, int key0, uint64_t bits) {
+    const char* vt = tile + BN * CK * 16;
+    f32x16 s1 = zero16(), s2 = zero16();
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      Ops<T>::mma(s1, row_frag<T, CK>(tile, 32 * sub + col, 2 * i + half), q1[i]);
+      Ops<T>::mma(s2, row_frag<T, CK>(tile, 32 * sub + col, CK / 2 + 2 * i + half), q2[i]);
+    }
+    const int k0 = key0 + 32 * sub;
+    unsigned lo = (unsigned)(bits >> (32 * sub));
+    const int above = limit - k0;  // keys of the tile up to this one
+    if (lo != 0xffffffffu || __any(above < 31)) {
+      if (above < 31) lo = above < 0 ? 0u : lo & ((2u << above) - 1);
+      lo >>= 4 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool in = (lo >> (8 * (i / 4) + i % 4)) & 1;
+        s1[i] = in ? s1[i] : -INFINITY;
+        s2[i] = in ? s2[i] : -INFINITY;
+      }
+    }
+    float x1 = s1[0], x2 = s2[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) x1 = fmaxf(x1, s1[i]), x2 = fmaxf(x2, s2[i]);
+    x1 = swap_max(x1) * a.scale_log2, x2 = swap_max(x2) * a.scale_log2;
+    // the accumulators are rescaled only when a maximum grew by more than 2^8: weights stay below 2^8, sums are exact either way
+    if (__any(x1 > m1 + 8.f || x2 > m2 + 8.f)) {
+      const float n1 = fmaxf(m1, x1), n2 = fmaxf(m2, x2);
+      const float c1 = n1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m1 - n1), c2 = n2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m2 - n2);
+      m1 = n1, m2 = n2, l1 *= c1, l2 *= c2;
+      huge = __any((fabsf(m1) > kHuge && m1 > -INFINITY) || (fabsf(m2) > kHuge && m2 > -INFINITY));
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc1[i][j] *= c1, acc2[i][j] *= c2;
+    }
+    const float b1 = m1 == -INFINITY ? 0.f : m1, b2 = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s1[i] = __builtin_amdgcn_exp2f(exponent(s1[i], a.scale_log2, b1, huge));
+      s2[i] = __builtin_amdgcn_exp2f(exponent(s2[i], a.scale_log2, b2, huge));
+      l1 += s1[i], l2 += s2[i];
+    }
+#pragma unroll
+    for (int p = 0; p < kPSteps<T>; ++p) {
+      const Frag p1 = pack<T>(s1, p), p2 = pack<T>(s2, p);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const Frag f = col_frag<T, CV>(vt, 32 * sub, p, 32 * i, lane);
+        Ops<T>::mma(acc1[i], f, p1);
+        Ops<T>::mma(acc2[i], f, p2);
+      }
+    }
+  };
+
+  if constexpr (KEYS) {
+    char* const mine = smem + wave * kTile;
+    for (int key0 = begin + 32 * wave; key0 < end; key0 += 32 * NW) {
+      const uint64_t bits = key_bits(a, s, key0, end, lane) & 0xffffffffull;
+      if (!bits) continue;
+      fill(mine, key0, bits);
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile is this wave's own
+      asm volatile("" ::: "memory");
+      consume(mine, 0, key0, bits);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  } else {
+    int which = 0;
+    uint64_t bits = key_bits(a, s, begin, end, lane);
+    if (begin < end) fill(smem, begin, bits);
+    for (int key0 = begin; key0 < end; key0 += BN) {
+      __syncthreads();  // waits for this wave's loads: the tile is complete, and nobody reads the other buffer any more
+      uint64_t next = 0;
+      if (key0 + BN < end) {
+        next = key_bits(a, s, key0 + BN, end, lane);
+        fill(smem + (which ^ 1) * kTile, key0 + BN, next);
+      }
+#pragma unroll
+      for (int sub = 0; sub < BN / 32; ++sub)
+        if ((unsigned)(bits >> (32 * sub))) consume(smem + which * kTile, sub, key0, bits);
+      bits = next;
+      which ^= 1;
+    }
+  }
+
+  l1 = swap_add(l1), l2 = swap_add(l2);
+  if constexpr (KEYS) {  // join the waves' partials, the upper half of them through LDS, twice
+#pragma unroll
+    for (int step = NW / 2; step >= 1; step /= 2) {
+      __syncthreads();
+      float* const box = (float*)smem + (wave % step) * 64 * (2 * NT * 16 + 4);
+      if (wave >= step && wave < 2 * step) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) box[(i * 16 + j) * 64 + lane] = acc1[i][j], box[((NT + i) * 16 + j) * 64 + lane] = acc2[i][j];
+        float* st = box + 2 * NT * 16 * 64;
+        st[lane] = m1, st[64 + lane] = m2, st[128 + lane] = l1, st[192 + lane] = l2;
+      }
+      __syncthreads();
+      if (wave < step) {
+        const float* st = box + 2 * NT * 16 * 64;
+        const float om1 = st[lane], om2 = st[64 + lane], n1 = fmaxf(m1, om1), n2 = fmaxf(m2, om2);
+        const float u1 = n1 == -INFINITY ? 0.f : n1, u2 = n2 == -INFINITY ? 0.f : n2;
+        const float c1 = __builtin_amdgcn_exp2f(m1 - u1), c2 = __builtin_amdgcn_exp2f(m2 - u2);
+        const float d1 = __builtin_amdgcn_exp2f(om1 - u1), d2 = __builtin_amdgcn_exp2f(om2 - u2);
+        l1 = l1 * c1 + st[128 + lane] * d1, l2 = l2 * c2 + st[192 + lane] * d2;
+        m1 = n1, m2 = n2;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            acc1[i][j] = acc1[i][j] * c1 + box[(i * 16 + j) * 64 + lane] * d1;
+            acc2[i][j] = acc2[i][j] * c2 + box[((NT + i) * 16 + j) * 64 + lane] * d2;
+          }
+      }
+    }
+    if (wave) return;
+  }
+
+  if (r >= rows_here * a.g) return;
+  if (!row.in) m1 = m2 = -INFINITY, l1 = l2 = 0.f;
+  const int64_t at = s.q0 + row.i;
+  const int head = kvh * a.g + row.h;
+  if (a.splits > 1) {  // unnormalised, with its maximum and sum: (split, row, head, 2, 4 + dv)
+    const int w = a.dv + 4;
+    float* p1 = a.part + (((int64_t)blockIdx.z * a.nq + at) * a.hk * a.g + head) * 2 * w;
+    float* p2 = p1 + w;
+    if (half == 0) p1[0] = m1, p1[1] = l1, p2[0] = m2, p2[1] = l2;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = 32 * i + 8 * j + 4 * half;
+        if (c < a.dv) {
+          store4<float>(p1 + 4 + c, acc1[i][4 * j], acc1[i][4 * j + 1], acc1[i][4 * j + 2], acc1[i][4 * j + 3]);
+          store4<float>(p2 + 4 + c, acc2[i][4 * j], acc2[i][4 * j + 1], acc2[i][4 * j + 2], acc2[i][4 * j + 3]);
+        }
+      }
+    return;
+  }
+  const float lam = a.lam[head];
+  const bool some = l1 != 0.f;  // false: no key (the maps share their keys), zero rows; a NaN stays one
+  const float i1 = 1.f / l1, i2 = 1.f / l2;
+  if (a.lse && half == 0) {
+    const int64_t st = stat_at(a, kvh, 0, at, row.h);
+    a.lse[st] = some ? m1 + log2f(l1) : INFINITY;
+    a.lse[st + a.nq * a.g] = some ? m2 + log2f(l2) : INFINITY;
+  }
+  T* const po = out + (at * a.hk * a.g + head) * a.dv;
+  T* const p2 = o2 ? o2 + (at * a.hk * a.g + head) * a.dv : nullptr;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 32 * i + 8 * j + 4 * half;
+      if (c < a.dv) {
+        float y[4], z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          z[e] = some ? acc2[i][4 * j + e] * i2 : 0.f;
+          y[e] = some ? fmaf(-lam, z[e], acc1[i][4 * j + e] * i1) : 0.f;
+        }
+        store4<T>(po + c, y[0], y[1], y[2], y[3]);
+        if (p2) store4<T>(p2 + c, z[0], z[1], z[2], z[3]);
+      }
+    }
+}
+
+// ---- backward: query rows (dQ, sum of P2 dP) --------------------------------------------------------------------------------------------
+// fp16: the power of two that brings the largest |dout| to [2, 4), so that dS neither underflows for the small gradients of a mean loss
+// nor overflows (|dP| < 4 Dv max|v|); 1 for the types with the exponent range of 32 bits
+template <typename T>
+struct Narrow {
+  static constexpr bool value = false;
+};
+template <>
+struct Narrow<_Float16> {
+  static constexpr bool value = true;
+};
+template <typename T>
+__device__ __forceinline__ float grad_scale(const Args& a) {
+  if constexpr (Narrow<T>::value) {
+    const float m = *a.amax;
+    if (m > 0.f && m < INFINITY) return ldexpf(1.f, 1 - ilogbf(m));
+  }
+  return 1.f;
+}
+
+template <typename T, int DB, int DVB, int NW>
+__global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
+  using Frag = typename Ops<T>::Frag;
+  constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, ND = DB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
+  constexpr int kTile = 32 * (CK + CV) * 16, TILE = 32 * NW;
+  constexpr int NB = 2 * kTile <= 131072 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) char smem[NB * kTile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+  const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
+  const int t = a.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
+  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
+  T* const dq = (T*)a.gq;
+  if (s.tile < 0) {
+    const int64_t rows = s.q_end < a.nq ? a.nq - s.q_end : 0, per = (int64_t)a.g * 2 * a.d;
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * per; e += (int64_t)s.spares * (NW * 64)) {
+      const int64_t i = e / per;
+      dq[((s.q_end + i) * a.hk + kvh) * per + (e - i * per)] = (T)0.f;
+    }
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * a.g; e += (int64_t)s.spares * (NW * 64))
+      a.drow[((int64_t)kvh * a.nq + s.q_end) * a.g + e] = 0.f;
+    return;
+  }
+  const int row_base = s.tile * TILE;
+  const int rows_here = a.stacked ? s.n : a.n;
+  if (row_base >= rows_here * a.g) return;
+  const int r = row_base + 32 * wave + col;
+  const Row row = row_of(a, s, r);
+  const int64_t at = s.q0 + row.i;
+  const int head = kvh * a.g + row.h;
+  const float gs = grad_scale<T>(a);
+
+  Frag q1[QS], q2[QS], go[VS];
+  {
+    const int i0 = row_base / a.g;
+    const auto rq = buffer((const T*)a.q.data + s.b * a.q.batch_stride + ((a.stacked ? s.q0 : 0) + i0) * a.q.row_stride +
+                           (int64_t)kvh * 2 * a.g * a.q.head_stride);
+    const auto ro = buffer((const T*)a.dout.data + s.b * a.dout.batch_stride + ((a.stacked ? s.q0 : 0) + i0) * a.dout.row_stride +
+                           (int64_t)kvh * a.g * a.dout.head_stride);
+    const int oq = (int)(((row.i - i0) * a.q.row_stride + 2 * row.h * a.q.head_stride) * (int)sizeof(T)), hs = (int)(a.q.head_stride * sizeof(T));
+    const int oo = (int)(((row.i - i0) * a.dout.row_stride + row.h * a.dout.head_stride) * (int)sizeof(T));
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      const int c = (2 * i + half) * kE<T>;
+      const bool in = row.in && c < a.d;
+      q1[i] = load_frag<T>(rq, in ? oq + c * (int)sizeof(T) : kOutside);
+      q2[i] = load_frag<T>(rq, in ? oq + hs + c * (int)sizeof(T) : kOutside);
+    }
+#pragma unroll
+    for (int i = 0; i < VS; ++i) {
+      const int c = (2 * i + half) * kE<T>;
+      go[i] = load_frag<T>(ro, row.in && c < a.dv ? oo + c * (int)sizeof(T) : kOutside);
+    }
+  }
+  float lse1 = INFINITY, lse2 = INFINITY, del1 = 0.f, del2 = 0.f, lam = 0.f;
+  if (row.in) {
+    const int64_t st = stat_at(a, kvh, 0, at, row.h);
+    lse1 = a.lse[st], lse2 = a.lse[st + a.nq * a.g], del1 = a.del[st], del2 = a.del[st + a.nq * a.g], lam = a.lam[head];
+  }
+  const bool huge = __any((fabsf(lse1) > kHuge && lse1 < INFINITY) || (fabsf(lse2) > kHuge && lse2 < INFINITY));
+  f32x16 acc1[ND], acc2[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc1[i] = zero16(), acc2[i] = zero16();
+  float dsum = 0.f;
+
+  const T* const kp = (const T*)a.k.data + s.b * a.k.batch_stride + (a.stacked ? s.k0 : 0) * a.k.row_stride + (int64_t)kvh * 2 * a.k.head_stride;
+  const T* const vp = (const T*)a.v.data + s.b * a.v.batch_stride + (a.stacked ? s.k0 : 0) * a.v.row_stride + (int64_t)kvh * a.v.head_stride;
+  const int off = s.m - s.n;
+  const int limit = a.causal ? row.i + off : 0x7fffffff;
+  int end = s.m;
+  if (a.causal) {
+    const int last = min(row_base + TILE, s.n * a.g) - 1;
+    end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
+  }
+  auto fill = [&](char* tile, int key0, uint64_t bits) {
+    const auto rk = buffer(kp + (int64_t)key0 * a.k.row_stride);
+    const auto rv = buffer(vp + (int64_t)key0 * a.v.row_stride);
+    const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
+    stage<T, 32, 2, DB, NW>(tile, rk, a.d, (int)(a.k.head_stride * sizeof(T)), wave, lane,
+                        [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
+    stage<T, 32, 1, DVB, NW>(tile + 32 * CK * 16, rv, a.dv, 0, wave, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
+  };
+  auto consume = [&](const char* tile, int key0, uint64_t bits) {
+    const char* vt = tile + 32 * CK * 16;
+    f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      Ops<T>::mma(s1, row_frag<T, CK>(tile, col, 2 * i + half), q1[i]);
+      Ops<T>::mma(s2, row_frag<T, CK>(tile, col, CK / 2 + 2 * i + half), q2[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, row_frag<T, CV>(vt, col, 2 * i + half), go[i]);
+    unsigned lo = (unsigned)bits;
+    const int above = limit - key0;
+    if (above < 31) lo = above < 0 ? 0u : lo & ((2u << above) - 1);
+    const bool some = __any(lo != 0xffffffffu);
+    lo >>= 4 * half;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float p1 = __builtin_amdgcn_exp2f(exponent(s1[i], a.scale_log2, lse1, huge));
+      float p2 = __builtin_amdgcn_exp2f(exponent(s2[i], a.scale_log2, lse2, huge));
+      if (some) {
+        const bool in = (lo >> (8 * (i / 4) + i % 4)) & 1;
+        p1 = in ? p1 : 0.f, p2 = in ? p2 : 0.f;
+      }
+      dsum = fmaf(p2, dp[i], dsum);
+      s1[i] = p1 * (dp[i] - del1), s2[i] = -lam * p2 * (dp[i] - del2);
+      if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs;
+    }
+#pragma unroll
+    for (int p = 0; p < kPSteps<T>; ++p) {
+      const Frag d1 = pack<T>(s1, p), d2 = pack<T>(s2, p);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        Ops<T>::mma(acc1[i], col_frag<T, CK>(tile, 0, p, 32 * i, lane), d1);
+        Ops<T>::mma(acc2[i], col_frag<T, CK>(tile, 0, p, DB + 32 * i, lane), d2);
+      }
+    }
+  };
+  if constexpr (NB == 2) {
+    int which = 0;
+    uint64_t bits = key_bits(a, s, 0, end, lane) & 0xffffffffull;
+    if (0 < end) fill(smem, 0, bits);
+    for (int key0 = 0; key0 < end; key0 += 32) {
+      __syncthreads();
+      uint64_t next = 0;
+      if (key0 + 32 < end) {
+        next = key_bits(a, s, key0 + 32, end, lane) & 0xffffffffull;
+        fill(smem + (which ^ 1) * kTile, key0 + 32, next);
+      }
+      if (bits) consume(smem + which * kTile, key0, bits);
+      bits = next;
+      which ^= 1;
+    }
+  } else {
+    for (int key0 = 0; key0 < end; key0 += 32) {
+      const uint64_t bits = key_bits(a, s, key0, end, lane) & 0xffffffffull;
+      if (!bits) continue;
+      __syncthreads();
+      fill(smem, key0, bits);
+      __syncthreads();
+      consume(smem, key0, bits);
+    }
+  }
+  if (r >= rows_here * a.g) return;
+  dsum = swap_add(dsum);
+  if (!row.in) dsum = 0.f;
+  if (half == 0) a.drow[((int64_t)kvh * a.nq + at) * a.g + row.h] = dsum;
+  const float f = a.scale / gs;
+  T* const p1 = dq + (at * a.hk * a.g + head) * 2 * a.d;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 32 * i + 8 * j + 4 * half;
+      if (c < a.d) {
+        if (row.in) {
+          store4<T>(p1 + c, acc1[i][4 * j] * f, acc1[i][4 * j + 1] * f, acc1[i][4 * j + 2] * f, acc1[i][4 * j + 3] * f);
+          store4<T>(p1 + a.d + c, acc2[i][4 * j] * f, acc2[i][4 * j + 1] * f, acc2[i][4 * j + 2] * f, acc2[i][4 * j + 3] * f);
+        } else {
+          store4<T>(p1 + c, 0.f, 0.f, 0.f, 0.f);
+          store4<T>(p1 + a.d + c, 0.f, 0.f, 0.f, 0.f);
+        }
+      }
+    }
+}
+
+// ---- backward: keys (dK, dV) --------------------------------------------------------------------------------------------------------------
+// A wave owns 32 keys; K and V are the B operands (lane = key), in registers where they fit beside the accumulators (16-bit types), else
+// read again from memory for every tile of 32 packed query rows (32-bit: a product takes 16 times as long as its operand's load).
+template <typename T, int DB, int DVB, int NW>
+__global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
+  using Frag = typename Ops<T>::Frag;
+  constexpr int CQ = 2 * DB * (int)sizeof(T) / 16, CO = DVB * (int)sizeof(T) / 16, ND = DB / 32, NV = DVB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
+  constexpr bool kHold = sizeof(T) == 2;
+  constexpr int kStats = 32 * 6 * 4 + 16;  // lse1, lse2, del1, del2, lam, limit of a tile's rows; whether a score is huge
+  constexpr int kTile = 32 * (CQ + CO) * 16, TILE = 32 * NW;
+  __shared__ __attribute__((aligned(1024))) char smem[kTile + kStats];
+  float* const st = (float*)(smem + kTile);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+  const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
+  const Seq s = find_seq<TILE, true>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
+  T* const dk = (T*)a.gk;
+  T* const dv = (T*)a.gv;
+  if (s.tile < 0) {
+    const int64_t rows = s.k_end < a.nk ? a.nk - s.k_end : 0;
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * (2 * a.d); e += (int64_t)s.spares * (NW * 64)) {
+      const int64_t i = e / (2 * a.d);
+      dk[((s.k_end + i) * a.hk + kvh) * 2 * a.d + (e - i * 2 * a.d)] = (T)0.f;
+    }
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * a.dv; e += (int64_t)s.spares * (NW * 64)) {
+      const int64_t i = e / a.dv;
+      dv[((s.k_end + i) * a.hk + kvh) * a.dv + (e - i * a.dv)] = (T)0.f;
+    }
+    return;
+  }
+  const int key_base = s.tile * TILE;
+  const int keys_here = a.stacked ? s.m : a.m;
+  if (key_base >= keys_here) return;
+  const int key = key_base + 32 * wave + col;
+  const bool in = key < s.m && !(a.masks && a.masks[s.k0 + key]);
+  const float gs = grad_scale<T>(a);
+  constexpr float kBoost = Narrow<T>::value ? 256.f : 1.f;  // fp16: P 2^8 in the product with dout, the weights of a long row stay normal numbers
+
+  const auto rk = buffer((const T*)a.k.data + s.b * a.k.batch_stride + ((a.stacked ? s.k0 : 0) + key_base) * a.k.row_stride +
+                         (int64_t)kvh * 2 * a.k.head_stride);
+  const auto rv = buffer((const T*)a.v.data + s.b * a.v.batch_stride + ((a.stacked ? s.k0 : 0) + key_base) * a.v.row_stride +
+                         (int64_t)kvh * a.v.head_stride);
+  const int ok = (int)((32 * wave + col) * a.k.row_stride * (int)sizeof(T)), hs = (int)(a.k.head_stride * sizeof(T));
+  const int ov = (int)((32 * wave + col) * a.v.row_stride * (int)sizeof(T));
+  auto k_frag = [&](int map, int i) {
+    const int c = (2 * i + half) * kE<T>;
+    return load_frag<T>(rk, in && c < a.d ? ok + map * hs + c * (int)sizeof(T) : kOutside);
+  };
+  auto v_frag = [&](int i) {
+    const int c = (2 * i + half) * kE<T>;
+    return load_frag<T>(rv, in && c < a.dv ? ov + c * (int)sizeof(T) : kOutside);
+  };
+  Frag k1[kHold ? QS : 1], k2[kHold ? QS : 1], vv[kHold ? VS : 1];
+  if constexpr (kHold) {
+#pragma unroll
+    for (int i = 0; i < QS; ++i) k1[i] = k_frag(0, i), k2[i] = k_frag(1, i);
+#pragma unroll
+    for (int i = 0; i < VS; ++i) vv[i] = v_frag(i);
+  }
+  f32x16 ak1[ND], ak2[ND], av[NV];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) ak1[i] = zero16(), ak2[i] = zero16();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) av[i] = zero16();
+
+  const int off = s.m - s.n;
+  const int rows = s.n * a.g;
+  int first = 0;
+  if (a.causal) first = min(s.n, max(0, key_base - off)) * a.g / 32 * 32;  // rows before see none of these keys
+  const T* const qp = (const T*)a.q.data + s.b * a.q.batch_stride + (a.stacked ? s.q0 : 0) * a.q.row_stride + (int64_t)kvh * 2 * a.g * a.q.head_stride;
+  const T* const op = (const T*)a.dout.data + s.b * a.dout.batch_stride + (a.stacked ? s.q0 : 0) * a.dout.row_stride +
+                      (int64_t)kvh * a.g * a.dout.head_stride;
+  for (int r0 = first; r0 < rows; r0 += 32) {
+    __syncthreads();
+    const int i0 = a.g == 1 ? r0 : r0 / a.g;
+    const auto rq = buffer(qp + (int64_t)i0 * a.q.row_stride);
+    const auto ro = buffer(op + (int64_t)i0 * a.dout.row_stride);
+    auto q_off = [&](int x, int64_t rs, int64_t hstr) {
+      const int r = r0 + x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
+      return r < rows ? (int)(((i - i0) * rs + h * hstr) * (int)sizeof(T)) : kOutside;
+    };
+    stage<T, 32, 2, DB, NW>(smem, rq, a.d, (int)(a.q.head_stride * sizeof(T)), wave, lane,
+                        [&](int x) { return q_off(x, a.q.row_stride, 2 * a.q.head_stride); });
+    stage<T, 32, 1, DVB, NW>(smem + 32 * CQ * 16, ro, a.dv, 0, wave, lane,
+                         [&](int x) { return q_off(x, a.dout.row_stride, a.dout.head_stride); });
+    if (threadIdx.x < 32) {
+      const int r = r0 + threadIdx.x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
+      const bool there = r < rows;
+      const int64_t p = stat_at(a, kvh, 0, s.q0 + i, h);
+      const float e1 = there ? a.lse[p] : INFINITY, e2 = there ? a.lse[p + a.nq * a.g] : INFINITY;
+      st[threadIdx.x] = e1, st[32 + threadIdx.x] = e2;
+      const bool big = __any((fabsf(e1) > kHuge && e1 < INFINITY) || (fabsf(e2) > kHuge && e2 < INFINITY));
+      if (threadIdx.x == 0) ((int*)st)[192] = big;
+      st[64 + threadIdx.x] = there ? a.del[p] : 0.f;
+      st[96 + threadIdx.x] = there ? a.del[p + a.nq * a.g] : 0.f;
+      st[128 + threadIdx.x] = there ? a.lam[kvh * a.g + h] : 0.f;
+      ((int*)st)[160 + threadIdx.x] = a.causal ? i + off : 0x7fffffff;
+    }
+    __syncthreads();
+    const char* ot = smem + 32 * CQ * 16;
+    f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      Ops<T>::mma(s1, row_frag<T, CQ>(smem, col, 2 * i + half), kHold ? k1[i % (kHold ? QS : 1)] : k_frag(0, i));
+      Ops<T>::mma(s2, row_frag<T, CQ>(smem, col, CQ / 2 + 2 * i + half), kHold ? k2[i % (kHold ? QS : 1)] : k_frag(1, i));
+    }
+#pragma unroll
+    for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, row_frag<T, CO>(ot, col, 2 * i + half), kHold ? vv[i % (kHold ? VS : 1)] : v_frag(i));
+    const bool huge = __builtin_amdgcn_readfirstlane(((const int*)st)[192]) != 0;
+    f32x16 pj;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int x = 8 * j + 4 * half;
+      const f32x4 e1 = *(const f32x4*)(st + x), e2 = *(const f32x4*)(st + 32 + x), d1 = *(const f32x4*)(st + 64 + x),
+                  d2 = *(const f32x4*)(st + 96 + x), lm = *(const f32x4*)(st + 128 + x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * j + e;
+        float p1 = __builtin_amdgcn_exp2f(exponent(s1[i], a.scale_log2, e1[e], huge));
+        float p2 = __builtin_amdgcn_exp2f(exponent(s2[i], a.scale_log2, e2[e], huge));
+        if (a.causal && key > ((const int*)st)[160 + x + e]) p1 = 0.f, p2 = 0.f;
+        pj[i] = fmaf(-lm[e], p2, p1) * kBoost;
+        s1[i] = p1 * (dp[i] - d1[e]), s2[i] = -lm[e] * p2 * (dp[i] - d2[e]);
+        if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPSteps<T>; ++p) {
+      const Frag fp = pack<T>(pj, p), f1 = pack<T>(s1, p), f2 = pack<T>(s2, p);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) Ops<T>::mma(av[i], col_frag<T, CO>(ot, 0, p, 32 * i, lane), fp);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        Ops<T>::mma(ak1[i], col_frag<T, CQ>(smem, 0, p, 32 * i, lane), f1);
+        Ops<T>::mma(ak2[i], col_frag<T, CQ>(smem, 0, p, DB + 32 * i, lane), f2);
+      }
+    }
+  }
+  if (key >= keys_here) return;
+  const float fk = a.scale / gs, fv = 1.f / kBoost;
+  const int64_t at = s.k0 + key;
+  T* const pk = dk + (at * a.hk + kvh) * 2 * a.d;
+  T* const pv = dv + (at * a.hk + kvh) * a.dv;
+  // a key that is masked or does not exist: zero, whatever its lane accumulated
+  auto out4 = [&](T* p, const f32x16& x, int j, float f) {
+    if (in) store4<T>(p, x[4 * j] * f, x[4 * j + 1] * f, x[4 * j + 2] * f, x[4 * j + 3] * f);
+    else store4<T>(p, 0.f, 0.f, 0.f, 0.f);
+  };
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const int c = 32 * i + 8 * j + 4 * half;
+      if (c < a.d) out4(pk + c, ak1[i], j, fk), out4(pk + a.d + c, ak2[i], j, fk);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 32 * i + 8 * j + 4 * half;
+      if (c < a.dv) out4(pv + c, av[i], j, fv);
+    }
+  }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------------------------------
+enum Which { kForward, kForwardKeys, kBackwardQ, kBackwardKV };
+
+// stack mode: every sequence may end inside a tile, and one block more takes the rows behind the last
+inline int64_t tiles_of(const Args& a, bool keys, int tile) {
+  const int64_t rows = keys ? (a.stacked ? a.nk : a.m) : (a.stacked ? a.nq : a.n) * (int64_t)a.g;
+  return (rows + tile - 1) / tile + (a.stacked ? a.batch + 1 : 0);
+}
+
+template <typename T, int DB, int DVB>
+int launch_dims(const Args& a, Which which, hipStream_t s) {
+  constexpr int NWK = 32 * (2 * DB + DVB) * (int)sizeof(T) * 4 <= 131072 ? 4 : 2;  // KEYS: a tile for every wave
+  const bool fwd = which == kForward || which == kForwardKeys;
+  const int64_t tiles = tiles_of(a, which == kBackwardKV, which == kForwardKeys ? 32 : 128), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
+  if (tiles == 0 || x == 0) return GEOTR_OK;
+  if (tiles > 65535 || x > 0x7fffffff) return fail(GEOTR_E_INVALID, "differential attention: %lld tiles of rows in one call", (long long)tiles);
+  const dim3 grid((unsigned)x, (unsigned)tiles, fwd ? (unsigned)a.splits : 1u);
+  if (which == kForward) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, 4, false>), grid, dim3(256), 0, s, a);
+  else if (which == kForwardKeys) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, NWK, true>), grid, dim3(64 * NWK), 0, s, a);
+  else if (which == kBackwardQ) hipLaunchKernelGGL((dq_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
+  GEOTR_CHECK_LAUNCH("differential attention");
+  return GEOTR_OK;
+}
+
+// head dimensions: the next of 32, 64, 128 for q and k; one or two times that for v
+template <typename T>
+int launch_type(const Args& a, Which which, hipStream_t s) {
+  if (a.d <= 32 && a.dv <= 32) return launch_dims<T, 32, 32>(a, which, s);
+  if (a.d <= 32 && a.dv <= 64) return launch_dims<T, 32, 64>(a, which, s);
+  if (a.d <= 64 && a.dv <= 64) return launch_dims<T, 64, 64>(a, which, s);
+  if (a.d <= 64 && a.dv <= 128) return launch_dims<T, 64, 128>(a, which, s);
+  if (a.d <= 128 && a.dv <= 128) return launch_dims<T, 128, 128>(a, which, s);
+  return launch_dims<T, 128, 256>(a, which, s);
+}
+
+int launch_f32(const Args& a, Which which, hipStream_t s);
+int launch_bf16(const Args& a, Which which, hipStream_t s);
+int launch_f16(const Args& a, Which which, hipStream_t s);
+
+}  // namespace dattn
+}  // namespace geotr

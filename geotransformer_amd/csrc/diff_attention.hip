@@ -1,0 +1,272 @@
+// diff_attention.hip -- entry points of the differential attention (include/geotr.h) and its small kernels: joining the partials of keys
+// dealt over several blocks, del = dout . output of each map, and the gradient of lam.  The matrix work is in diff_attention.h.
+#include <algorithm>
+
+#include "diff_attention.h"
+
+namespace geotr {
+namespace dattn {
+namespace {
+
+constexpr int kMostSplits = 64;  // the join holds one split per lane
+
+// One wave per (row, head): maxima and sums of the splits in the lanes, channels over the lanes.  Bound: HBM / latency.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  const int lane = threadIdx.x & 63, heads = a.hk * a.g;
+  const int64_t e = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (e >= a.nq * heads) return;
+  const int64_t row = e / heads;
+  const int head = (int)(e - row * heads), w = a.dv + 4;
+  const int64_t step = a.nq * heads * 2 * (int64_t)w;
+  const float* p = a.part + e * 2 * w;
+  float m[2], l[2], f[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    m[x] = lane < a.splits ? p[lane * step + x * w] : -INFINITY;
+    l[x] = lane < a.splits ? p[lane * step + x * w + 1] : 0.f;
+    float top = m[x];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    f[x] = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[x] - top);
+    float sum = l[x] * f[x];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    m[x] = top, l[x] = sum;
+  }
+  const bool some = l[0] != 0.f;
+  const float lam = a.lam[head];
+  for (int c = lane; c < a.dv; c += 64) {
+    float y = 0.f, z = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const float f1 = __shfl(f[0], s, 64), f2 = __shfl(f[1], s, 64);
+      const float* q = p + s * step + 4 + c;
+      if (f1 != 0.f) y = fmaf(q[0], f1, y);
+      if (f2 != 0.f) z = fmaf(q[w], f2, z);
+    }
+    z = some ? z / l[1] : 0.f;
+    y = some ? fmaf(-lam, z, y / l[0]) : 0.f;
+    ((T*)a.out)[e * a.dv + c] = (T)y;
+    if (a.o2) ((T*)a.o2)[e * a.dv + c] = (T)z;
+  }
+  if (a.lse && lane < 2) {
+    const int kvh = head / a.g;
+    a.lse[stat_at(a, kvh, lane, row, head - kvh * a.g)] = some ? (lane ? m[1] + log2f(l[1]) : m[0] + log2f(l[0])) : INFINITY;
+  }
+}
+
+// del_2 = dout . O2, del_1 = dout . O1 = dout . out + lam del_2; 16 lanes per (row, head).  fp16: the largest |dout| of the rows that
+// exist (an order-free maximum).  Bound: HBM.
+template <typename T>
+__global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
+  using Frag = typename Ops<T>::Frag;
+  const int lane = threadIdx.x & 63, heads = a.hk * a.g, c0 = lane & 15;
+  const int64_t e = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
+  const bool in = e < a.nq * heads;
+  float x = 0.f, z = 0.f, top = 0.f;
+  const int64_t row = in ? e / heads : 0;
+  const int head = in ? (int)(e - row * heads) : 0;
+  if (in) {
+    const int64_t b = a.stacked ? 0 : row / a.n, i = a.stacked ? row : row - b * a.n;
+    const T* g = (const T*)a.dout.data + b * a.dout.batch_stride + i * a.dout.row_stride + head * a.dout.head_stride;
+    const T* y = (const T*)a.out + e * a.dv;
+    const T* y2 = (const T*)a.o2 + e * a.dv;
+    for (int c = c0 * kE<T>; c < a.dv; c += 16 * kE<T>) {
+      const Frag fg = *(const Frag*)(g + c), fy = *(const Frag*)(y + c), f2 = *(const Frag*)(y2 + c);
+#pragma unroll
+      for (int j = 0; j < kE<T>; ++j) {
+        x = fmaf((float)fg[j], (float)fy[j], x), z = fmaf((float)fg[j], (float)f2[j], z);
+        if constexpr (Narrow<T>::value) top = fmaxf(top, fabsf((float)fg[j]));
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) x += __shfl_xor(x, o, 64), z += __shfl_xor(z, o, 64);
+  if (in && c0 == 0) {
+    const int kvh = head / a.g;
+    const int64_t at = stat_at(a, kvh, 0, row, head - kvh * a.g);
+    a.del[at] = fmaf(a.lam[head], z, x), a.del[at + a.nq * a.g] = z;
+  }
+  if constexpr (Narrow<T>::value) {
+    if (a.q_len) {  // gradients of rows that do not exist say nothing
+      if (a.stacked) {
+        int64_t end = 0;
+        for (int b = lane; b < a.batch; b += 64) end += clamp_len(a.q_len[b], a.nq);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) end += __shfl_xor(end, o, 64);
+        if (row >= end) top = 0.f;
+      } else if (in && row % a.n >= a.q_len[row / a.n]) {
+        top = 0.f;
+      }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (lane == 0 && top > 0.f) atomicMax((int*)amax, __float_as_int(top));
+  }
+}
+
+// dlam_h = - sum over rows, in a fixed order: 1 024 partial sums in 64 bits, then a tree
+__global__ __launch_bounds__(1024) void dlam_kernel(const float* drow, int64_t nq, int g, float* dlam) {
+  __shared__ double box[1024];
+  const int kvh = blockIdx.x / g, h = blockIdx.x - kvh * g;
+  const float* p = drow + (int64_t)kvh * nq * g + h;
+  double s = 0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < nq; i += 1024) s += (double)p[i * g];
+  box[threadIdx.x] = s;
+  for (int o = 512; o; o >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < o) box[threadIdx.x] += box[threadIdx.x + o];
+  }
+  if (threadIdx.x == 0) dlam[blockIdx.x] = (float)-box[0];
+}
+
+int launch(int dtype, const Args& a, Which which, hipStream_t s) {
+  return dtype == GEOTR_F32 ? launch_f32(a, which, s) : dtype == GEOTR_BF16 ? launch_bf16(a, which, s) : launch_f16(a, which, s);
+}
+
+int check_view(const geotr_heads& v, int64_t heads, int size, int64_t batch, int64_t rows, const char* what) {
+  GEOTR_CHECK_ARG(v.heads == heads, "differential attention: %s has %lld heads, expected %lld", what, (long long)v.heads, (long long)heads);
+  if (batch * rows == 0) return GEOTR_OK;
+  GEOTR_CHECK_ARG(v.data, "differential attention: %s is a null pointer", what);
+  const int e = 16 / size;
+  GEOTR_CHECK_ARG((uintptr_t)v.data % 16 == 0 && v.batch_stride % e == 0 && v.row_stride % e == 0 && v.head_stride % e == 0,
+                  "differential attention: %s is not a 16-byte aligned view", what);
+  // a tile of 128 rows is addressed by 32-bit offsets from its first row, below the 1 GiB a buffer descriptor here covers
+  GEOTR_CHECK_ARG(v.row_stride >= 0 && v.head_stride >= 0 && (128 * v.row_stride + 128 * v.head_stride + 512) * size < kNumRecords,
+                  "differential attention: strides of %s (rows %lld, heads %lld elements)", what, (long long)v.row_stride, (long long)v.head_stride);
+  return GEOTR_OK;
+}
+
+int make_args(const geotr_diff_attn* op, Args& a) {
+  GEOTR_CHECK_ARG(op, "differential attention: null descriptor");
+  GEOTR_CHECK_ARG(op->dtype >= GEOTR_F32 && op->dtype <= GEOTR_F16, "differential attention: unknown dtype %d", op->dtype);
+  GEOTR_CHECK_ARG(op->batch >= 0 && op->n >= 0 && op->m >= 0 && op->batch <= (1 << 20), "differential attention: batch %lld, rows %lld and %lld",
+                  (long long)op->batch, (long long)op->n, (long long)op->m);
+  GEOTR_CHECK_ARG(op->dim >= 8 && op->dim <= 128 && op->dim % 8 == 0 && op->v_dim >= 8 && op->v_dim <= 256 && op->v_dim % 8 == 0,
+                  "differential attention: head dimensions %lld and %lld (multiples of 8 up to 128 and 256)", (long long)op->dim, (long long)op->v_dim);
+  const int64_t hk = op->v.heads, h = op->q.heads / 2;
+  GEOTR_CHECK_ARG(hk >= 1 && h >= hk && h % hk == 0 && op->q.heads % 2 == 0 && h / hk <= 64 && hk <= 65535,
+                  "differential attention: %lld query, %lld key and %lld value heads", (long long)op->q.heads, (long long)op->k.heads, (long long)hk);
+  GEOTR_CHECK_ARG(op->scale > 0.f && op->scale < 1e30f, "differential attention: scale %g", (double)op->scale);
+  GEOTR_CHECK_ARG(op->lam, "differential attention: lam is a null pointer");
+  GEOTR_CHECK_ARG(!op->stacked || (op->q_lengths && op->k_lengths), "differential attention: stack mode needs both lengths");
+  const int size = op->dtype == GEOTR_F32 ? 4 : 2;
+  const int64_t g = h / hk;
+  a.nq = op->stacked ? op->n : op->batch * op->n, a.nk = op->stacked ? op->m : op->batch * op->m;
+  GEOTR_CHECK_ARG(a.nq * g <= kMostRows && a.nk <= kMostRows, "differential attention: %lld query rows (x %lld heads) and %lld keys in one call",
+                  (long long)a.nq, (long long)g, (long long)a.nk);
+  int rc;
+  if ((rc = check_view(op->q, 2 * h, size, op->batch, op->n, "q")) || (rc = check_view(op->k, 2 * hk, size, op->batch, op->m, "k")) ||
+      (rc = check_view(op->v, hk, size, op->batch, op->m, "v")))
+    return rc;
+  a.q = op->q, a.k = op->k, a.v = op->v, a.dout = geotr_heads{nullptr, 0, 0, 0, 0};
+  a.out = a.o2 = a.gq = a.gk = a.gv = nullptr, a.lse = a.del = a.part = a.drow = nullptr, a.amax = nullptr;
+  a.lam = op->lam, a.q_len = op->q_lengths, a.k_len = op->k_lengths, a.masks = op->key_masks;
+  a.batch = (int)op->batch, a.stacked = op->stacked != 0, a.n = (int)op->n, a.m = (int)op->m;
+  a.hk = (int)hk, a.g = (int)g, a.d = (int)op->dim, a.dv = (int)op->v_dim, a.causal = op->causal != 0, a.splits = 1;
+  a.scale = op->scale, a.scale_log2 = (float)((double)op->scale * 1.4426950408889634);
+  return GEOTR_OK;
+}
+
+// Few rows to a sequence (32 packed rows or less): blocks of one 32-row tile whose waves stream keys of their own.  Keys are dealt over
+// blocks until there are two for each compute unit, as long as every block keeps 256 keys.
+bool keys_form(const Args& a) {
+  const int64_t rows = a.stacked ? (a.nq + a.batch - 1) / std::max(a.batch, 1) : a.n;
+  return rows * a.g <= 32;
+}
+int choose_splits(const Args& a) {
+  const int64_t per = a.stacked ? a.nk / std::max(a.batch, 1) : a.m, seqs = std::max(a.batch, 1);
+  const int64_t rows = (a.stacked ? (a.nq + seqs - 1) / seqs : a.n) * a.g, tile = keys_form(a) ? 32 : 128;
+  const int64_t blocks = seqs * a.hk * std::max<int64_t>(1, (rows + tile - 1) / tile);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kMostSplits, 512 / blocks, per / 256}));
+}
+size_t part_bytes(const Args& a, int splits) {
+  return splits > 1 ? align_up((size_t)splits * a.nq * a.hk * a.g * 2 * (a.dv + 4) * sizeof(float)) : 0;
+}
+
+}  // namespace
+}  // namespace dattn
+}  // namespace geotr
+
+using namespace geotr;
+using namespace geotr::dattn;
+
+extern "C" {
+
+size_t geotr_diff_attn_workspace_bytes(const geotr_diff_attn* op) {
+  Args a;
+  if (make_args(op, a) != GEOTR_OK) return 0;
+  return part_bytes(a, choose_splits(a));
+}
+
+int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, void* out2, float* lse, void* ws, size_t ws_bytes, void* stream) {
+  Args a;
+  const int rc = make_args(op, a);
+  if (rc != GEOTR_OK) return rc;
+  if (a.nq == 0) return GEOTR_OK;
+  GEOTR_CHECK_ARG(out, "geotr_diff_attn_forward: out is a null pointer");
+  GEOTR_CHECK_ARG(!out2 == !lse, "geotr_diff_attn_forward: out2 and lse go together");
+  GEOTR_CHECK_ARG((uintptr_t)out % 16 == 0 && (uintptr_t)out2 % 16 == 0, "geotr_diff_attn_forward: results are not 16-byte aligned");
+  a.out = out, a.o2 = out2, a.lse = lse, a.splits = choose_splits(a);
+  const size_t need = part_bytes(a, a.splits);
+  if (need) {
+    if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_forward: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    a.part = (float*)ws;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  if (const int r = launch(op->dtype, a, keys_form(a) ? kForwardKeys : kForward, s)) return r;
+  if (a.splits > 1) {
+    const dim3 grid((unsigned)((a.nq * a.hk * a.g + 3) / 4));
+    if (op->dtype == GEOTR_F32) hipLaunchKernelGGL((join_kernel<float>), grid, dim3(256), 0, s, a);
+    else if (op->dtype == GEOTR_BF16) hipLaunchKernelGGL((join_kernel<__bf16>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((join_kernel<_Float16>), grid, dim3(256), 0, s, a);
+    GEOTR_CHECK_LAUNCH("geotr_diff_attn_forward");
+  }
+  return GEOTR_OK;
+}
+
+size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op) {
+  Args a;
+  if (make_args(op, a) != GEOTR_OK) return 0;
+  const size_t rows = (size_t)a.nq * a.hk * a.g;
+  return align_up(2 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(sizeof(float));
+}
+
+int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const void* out, const void* out2, const float* lse,
+                             void* dq, void* dk, void* dv, float* dlam, void* ws, size_t ws_bytes, void* stream) {
+  Args a;
+  const int rc = make_args(op, a);
+  if (rc != GEOTR_OK) return rc;
+  GEOTR_CHECK_ARG(dout && dlam, "geotr_diff_attn_backward: null pointer");
+  const int size = op->dtype == GEOTR_F32 ? 4 : 2;
+  if (const int r = check_view(*dout, (int64_t)a.hk * a.g, size, op->batch, op->n, "dout")) return r;
+  GEOTR_CHECK_ARG((a.nq == 0 || (out && out2 && lse && dq)) && (a.nk == 0 || (dk && dv)), "geotr_diff_attn_backward: null pointer");
+  GEOTR_CHECK_ARG((uintptr_t)out % 16 == 0 && (uintptr_t)out2 % 16 == 0 && (uintptr_t)dq % 16 == 0 && (uintptr_t)dk % 16 == 0 && (uintptr_t)dv % 16 == 0,
+                  "geotr_diff_attn_backward: results are not 16-byte aligned");
+  const size_t rows = (size_t)a.nq * a.hk * a.g, need = geotr_diff_attn_backward_workspace_bytes(op);
+  if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  Carver c(ws);
+  a.del = c.take<float>(2 * rows), a.drow = c.take<float>(rows);
+  float* amax = c.take<float>(1);
+  a.dout = *dout, a.out = const_cast<void*>(out), a.o2 = const_cast<void*>(out2), a.lse = const_cast<float*>(lse);
+  a.gq = dq, a.gk = dk, a.gv = dv, a.amax = amax;
+  hipStream_t s = (hipStream_t)stream;
+  if (op->dtype == GEOTR_F16)
+    if (const int r = zero_async(amax, sizeof(float), s)) return r;
+  if (a.nq) {
+    const dim3 grid((unsigned)((rows + 15) / 16));
+    if (op->dtype == GEOTR_F32) hipLaunchKernelGGL((del_kernel<float>), grid, dim3(256), 0, s, a, amax);
+    else if (op->dtype == GEOTR_BF16) hipLaunchKernelGGL((del_kernel<__bf16>), grid, dim3(256), 0, s, a, amax);
+    else hipLaunchKernelGGL((del_kernel<_Float16>), grid, dim3(256), 0, s, a, amax);
+    GEOTR_CHECK_LAUNCH("geotr_diff_attn_backward");
+    if (const int r = launch(op->dtype, a, kBackwardQ, s)) return r;
+  }
+  if (a.nk)
+    if (const int r = launch(op->dtype, a, kBackwardKV, s)) return r;
+  hipLaunchKernelGGL(dlam_kernel, dim3((unsigned)(a.hk * a.g)), dim3(1024), 0, s, a.drow, a.nq, a.g, dlam);
+  GEOTR_CHECK_LAUNCH("geotr_diff_attn_backward");
+  return GEOTR_OK;
+}
+
+}  // extern "C"

@@ -763,3 +763,172 @@ def node_correspondences(ref_nodes, src_nodes, ref_knn_points, src_knn_points, t
         float(pos_radius), _lib.ptr(ref_masks), _lib.ptr(src_masks), _lib.ptr(ref_knn_masks), _lib.ptr(src_knn_masks), m, n, k,
         _lib.ptr(idx), _lib.ptr(ov), _lib.ptr(count), _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), 'geotr_node_correspondences')
     return idx, ov, count
+
+
+# ---- rotary positions and differential attention: (rows, heads, channels) in stack mode, (batch, rows, heads, channels) in batches --------
+class Heads(ctypes.Structure):  # geotr_heads
+    _fields_ = [('data', ctypes.c_void_p), ('heads', ctypes.c_int64), ('batch_stride', ctypes.c_int64), ('row_stride', ctypes.c_int64),
+                ('head_stride', ctypes.c_int64)]
+
+
+class DiffAttn(ctypes.Structure):  # geotr_diff_attn
+    _fields_ = [('q', Heads), ('k', Heads), ('v', Heads), ('dtype', ctypes.c_int32), ('stacked', ctypes.c_int32), ('causal', ctypes.c_int32),
+                ('pad_', ctypes.c_int32), ('batch', ctypes.c_int64), ('n', ctypes.c_int64), ('m', ctypes.c_int64), ('dim', ctypes.c_int64),
+                ('v_dim', ctypes.c_int64), ('lam', ctypes.c_void_p), ('q_lengths', ctypes.c_void_p), ('k_lengths', ctypes.c_void_p),
+                ('key_masks', ctypes.c_void_p), ('scale', ctypes.c_float), ('pad2_', ctypes.c_int32)]
+
+
+HEAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+
+
+def _heads(t):
+    """geotr_heads of a (rows, heads, channels) or (batch, rows, heads, channels) tensor whose channels are contiguous; the stride of a
+    dimension of one element says nothing and is passed as 0."""
+    if t is None:
+        return Heads(None, 0, 0, 0, 0)
+    size, stride = t.shape[-3:], [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+    return Heads(t.data_ptr(), size[1], stride[0] if t.dim() == 4 else 0, stride[-3], stride[-2])
+
+
+def _same_device(*tensors):
+    """The one device of all given tensors; RuntimeError when it is not a GPU."""
+    device = next(t for t in tensors if t is not None).device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f'all tensors of a call live on one device: {t.device} and {device}')
+    if device.type != 'cuda':
+        raise RuntimeError('geotransformer_amd needs device tensors (MI355X / gfx950); no CPU fallback exists.')
+    return device
+
+
+def check_rotary_heads(q, k):
+    """Refuses heads that geotr_rotary does not turn, with the reason."""
+    if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
+        raise ValueError('heads are (rows, heads, channels) or (batch, rows, heads, channels), q and k of the same rows and channels: got '
+                         f'{tuple(q.shape)} and {None if k is None else tuple(k.shape)}')
+    if q.dtype not in HEAD_TYPES or (k is not None and k.dtype != q.dtype):
+        raise TypeError(f'heads are float32, bfloat16 or float16, all of one type: got {q.dtype} and {None if k is None else k.dtype}')
+
+
+def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0, inverse=False):
+    """(q, k) with the first rotary_dim channels of every head turned by their token's position (geotr_rotary); k may be None.
+    positions: (rows,) / (batch, rows) or with a last dimension of axes; turns (rotary_dim / 2) float64: turns per unit of position;
+    axis (rotary_dim / 2) int32: the axis of each pair.  inverse: the transposed rotation (the gradient)."""
+    check_rotary_heads(q, k)
+    if rotary_dim % 2 or not 2 <= rotary_dim <= q.shape[-1]:
+        raise ValueError(f'rotary_dim {rotary_dim} of a head of {q.shape[-1]} channels: an even number up to it')
+    if positions.dtype not in POSITION_TYPES:
+        raise TypeError(f'positions are int32, int64, float32 or float64, not {positions.dtype}')
+    lead = q.shape[:-2]
+    pos = positions.unsqueeze(-1) if positions.dim() == len(lead) else positions
+    if pos.dim() != len(lead) + 1 or tuple(pos.shape[:-1]) != tuple(lead):
+        raise ValueError(f'positions of rows {tuple(lead)}: got {tuple(positions.shape)}')
+    assert turns.dtype == torch.float64 and axis.dtype == torch.int32 and turns.numel() == axis.numel() == rotary_dim // 2
+    device = _same_device(q, k, positions, turns, axis)
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    k = k if k is None or k.stride(-1) == 1 else k.contiguous()
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    views = [_heads(t) for t in (q, q_out, k, k_out)]
+    batch, rows = (1, lead[0]) if len(lead) == 1 else lead
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().geotr_rotary(ctypes.byref(views[0]), ctypes.byref(views[1]), None if k is None else ctypes.byref(views[2]),
+                                            None if k is None else ctypes.byref(views[3]), HEAD_TYPES[q.dtype], batch, rows, q.shape[-1],
+                                            int(rotary_dim), int(bool(interleaved)), _lib.ptr(pos), POSITION_TYPES[pos.dtype],
+                                            pos.stride(0) if len(lead) == 2 else 0, pos.stride(-2), pos.stride(-1), _lib.ptr(turns),
+                                            _lib.ptr(axis), float(gain), int(bool(inverse)), _lib.stream_ptr()), 'geotr_rotary')
+    return q_out, k_out
+
+
+def _aligned(t):
+    """Channels contiguous, addresses and strides multiples of 16 bytes (what the tiles are loaded in): t itself, or a contiguous copy."""
+    e = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % e == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def check_diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None, scale=None):
+    """Refuses what geotr_diff_attn_* does not compute, with the reason."""
+    if q.dim() not in (3, 4) or k.dim() != q.dim() or v.dim() != q.dim():
+        raise ValueError('q, k and v are (rows, heads, channels) in stack mode or (batch, rows, heads, channels): got '
+                         f'{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
+    if q.dtype not in HEAD_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f'q, k and v are float32, bfloat16 or float16, all of one type: got {q.dtype}, {k.dtype}, {v.dtype}')
+    heads, kv_heads = q.shape[-2] // 2, v.shape[-2]
+    if q.shape[-2] % 2 or k.shape[-2] != 2 * kv_heads or kv_heads < 1 or heads < 1 or heads % kv_heads or heads // kv_heads > 64:
+        raise ValueError(f'q has 2 H heads, k 2 Hk, v Hk, H a multiple of Hk (up to 64 times): got {q.shape[-2]}, {k.shape[-2]}, {kv_heads}')
+    if k.shape[:-2] != v.shape[:-2] or (q.dim() == 4 and q.shape[0] != k.shape[0]):
+        raise ValueError(f'rows of q {tuple(q.shape[:-2])}, k {tuple(k.shape[:-2])} and v {tuple(v.shape[:-2])} do not fit')
+    dim, v_dim = q.shape[-1], v.shape[-1]
+    if k.shape[-1] != dim or dim % 8 or not 8 <= dim <= 128 or v_dim % 8 or not 8 <= v_dim <= 256:
+        raise ValueError(f'channels of a head are multiples of 8, q and k alike up to 128, v up to 256: got {dim}, {k.shape[-1]}, {v_dim}')
+    if lam.dtype != torch.float32 or lam.dim() > 1 or lam.numel() not in (1, heads):
+        raise ValueError(f'lam is a float32 tensor of 1 or {heads} values: got {lam.dtype} {tuple(lam.shape)}')
+    if scale is not None and not 0.0 < float(scale) < 1e30:
+        raise ValueError(f'scale is a positive number, not {scale}')
+    if q.dim() == 3 and (q_lengths is None) != (k_lengths is None):
+        raise ValueError('stack mode takes both lengths (or none: one sequence)')
+    sequences = q.shape[0] if q.dim() == 4 else None
+    for name, t in (('q_lengths', q_lengths), ('k_lengths', k_lengths)):
+        if t is None:
+            continue
+        if t.dtype != torch.int64 or t.dim() != 1:
+            raise TypeError(f'{name} is an int64 tensor (sequences,): got {t.dtype} {tuple(t.shape)}')
+        sequences = t.shape[0] if sequences is None else sequences
+        if t.shape[0] != sequences:
+            raise ValueError(f'{name} of {t.shape[0]} sequences, expected {sequences}')
+    if key_masks is not None and (key_masks.dtype != torch.bool or key_masks.shape != k.shape[:-2]):
+        raise ValueError(f'key_masks are truth values of the rows of k {tuple(k.shape[:-2])}, True = ignored: got {key_masks.dtype} '
+                         f'{tuple(key_masks.shape)}')
+
+
+def _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale):
+    """(descriptor, what it points into) of a call."""
+    device = _same_device(q, k, v, lam, q_lengths, k_lengths, key_masks)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    lam = lam.expand(q.shape[-2] // 2).contiguous()
+    q_lengths, k_lengths, key_masks = (None if t is None else t.contiguous() for t in (q_lengths, k_lengths, key_masks))
+    stacked = q.dim() == 3 and q_lengths is not None
+    batch = q_lengths.shape[0] if stacked else 1 if q.dim() == 3 else q.shape[0]
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    op = DiffAttn(_heads(q), _heads(k), _heads(v), HEAD_TYPES[q.dtype], int(stacked), int(bool(causal)), 0, batch, q.shape[-3], k.shape[-3],
+                  q.shape[-1], v.shape[-1], lam.data_ptr(), *(None if t is None else t.data_ptr() for t in (q_lengths, k_lengths, key_masks)),
+                  scale, 0)
+    return op, (q, k, v, lam, q_lengths, k_lengths, key_masks), device
+
+
+def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None, want_state=False):
+    """out[i, h] = sum_j (softmax_j(scale q[i, 2h] . k[j, 2c]) - lam[h] softmax_j(scale q[i, 2h+1] . k[j, 2c+1])) v[j, c], c = h Hk / H
+    (geotr_diff_attn_forward).  want_state: also what diff_attention_backward needs, (out, (out2, lse))."""
+    check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
+    op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
+    lib, heads, kv_heads = _lib.load(), q.shape[-2] // 2, v.shape[-2]
+    out = torch.empty(q.shape[:-2] + (heads, v.shape[-1]), dtype=q.dtype, device=device)
+    out2 = lse = None
+    if want_state:
+        out2 = torch.empty_like(out)
+        lse = torch.empty((kv_heads, 2) + q.shape[:-2] + (heads // kv_heads,), dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        ws = _lib.workspace(lib.geotr_diff_attn_workspace_bytes(ctypes.byref(op)), device)
+        _lib.check(lib.geotr_diff_attn_forward(ctypes.byref(op), _lib.ptr(out), _lib.ptr(out2), _lib.ptr(lse), _lib.ptr(ws), ws.numel(),
+                                               _lib.stream_ptr()), 'geotr_diff_attn_forward')
+    del keep
+    return (out, (out2, lse)) if want_state else out
+
+
+def diff_attention_backward(dout, q, k, v, lam, out, state, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None):
+    """(dq, dk, dv, dlam (H)) for dout from diff_attention(..., want_state=True)'s results (geotr_diff_attn_backward)."""
+    op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
+    lib = _lib.load()
+    dout = _aligned(dout)
+    view = _heads(dout)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
+    dlam = torch.empty(q.shape[-2] // 2, dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        ws = _lib.workspace(lib.geotr_diff_attn_backward_workspace_bytes(ctypes.byref(op)), device)
+        _lib.check(lib.geotr_diff_attn_backward(ctypes.byref(op), ctypes.byref(view), _lib.ptr(out), _lib.ptr(state[0]), _lib.ptr(state[1]),
+                                                _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(dlam), _lib.ptr(ws), ws.numel(),
+                                                _lib.stream_ptr()), 'geotr_diff_attn_backward')
+    del keep
+    return dq, dk, dv, dlam

@@ -34,7 +34,7 @@ extern "C" {
 const char* geotr_last_error(void);
 /* ABI version of this header; bumped on any signature change.  A host compares the macro it was compiled against with what the
  * loaded library reports. */
-#define GEOTR_ABI_VERSION 8
+#define GEOTR_ABI_VERSION 9
 int geotr_abi_version(void);
 
 /* ------------------------------------------------------------------------------------------------
@@ -610,6 +610,60 @@ int geotr_pairwise_distance(const float* x, const float* y, int64_t batch, int64
                             int channel_first, float* out, void* stream);
 int geotr_index_select(const void* data, const int64_t* index, int64_t outer, int64_t size, int64_t n_index, int64_t inner_bytes,
                        void* out, int32_t* error_flag, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Rotary positions and differential attention (geotransformer_amd.modules.transformer: RotaryPositionalEmbedding,
+ * differential_attention, DifferentialTransformerLayer): operators the reference does not have, beside its
+ * SinusoidalPositionalEmbedding and MultiHeadAttention.
+ *
+ * geotr_heads: a strided view (batch, rows, heads, channels) of one type; channels contiguous, strides in ELEMENTS.
+ * ---------------------------------------------------------------------------------------------- */
+#define GEOTR_F32 0
+#define GEOTR_BF16 1
+#define GEOTR_F16 2
+#define GEOTR_POS_I32 0
+#define GEOTR_POS_I64 1
+#define GEOTR_POS_F32 2
+#define GEOTR_POS_F64 3
+typedef struct geotr_heads {
+  const void* data;          /* written through where the view is an output */
+  int64_t heads, batch_stride, row_stride, head_stride;
+} geotr_heads;
+
+/* Turn channel pair i of the first rotary_dim channels of every head by 2 pi * position[axis[i]] * turns[i] (64 bits), times gain:
+ *   y_a = gain (x_a cos - x_b sin), y_b = gain (x_b cos + x_a sin); (a, b) = (i, i + rotary_dim / 2), interleaved: (2i, 2i + 1).
+ * The other channels are copied.  inverse: the transposed rotation (the gradient).  k / k_out may both be NULL; in place (out = in) is
+ * allowed, other overlaps are not.  turns, axis: (rotary_dim / 2) device.  positions: element strides over (batch, row, axis). */
+int geotr_rotary(const geotr_heads* q, const geotr_heads* q_out, const geotr_heads* k, const geotr_heads* k_out, int dtype, int64_t batch,
+                 int64_t rows, int64_t dim, int64_t rotary_dim, int interleaved, const void* positions, int position_type,
+                 int64_t pos_batch_stride, int64_t pos_row_stride, int64_t pos_axis_stride, const double* turns, const int32_t* axis,
+                 float gain, int inverse, void* stream);
+
+/* out[i, h] = sum_j (softmax_j(scale q[i, 2h] . k[j, 2c]) - lam[h] softmax_j(scale q[i, 2h+1] . k[j, 2c+1])) v[j, c],  c = h / (H / Hk).
+ * q: 2 H heads of dim channels, k: 2 Hk heads, v: Hk heads of v_dim; H a multiple of Hk; dim <= 128, v_dim <= 256, multiples of 8; 16-byte
+ * aligned views.  Two layouts: stacked = 0: (batch, n, ...) and (batch, m, ...), lengths NULL or (batch); stacked = 1: n and m are the
+ * rows of ALL `batch` sequences one behind the other (stack mode), both lengths given.  Lengths are read on the device and held to the
+ * rows that exist.  key_masks: bytes (batch, m) or (m), contiguous, nonzero = ignored.  causal: query i sees keys j <= i + (keys - queries) of its sequence.
+ * Results of rows without a key, beyond their length or behind the last sequence are zero; what such key rows hold is never used.
+ * out, out2 (optional: the second map's output before lam): contiguous (rows, H, v_dim); lse (optional): (Hk, 2, rows, H / Hk) fp32. */
+typedef struct geotr_diff_attn {
+  geotr_heads q, k, v;
+  int32_t dtype, stacked, causal, pad_;
+  int64_t batch, n, m, dim, v_dim;
+  const float* lam;          /* (H) */
+  const int64_t* q_lengths;
+  const int64_t* k_lengths;
+  const uint8_t* key_masks;
+  float scale;
+  int32_t pad2_;
+} geotr_diff_attn;
+size_t geotr_diff_attn_workspace_bytes(const geotr_diff_attn* op);
+int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, void* out2, float* lse, void* ws, size_t ws_bytes, void* stream);
+/* Gradients for dout (strided like q, H heads of v_dim) from what the forward call left in out, out2 and lse: dq, dk, dv contiguous in
+ * the layout of q, k, v; dlam (H) fp32. */
+size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op);
+int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const void* out, const void* out2, const float* lse,
+                             void* dq, void* dk, void* dv, float* dlam, void* ws, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Native pyramid: precompute_data_stack_mode (geotransformer/utils/data.py:13-77) as one host call: (S-1) grid
