@@ -74,6 +74,10 @@ constexpr int kStep = 2 * kE<T>;           // channels (row reads) or contractio
 template <typename T>
 constexpr int kPSteps = 32 / kStep<T>;     // steps of a 32-deep product
 
+// waves that a SIMD unit holds at a time, by the registers of the accumulators
+template <typename T, int DB, int DVB>
+constexpr int kWaves = sizeof(T) * DB <= 128 ? 2 : 1;
+
 // fragment t of the accumulator's 32 contraction indices: registers E t .. E t + E - 1 (rounded to T: the one rounding of P and dS)
 template <typename T>
 __device__ __forceinline__ typename Ops<T>::Frag pack(const f32x16& p, int t) {
@@ -84,41 +88,73 @@ __device__ __forceinline__ typename Ops<T>::Frag pack(const f32x16& p, int t) {
 }
 
 // ---- LDS tiles ------------------------------------------------------------------------------------------------------------------------
-// A tile of `rows` rows of C 16-byte chunks; chunk c of row r lies at position c ^ swz(r).  256 bytes (all banks) hold RP = 16 / C rows.
+// A tile of rows of C 16-byte chunks; chunk c of row r lies at position c ^ swz(r).  256 bytes (all banks) hold 16 / C rows.  swz moves row
+// bits to chunk bits (linear over xor): eight rows read at one chunk, and the 4 rows x 2 chunks of a transposed read, fall on distinct banks.
 template <int C>
-__device__ __forceinline__ int swz(int row) {
-  constexpr int RP = C >= 16 ? 1 : 16 / C, M = (C >= 16 ? 16 : C) - 1;
-  const int x = row / RP;
-  return (((x << 1) & 14) | ((x >> 3) & 1)) & M;
+__device__ __host__ constexpr int swz(int row) {
+  return C >= 16 ? ((row << 1) & 14) | ((row >> 3) & 1) : ((row / (16 / C)) << 1) & (C - 1);
 }
-// fragment of row `row`: channels of chunk `chunk` (C-operand order of a row read: lane % 32 = row, half h reads chunk 2 s + h)
-template <typename T, int C>
-__device__ __forceinline__ typename Ops<T>::Frag row_frag(const char* tile, int row, int chunk) {
-  return *(const typename Ops<T>::Frag*)(tile + (row * C + (chunk ^ swz<C>(row))) * 16);
+template <class V>
+__device__ __forceinline__ V lds_load(unsigned at) {
+  return *(const GEOTR_LDS V*)(uintptr_t)at;
 }
-// transposed fragment: lane % 32 = channel col0 + lane % 32, contraction indices = rows row0 + (order of accumulator registers, step t)
+__device__ __forceinline__ unsigned lds_at(const void* p) { return (unsigned)(uintptr_t)(const GEOTR_LDS char*)p; }
+
+// Row reads: lane % 32 = row, chunks 2 q + half.  One address for each xor pattern, everything else in the instruction's offset.
 template <typename T, int C>
-__device__ __forceinline__ typename Ops<T>::Frag col_frag(const char* tile, int row0, int t, int col0, int lane) {
-  typename Ops<T>::Frag f;
-  if constexpr (sizeof(T) == 2) {
-    const int row = row0 + 16 * t + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int chunk = col0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const char* a = tile + (row * C + (chunk ^ swz<C>(row))) * 16 + (lane & 1) * 8;
-    const char* b = tile + ((row + 8) * C + (chunk ^ swz<C>(row + 8))) * 16 + (lane & 1) * 8;
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GEOTR_LDS s16x4*)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GEOTR_LDS s16x4*)b);
-    const auto z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    f = __builtin_bit_cast(typename Ops<T>::Frag, z);
-  } else {
-    const int chunk = col0 / 4 + ((lane & 31) >> 2);
+struct Rows {
+  static constexpr int N = (C >= 16 ? 16 : C) / 2;
+  unsigned a[N];
+  __device__ __forceinline__ Rows(int col, int half) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + 8 * t + 4 * (lane >> 5) + i;
-      f[i] = *(const float*)(tile + (row * C + (chunk ^ swz<C>(row))) * 16 + (lane & 3) * 4);
-    }
+    for (int j = 0; j < N; ++j) a[j] = col * C * 16 + ((2 * j + half) ^ swz<C>(col)) * 16;
   }
-  return f;
-}
+  __device__ __forceinline__ typename Ops<T>::Frag get(unsigned tile, int row0, int q) const {  // row0 a multiple of 32
+    return lds_load<typename Ops<T>::Frag>(tile + a[q % N] + (unsigned)(row0 * C * 16 + (q / N) * 256));
+  }
+};
+// Transposed reads: lane % 32 = channel 32 v + lane % 32; contraction indices = rows, in the order of the accumulator registers, step t
+template <typename T, int C, int SIZE = sizeof(T)>
+struct Cols;
+template <typename T, int C>
+struct Cols<T, C, 2> {
+  static constexpr int NU = C >= 16 ? 2 : 1, NV = (C >= 16 ? 16 : C) / 4;
+  unsigned a[NV * NU];
+  __device__ __forceinline__ Cols(int lane) {
+    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), lp = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int u = 0; u < NU; ++u) a[v * NU + u] = row * C * 16 + ((4 * v + lp) ^ swz<C>(row + 8 * u)) * 16 + (lane & 1) * 8;
+  }
+  __device__ __forceinline__ typename Ops<T>::Frag get(unsigned tile, int row0, int t, int v) const {  // row0 a multiple of 32
+    const unsigned o = (row0 + 16 * t) * C * 16 + (v / NV) * 256, i = (v % NV) * NU;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GEOTR_LDS s16x4*)(uintptr_t)(tile + a[i] + o));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GEOTR_LDS s16x4*)(uintptr_t)(tile + a[i + NU - 1] + o + 8 * C * 16));
+    return __builtin_bit_cast(typename Ops<T>::Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+template <typename T, int C>
+struct Cols<T, C, 4> {
+  static constexpr int NT = C >= 16 ? 2 : 1, NV = C >= 16 ? 2 : 1;
+  unsigned a[4 * NT * NV];
+  __device__ __forceinline__ Cols(int lane) {
+    const int row = 4 * (lane >> 5), c = (lane & 31) >> 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < NV; ++v) a[(i * NT + t) * NV + v] = (row + i) * C * 16 + ((8 * v + c) ^ swz<C>(row + i + 8 * t)) * 16 + (lane & 3) * 4;
+  }
+  __device__ __forceinline__ typename Ops<T>::Frag get(unsigned tile, int row0, int t, int v) const {
+    typename Ops<T>::Frag f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = lds_load<float>(tile + a[(i * NT + t % NT) * NV + v % NV] + (unsigned)((row0 + 8 * t) * C * 16 + (v / NV) * 256));
+    return f;
+  }
+};
 
 constexpr int kNumRecords = 0x40000000, kOutside = 0x7fffff00;  // a chunk at kOutside lies past every buffer: zeros
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p) {
@@ -133,19 +169,22 @@ __device__ __forceinline__ typename Ops<T>::Frag load_frag(__amdgpu_buffer_rsrc_
 }
 
 // ROWS rows of NM maps of `width` channels (bucket DB) into `tile`, dealt over the SHARE waves that use it (wave w of them).  src(row)
-// gives the byte offset of a row or kOutside.
-template <typename T, int ROWS, int NM, int DB, int SHARE, class Src>
+// gives the byte offset of a row or kOutside; ALL: every row exists and src is row * stride.  The lane number is hidden from the compiler:
+// it would keep every offset in registers through the loop (and spill them: a spilled offset is read back with a wait for all loads).
+template <typename T, int ROWS, int NM, int DB, int SHARE, bool ALL, class Src>
 __device__ __forceinline__ void stage(char* tile, __amdgpu_buffer_rsrc_t r, int width, int map_bytes, int w, int lane, Src src) {
-  constexpr int CM = DB * (int)sizeof(T) / 16, C = NM * CM, N = ROWS * C / 64;
-  static_assert(ROWS * C % 64 == 0, "whole wave loads");
+  constexpr int CM = DB * (int)sizeof(T) / 16, C = NM * CM, N = ROWS * C / 64, S = SHARE * 64 / C > 0 ? SHARE * 64 / C : 1;  // rows of a step
+  static_assert(ROWS * C % 64 == 0 && C <= 64, "whole wave loads");
+  asm volatile("" : "+v"(lane));
+  const int p = w * 64 + lane, row0 = p / C, pos = (p % C) ^ swz<C>(row0);
 #pragma unroll
   for (int it = 0; it < (N + SHARE - 1) / SHARE; ++it) {
-    const int i = it * SHARE + w;
-    if (N % SHARE != 0 && i >= N) break;
-    const int p = i * 64 + lane, row = p / C, c = (p % C) ^ swz<C>(row);
+    if (N % SHARE != 0 && it * SHARE + w >= N) break;
+    const int c = pos ^ swz<C>(it * S);  // swz is linear and row0 < S
     const int map = NM == 1 ? 0 : c / CM, cc = NM == 1 ? c : c % CM;
-    const int o = src(row);
-    load_lds(r, tile + i * 1024, (o == kOutside || cc * kE<T> >= width) ? kOutside : o + map * map_bytes + cc * 16);
+    const int o = src(it * S + row0);
+    const bool out = cc * kE<T> >= width || (!ALL && o == kOutside);
+    load_lds(r, tile + (it * SHARE + w) * 1024, out ? kOutside : o + map * map_bytes + cc * 16);
   }
 }
 
@@ -236,7 +275,18 @@ __device__ __forceinline__ f32x16 zero16() {
 // Scores beyond 2^20 (in powers of two): s c - b with a product of its own.  An fma keeps the exact product, whose distance from the
 // rounded maximum b grows with it until the exponential overflows; rounded alike, the largest score gives exactly 0.
 constexpr float kHuge = 1048576.f;
-__device__ __forceinline__ float exponent(float s, float c, float b, bool huge) { return huge ? s * c - b : fmaf(s, c, -b); }
+template <class B>
+__device__ __forceinline__ void exponents(f32x16& s, float c, B b, bool huge) {
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(huge), 0)) {  // a branch of the wave, not a choice per element
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = s[i] * c - b(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], c, -b(i));
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
+}
 
 // One packed query row of a lane: its query, head within the group, and whether it exists
 struct Row {
@@ -266,7 +316,7 @@ __device__ __forceinline__ void store4(T* p, float x, float y, float z, float w)
 // KEYS = true (few rows): all waves own the same 32 rows and every wave streams key tiles of its own (no barrier), joined at the end; with
 // a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next launch.
 template <typename T, int DB, int DVB, int NW, bool KEYS>
-__global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>;
   constexpr int kTileBytes64 = 64 * (CK + CV) * 16;
@@ -352,19 +402,26 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
     const auto rk = buffer(kp + (int64_t)key0 * a.k.row_stride);
     const auto rv = buffer(vp + (int64_t)key0 * a.v.row_stride);
     const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
-    stage<T, BN, 2, DB, SHARE>(tile, rk, a.d, (int)(a.k.head_stride * sizeof(T)), w, lane,
-                        [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
-    stage<T, BN, 1, DVB, SHARE>(tile + BN * CK * 16, rv, a.dv, 0, w, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
+    const int hs = (int)(a.k.head_stride * sizeof(T));
+    if (bits == (BN == 64 ? ~0ull : 0xffffffffull)) {
+      stage<T, BN, 2, DB, SHARE, true>(tile, rk, a.d, hs, w, lane, [&](int x) { return x * krs; });
+      stage<T, BN, 1, DVB, SHARE, true>(tile + BN * CK * 16, rv, a.dv, 0, w, lane, [&](int x) { return x * vrs; });
+    } else {
+      stage<T, BN, 2, DB, SHARE, false>(tile, rk, a.d, hs, w, lane, [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
+      stage<T, BN, 1, DVB, SHARE, false>(tile + BN * CK * 16, rv, a.dv, 0, w, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
+    }
   };
 
+  const Rows<T, CK> krow(col, half);
+  const Cols<T, CV> vcol(lane);
   // 32 keys of a staged tile
-  auto consume = [&](const char* tile, int sub, int key0, uint64_t bits) {
-    const char* vt = tile + BN * CK * 16;
+  auto consume = [&](const char* at, int sub, int key0, uint64_t bits) {
+    const unsigned tile = lds_at(at), vt = tile + BN * CK * 16;
     f32x16 s1 = zero16(), s2 = zero16();
 #pragma unroll
     for (int i = 0; i < QS; ++i) {
-      Ops<T>::mma(s1, row_frag<T, CK>(tile, 32 * sub + col, 2 * i + half), q1[i]);
-      Ops<T>::mma(s2, row_frag<T, CK>(tile, 32 * sub + col, CK / 2 + 2 * i + half), q2[i]);
+      Ops<T>::mma(s1, krow.get(tile, 32 * sub, i), q1[i]);
+      Ops<T>::mma(s2, krow.get(tile, 32 * sub, CK / 4 + i), q2[i]);
     }
     const int k0 = key0 + 32 * sub;
     unsigned lo = (unsigned)(bits >> (32 * sub));
@@ -395,18 +452,16 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
         for (int j = 0; j < 16; ++j) acc1[i][j] *= c1, acc2[i][j] *= c2;
     }
     const float b1 = m1 == -INFINITY ? 0.f : m1, b2 = m2 == -INFINITY ? 0.f : m2;
+    exponents(s1, a.scale_log2, [&](int) { return b1; }, huge);
+    exponents(s2, a.scale_log2, [&](int) { return b2; }, huge);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s1[i] = __builtin_amdgcn_exp2f(exponent(s1[i], a.scale_log2, b1, huge));
-      s2[i] = __builtin_amdgcn_exp2f(exponent(s2[i], a.scale_log2, b2, huge));
-      l1 += s1[i], l2 += s2[i];
-    }
+    for (int i = 0; i < 16; ++i) l1 += s1[i], l2 += s2[i];
 #pragma unroll
     for (int p = 0; p < kPSteps<T>; ++p) {
       const Frag p1 = pack<T>(s1, p), p2 = pack<T>(s2, p);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const Frag f = col_frag<T, CV>(vt, 32 * sub, p, 32 * i, lane);
+        const Frag f = vcol.get(vt, 32 * sub, p, i);
         Ops<T>::mma(acc1[i], f, p1);
         Ops<T>::mma(acc2[i], f, p2);
       }
@@ -426,13 +481,14 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
     }
   } else {
     int which = 0;
-    uint64_t bits = key_bits(a, s, begin, end, lane);
+    constexpr uint64_t kKeys = BN == 64 ? ~0ull : 0xffffffffull;
+    uint64_t bits = key_bits(a, s, begin, end, lane) & kKeys;
     if (begin < end) fill(smem, begin, bits);
     for (int key0 = begin; key0 < end; key0 += BN) {
       __syncthreads();  // waits for this wave's loads: the tile is complete, and nobody reads the other buffer any more
       uint64_t next = 0;
       if (key0 + BN < end) {
-        next = key_bits(a, s, key0 + BN, end, lane);
+        next = key_bits(a, s, key0 + BN, end, lane) & kKeys;
         fill(smem + (which ^ 1) * kTile, key0 + BN, next);
       }
 #pragma unroll
@@ -548,7 +604,7 @@ __device__ __forceinline__ float grad_scale(const Args& a) {
 }
 
 template <typename T, int DB, int DVB, int NW>
-__global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, ND = DB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
   constexpr int kTile = 32 * (CK + CV) * 16, TILE = 32 * NW;
@@ -624,33 +680,45 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     const auto rk = buffer(kp + (int64_t)key0 * a.k.row_stride);
     const auto rv = buffer(vp + (int64_t)key0 * a.v.row_stride);
     const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
-    stage<T, 32, 2, DB, NW>(tile, rk, a.d, (int)(a.k.head_stride * sizeof(T)), wave, lane,
-                        [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
-    stage<T, 32, 1, DVB, NW>(tile + 32 * CK * 16, rv, a.dv, 0, wave, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
+    const int hs = (int)(a.k.head_stride * sizeof(T));
+    if (bits == 0xffffffffull) {
+      stage<T, 32, 2, DB, NW, true>(tile, rk, a.d, hs, wave, lane, [&](int x) { return x * krs; });
+      stage<T, 32, 1, DVB, NW, true>(tile + 32 * CK * 16, rv, a.dv, 0, wave, lane, [&](int x) { return x * vrs; });
+    } else {
+      stage<T, 32, 2, DB, NW, false>(tile, rk, a.d, hs, wave, lane, [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
+      stage<T, 32, 1, DVB, NW, false>(tile + 32 * CK * 16, rv, a.dv, 0, wave, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
+    }
   };
-  auto consume = [&](const char* tile, int key0, uint64_t bits) {
-    const char* vt = tile + 32 * CK * 16;
+  const Rows<T, CK> krow(col, half);
+  const Rows<T, CV> vrow(col, half);
+  const Cols<T, CK> kcol(lane);
+  auto consume = [&](const char* at, int key0, uint64_t bits) {
+    const unsigned tile = lds_at(at), vt = tile + 32 * CK * 16;
     f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
 #pragma unroll
     for (int i = 0; i < QS; ++i) {
-      Ops<T>::mma(s1, row_frag<T, CK>(tile, col, 2 * i + half), q1[i]);
-      Ops<T>::mma(s2, row_frag<T, CK>(tile, col, CK / 2 + 2 * i + half), q2[i]);
+      Ops<T>::mma(s1, krow.get(tile, 0, i), q1[i]);
+      Ops<T>::mma(s2, krow.get(tile, 0, CK / 4 + i), q2[i]);
     }
 #pragma unroll
-    for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, row_frag<T, CV>(vt, col, 2 * i + half), go[i]);
+    for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, vrow.get(vt, 0, i), go[i]);
     unsigned lo = (unsigned)bits;
     const int above = limit - key0;
     if (above < 31) lo = above < 0 ? 0u : lo & ((2u << above) - 1);
     const bool some = __any(lo != 0xffffffffu);
     lo >>= 4 * half;
+    exponents(s1, a.scale_log2, [&](int) { return lse1; }, huge);
+    exponents(s2, a.scale_log2, [&](int) { return lse2; }, huge);
+    if (__builtin_expect(some, 0)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool in = (lo >> (8 * (i / 4) + i % 4)) & 1;
+        s1[i] = in ? s1[i] : 0.f, s2[i] = in ? s2[i] : 0.f;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float p1 = __builtin_amdgcn_exp2f(exponent(s1[i], a.scale_log2, lse1, huge));
-      float p2 = __builtin_amdgcn_exp2f(exponent(s2[i], a.scale_log2, lse2, huge));
-      if (some) {
-        const bool in = (lo >> (8 * (i / 4) + i % 4)) & 1;
-        p1 = in ? p1 : 0.f, p2 = in ? p2 : 0.f;
-      }
+      const float p1 = s1[i], p2 = s2[i];
       dsum = fmaf(p2, dp[i], dsum);
       s1[i] = p1 * (dp[i] - del1), s2[i] = -lam * p2 * (dp[i] - del2);
       if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs;
@@ -660,8 +728,8 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
       const Frag d1 = pack<T>(s1, p), d2 = pack<T>(s2, p);
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        Ops<T>::mma(acc1[i], col_frag<T, CK>(tile, 0, p, 32 * i, lane), d1);
-        Ops<T>::mma(acc2[i], col_frag<T, CK>(tile, 0, p, DB + 32 * i, lane), d2);
+        Ops<T>::mma(acc1[i], kcol.get(tile, 0, p, i), d1);
+        Ops<T>::mma(acc2[i], kcol.get(tile, 0, p, ND + i), d2);
       }
     }
   };
@@ -717,7 +785,7 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
 // A wave owns 32 keys; K and V are the B operands (lane = key), in registers where they fit beside the accumulators (16-bit types), else
 // read again from memory for every tile of 32 packed query rows (32-bit: a product takes 16 times as long as its operand's load).
 template <typename T, int DB, int DVB, int NW>
-__global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CQ = 2 * DB * (int)sizeof(T) / 16, CO = DVB * (int)sizeof(T) / 16, ND = DB / 32, NV = DVB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
   constexpr bool kHold = sizeof(T) == 2;
@@ -784,6 +852,10 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   const T* const qp = (const T*)a.q.data + s.b * a.q.batch_stride + (a.stacked ? s.q0 : 0) * a.q.row_stride + (int64_t)kvh * 2 * a.g * a.q.head_stride;
   const T* const op = (const T*)a.dout.data + s.b * a.dout.batch_stride + (a.stacked ? s.q0 : 0) * a.dout.row_stride +
                       (int64_t)kvh * a.g * a.dout.head_stride;
+  const Rows<T, CQ> qrow(col, half);
+  const Rows<T, CO> orow(col, half);
+  const Cols<T, CQ> qcol(lane);
+  const Cols<T, CO> ocol(lane);
   for (int r0 = first; r0 < rows; r0 += 32) {
     __syncthreads();
     const int i0 = a.g == 1 ? r0 : r0 / a.g;
@@ -793,9 +865,9 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
       const int r = r0 + x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
       return r < rows ? (int)(((i - i0) * rs + h * hstr) * (int)sizeof(T)) : kOutside;
     };
-    stage<T, 32, 2, DB, NW>(smem, rq, a.d, (int)(a.q.head_stride * sizeof(T)), wave, lane,
+    stage<T, 32, 2, DB, NW, false>(smem, rq, a.d, (int)(a.q.head_stride * sizeof(T)), wave, lane,
                         [&](int x) { return q_off(x, a.q.row_stride, 2 * a.q.head_stride); });
-    stage<T, 32, 1, DVB, NW>(smem + 32 * CQ * 16, ro, a.dv, 0, wave, lane,
+    stage<T, 32, 1, DVB, NW, false>(smem + 32 * CQ * 16, ro, a.dv, 0, wave, lane,
                          [&](int x) { return q_off(x, a.dout.row_stride, a.dout.head_stride); });
     if (threadIdx.x < 32) {
       const int r = r0 + threadIdx.x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
@@ -811,28 +883,33 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
       ((int*)st)[160 + threadIdx.x] = a.causal ? i + off : 0x7fffffff;
     }
     __syncthreads();
-    const char* ot = smem + 32 * CQ * 16;
+    const unsigned qt = lds_at(smem), ot = qt + 32 * CQ * 16;
     f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
 #pragma unroll
     for (int i = 0; i < QS; ++i) {
-      Ops<T>::mma(s1, row_frag<T, CQ>(smem, col, 2 * i + half), kHold ? k1[i % (kHold ? QS : 1)] : k_frag(0, i));
-      Ops<T>::mma(s2, row_frag<T, CQ>(smem, col, CQ / 2 + 2 * i + half), kHold ? k2[i % (kHold ? QS : 1)] : k_frag(1, i));
+      Ops<T>::mma(s1, qrow.get(qt, 0, i), kHold ? k1[i % (kHold ? QS : 1)] : k_frag(0, i));
+      Ops<T>::mma(s2, qrow.get(qt, 0, CQ / 4 + i), kHold ? k2[i % (kHold ? QS : 1)] : k_frag(1, i));
     }
 #pragma unroll
-    for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, row_frag<T, CO>(ot, col, 2 * i + half), kHold ? vv[i % (kHold ? VS : 1)] : v_frag(i));
+    for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, orow.get(ot, 0, i), kHold ? vv[i % (kHold ? VS : 1)] : v_frag(i));
     const bool huge = __builtin_amdgcn_readfirstlane(((const int*)st)[192]) != 0;
     f32x16 pj;
+    auto stat = [&](int which, int i) { return st[32 * which + 8 * (i / 4) + 4 * half + i % 4]; };
+    exponents(s1, a.scale_log2, [&](int i) { return stat(0, i); }, huge);
+    exponents(s2, a.scale_log2, [&](int i) { return stat(1, i); }, huge);
+    if (a.causal && r0 < (key_base + TILE - 1 - off) * a.g) {  // a tile that some key of the block is not seen by
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (key > __float_as_int(stat(5, i))) s1[i] = 0.f, s2[i] = 0.f;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int x = 8 * j + 4 * half;
-      const f32x4 e1 = *(const f32x4*)(st + x), e2 = *(const f32x4*)(st + 32 + x), d1 = *(const f32x4*)(st + 64 + x),
-                  d2 = *(const f32x4*)(st + 96 + x), lm = *(const f32x4*)(st + 128 + x);
+      const f32x4 d1 = *(const f32x4*)(st + 64 + x), d2 = *(const f32x4*)(st + 96 + x), lm = *(const f32x4*)(st + 128 + x);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * j + e;
-        float p1 = __builtin_amdgcn_exp2f(exponent(s1[i], a.scale_log2, e1[e], huge));
-        float p2 = __builtin_amdgcn_exp2f(exponent(s2[i], a.scale_log2, e2[e], huge));
-        if (a.causal && key > ((const int*)st)[160 + x + e]) p1 = 0.f, p2 = 0.f;
+        const float p1 = s1[i], p2 = s2[i];
         pj[i] = fmaf(-lm[e], p2, p1) * kBoost;
         s1[i] = p1 * (dp[i] - d1[e]), s2[i] = -lm[e] * p2 * (dp[i] - d2[e]);
         if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs;
@@ -842,11 +919,11 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     for (int p = 0; p < kPSteps<T>; ++p) {
       const Frag fp = pack<T>(pj, p), f1 = pack<T>(s1, p), f2 = pack<T>(s2, p);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) Ops<T>::mma(av[i], col_frag<T, CO>(ot, 0, p, 32 * i, lane), fp);
+      for (int i = 0; i < NV; ++i) Ops<T>::mma(av[i], ocol.get(ot, 0, p, i), fp);
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        Ops<T>::mma(ak1[i], col_frag<T, CQ>(smem, 0, p, 32 * i, lane), f1);
-        Ops<T>::mma(ak2[i], col_frag<T, CQ>(smem, 0, p, DB + 32 * i, lane), f2);
+        Ops<T>::mma(ak1[i], qcol.get(qt, 0, p, i), f1);
+        Ops<T>::mma(ak2[i], qcol.get(qt, 0, p, ND + i), f2);
       }
     }
   }
