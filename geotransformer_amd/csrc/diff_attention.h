@@ -30,6 +30,7 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 #define GEOTR_LDS __attribute__((address_space(3)))
+#define GEOTR_INLINE __attribute__((always_inline))
 
 struct Args {
   geotr_heads q, k, v, dout;             // dout: backward only
@@ -77,6 +78,10 @@ constexpr int kPSteps = 32 / kStep<T>;     // steps of a 32-deep product
 // waves that a SIMD unit holds at a time, by the registers of the accumulators
 template <typename T, int DB, int DVB>
 constexpr int kWaves = sizeof(T) * DB <= 128 ? 2 : 1;
+template <typename T, int DB, int DVB>
+constexpr int kWavesRows = sizeof(T) == 4 ? (DB <= 32 ? 3 : DB <= 64 ? 2 : 1) : DVB <= 64 ? 4 : DVB <= 128 ? 3 : 2;
+template <typename T, int DB, int DVB>
+constexpr int kGroups = 2;
 
 // fragment t of the accumulator's 32 contraction indices: registers E t .. E t + E - 1 (rounded to T: the one rounding of P and dS)
 template <typename T>
@@ -92,7 +97,7 @@ __device__ __forceinline__ typename Ops<T>::Frag pack(const f32x16& p, int t) {
 // bits to chunk bits (linear over xor): eight rows read at one chunk, and the 4 rows x 2 chunks of a transposed read, fall on distinct banks.
 template <int C>
 __device__ __host__ constexpr int swz(int row) {
-  return C >= 16 ? ((row << 1) & 14) | ((row >> 3) & 1) : ((row / (16 / C)) << 1) & (C - 1);
+  return C >= 16 ? ((row << 1) & 14) | ((row >> 3) & 1) : ((row * C / 16) << 1) & (C - 1);
 }
 template <class V>
 __device__ __forceinline__ V lds_load(unsigned at) {
@@ -100,14 +105,15 @@ __device__ __forceinline__ V lds_load(unsigned at) {
 }
 __device__ __forceinline__ unsigned lds_at(const void* p) { return (unsigned)(uintptr_t)(const GEOTR_LDS char*)p; }
 
-// Row reads: lane % 32 = row, chunks 2 q + half.  One address for each xor pattern, everything else in the instruction's offset.
-template <typename T, int C>
+// Row reads: lane % 32 = row, chunks c0 + 2 q + half of the CM from c0 (a multiple of CM) on.  One address for each xor pattern, everything
+// else in the instruction's offset.
+template <typename T, int C, int CM = C>
 struct Rows {
-  static constexpr int N = (C >= 16 ? 16 : C) / 2;
+  static constexpr int N = (CM >= 16 ? 16 : CM) / 2;
   unsigned a[N];
-  __device__ __forceinline__ Rows(int col, int half) {
+  __device__ __forceinline__ Rows(int col, int half, int c0 = 0) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) a[j] = col * C * 16 + ((2 * j + half) ^ swz<C>(col)) * 16;
+    for (int j = 0; j < N; ++j) a[j] = col * C * 16 + ((c0 + 2 * j + half) ^ swz<C>(col)) * 16;
   }
   __device__ __forceinline__ typename Ops<T>::Frag get(unsigned tile, int row0, int q) const {  // row0 a multiple of 32
     return lds_load<typename Ops<T>::Frag>(tile + a[q % N] + (unsigned)(row0 * C * 16 + (q / N) * 256));
@@ -160,31 +166,97 @@ constexpr int kNumRecords = 0x40000000, kOutside = 0x7fffff00;  // a chunk at kO
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, kNumRecords, 0x00020000);
 }
-__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, char* lds, int offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (GEOTR_LDS void*)lds, 16, offset, 0, 0, 0);
+// 16 bytes per lane from byte offset + scalar into 1 024 bytes of LDS.  Issued by asm (it writes no register): the compiler takes a
+// transposed LDS read for one that may depend on every such load in flight and would wait for the next tile before this one's products
+// (causal 8 192: 489 us with the builtin).  The loops wait themselves (tile_ready).
+using i32x4 = __attribute__((ext_vector_type(4))) int;
+__device__ __forceinline__ i32x4 words(const void* p) {
+  const uint64_t u = (uint64_t)p;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)u), __builtin_amdgcn_readfirstlane((int)(u >> 32)) & 0xffff, kNumRecords, 0x00020000};
+}
+__device__ __forceinline__ void load_lds(i32x4 d, unsigned lds, int offset, int scalar = 0) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(d), "s"(scalar)
+               : "memory");
+}
+// the descriptor `bytes` further on
+__device__ __forceinline__ i32x4 advance(i32x4 d, unsigned bytes) {
+  const uint64_t u = (((uint64_t)(unsigned)d[1] << 32) | (unsigned)d[0]) + bytes;
+  return i32x4{(int)u, (int)(u >> 32), d[2], d[3]};
+}
+// this wave's tile loads have arrived, all but the youngest PENDING
+template <int PENDING = 0>
+__device__ __forceinline__ void tile_ready() {
+  static_assert(PENDING < 64, "six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PENDING) : "memory");
+}
+// Ends the compiler's own wait for what it loaded into x: a use inside a loop would wait for the tile loads in flight as well.
+template <class V>
+__device__ __forceinline__ void arrived(V& x) {
+  asm volatile("" : "+v"(x));
 }
 template <typename T>
 __device__ __forceinline__ typename Ops<T>::Frag load_frag(__amdgpu_buffer_rsrc_t r, int offset) {
   return __builtin_bit_cast(typename Ops<T>::Frag, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
 }
 
-// ROWS rows of NM maps of `width` channels (bucket DB) into `tile`, dealt over the SHARE waves that use it (wave w of them).  src(row)
-// gives the byte offset of a row or kOutside; ALL: every row exists and src is row * stride.  The lane number is hidden from the compiler:
-// it would keep every offset in registers through the loop (and spill them: a spilled offset is read back with a wait for all loads).
-template <typename T, int ROWS, int NM, int DB, int SHARE, bool ALL, class Src>
-__device__ __forceinline__ void stage(char* tile, __amdgpu_buffer_rsrc_t r, int width, int map_bytes, int w, int lane, Src src) {
-  constexpr int CM = DB * (int)sizeof(T) / 16, C = NM * CM, N = ROWS * C / 64, S = SHARE * 64 / C > 0 ? SHARE * 64 / C : 1;  // rows of a step
+// ROWS rows of NM maps of `width` channels (bucket DB) from rows of rs bytes into a tile, dealt over the SHARE waves that use it (wave w of
+// them).  A step of the waves covers S rows; the swizzle repeats after 16 (and is linear over xor), so a lane keeps one offset for each of
+// NB steps and reaches the others by a scalar: no vector arithmetic per load where every row exists.
+template <typename T, int ROWS, int NM, int DB, int SHARE>
+struct Stage {
+  static constexpr int CM = DB * (int)sizeof(T) / 16, C = NM * CM, N = ROWS * C / 64, S = SHARE * 64 / C > 0 ? SHARE * 64 / C : 1;
+  static constexpr int NS = (N + SHARE - 1) / SHARE, NB = C < 16 || S >= 16 ? 1 : 16 / S < NS ? 16 / S : NS;
   static_assert(ROWS * C % 64 == 0 && C <= 64, "whole wave loads");
-  asm volatile("" : "+v"(lane));
-  const int p = w * 64 + lane, row0 = p / C, pos = (p % C) ^ swz<C>(row0);
+  int base[NB], row0;
+  __device__ __forceinline__ Stage(int width, int rs, int map_bytes, int w, int lane) {
+    const int p = w * 64 + lane;
+    row0 = p / C;
+    const int pos = (p % C) ^ swz<C>(row0);
 #pragma unroll
-  for (int it = 0; it < (N + SHARE - 1) / SHARE; ++it) {
-    if (N % SHARE != 0 && it * SHARE + w >= N) break;
-    const int c = pos ^ swz<C>(it * S);  // swz is linear and row0 < S
-    const int map = NM == 1 ? 0 : c / CM, cc = NM == 1 ? c : c % CM;
-    const int o = src(it * S + row0);
-    const bool out = cc * kE<T> >= width || (!ALL && o == kOutside);
-    load_lds(r, tile + (it * SHARE + w) * 1024, out ? kOutside : o + map * map_bytes + cc * 16);
+    for (int j = 0; j < NB; ++j) {
+      const int c = pos ^ swz<C>(j * S), map = NM == 1 ? 0 : c / CM, cc = NM == 1 ? c : c % CM;
+      base[j] = cc * kE<T> >= width ? kOutside : (j * S + row0) * rs + map * map_bytes + cc * 16;
+    }
+  }
+  template <class Row>
+  __device__ __forceinline__ void load(unsigned tile, i32x4 r, int rs, int w, Row row) const {
+#pragma unroll
+    for (int it = 0; it < NS; ++it) {
+      if (N % SHARE != 0 && it * SHARE + w >= N) break;
+      const int j = it % NB;
+      load_lds(r, tile + (it * SHARE + w) * 1024, row(it * S + row0) ? base[j] : kOutside, (it - j) * S * rs);
+    }
+  }
+  // every row exists; the descriptor's base runs along
+  __device__ __forceinline__ void load_all(unsigned tile, i32x4 r, int rs, int w) const {
+#pragma unroll
+    for (int it = 0; it < NS; ++it) {
+      if (N % SHARE != 0 && it * SHARE + w >= N) break;
+      load_lds(r, tile + (it * SHARE + w) * 1024, base[it % NB], (it - it % NB) * S * rs);
+    }
+  }
+  // rows `bits` of the tile
+  __device__ __forceinline__ void load(unsigned tile, i32x4 r, int rs, int w, uint64_t bits) const {
+    if (bits == (ROWS == 64 ? ~0ull : 0xffffffffull)) load(tile, r, rs, w, [](int) { return true; });
+    else load(tile, r, rs, w, [&](int x) { return (bits >> x) & 1; });
+  }
+};
+
+// the same for rows at offsets of their own: src(row) gives a byte offset or kOutside
+template <typename T, int ROWS, int NM, int DB, int SHARE, class Src>
+__device__ __forceinline__ void stage_at(unsigned tile, i32x4 r, int width, int map_bytes, int w, int lane, Src src) {
+  using L = Stage<T, ROWS, NM, DB, SHARE>;
+  asm volatile("" : "+v"(lane));  // recomputed for every tile: kept in registers the offsets would be spilled
+  const int p = w * 64 + lane, row0 = p / L::C, pos = (p % L::C) ^ swz<L::C>(row0);
+#pragma unroll
+  for (int it = 0; it < L::NS; ++it) {
+    if (L::N % SHARE != 0 && it * SHARE + w >= L::N) break;
+    const int c = pos ^ swz<L::C>(it * L::S);  // swz is linear and row0 < S
+    const int map = NM == 1 ? 0 : c / L::CM, cc = NM == 1 ? c : c % L::CM;
+    const int o = src(it * L::S + row0);
+    load_lds(r, tile + (it * SHARE + w) * 1024, o == kOutside || cc * kE<T> >= width ? kOutside : o + map * map_bytes + cc * 16);
   }
 }
 
@@ -277,7 +349,7 @@ __device__ __forceinline__ f32x16 zero16() {
 constexpr float kHuge = 1048576.f;
 template <class B>
 __device__ __forceinline__ void exponents(f32x16& s, float c, B b, bool huge) {
-  if (__builtin_expect(__builtin_amdgcn_readfirstlane(huge), 0)) {  // a branch of the wave, not a choice per element
+  if (__builtin_expect(huge, 0)) {  // a branch of the wave, not a choice per element
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = s[i] * c - b(i);
   } else {
@@ -312,51 +384,290 @@ __device__ __forceinline__ void store4(T* p, float x, float y, float z, float w)
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------
-// NW waves.  KEYS = false: wave w owns packed rows 32 w .. of the block's 32 NW, all waves share the staged tile of BN keys.
-// KEYS = true (few rows): all waves own the same 32 rows and every wave streams key tiles of its own (no barrier), joined at the end; with
-// a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next launch.
-template <typename T, int DB, int DVB, int NW, bool KEYS>
-__global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_kernel(Args a) {
+// Order of the tiles of one sequence: causal rows cost what lies before them.  With two blocks to a compute unit at most, all run at once
+// and the second half goes up from the shortest (a long block shares its unit with a short one); else the longest go first.
+__device__ __forceinline__ int tile_order(const Args& a, int y, int tiles, int others) {
+  if (!a.causal) return y;
+  if ((int64_t)tiles * others > 512) return tiles - 1 - y;
+  return y < (tiles + 1) / 2 ? tiles - 1 - y : y - (tiles + 1) / 2;
+}
+// keys of this block when they are dealt over blockIdx.z
+__device__ __forceinline__ void split_keys(const Args& a, int& begin, int& end) {
+  const int tiles = (end + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
+  begin = min(end, (int)blockIdx.z * per * 32);
+  end = min(end, begin + per * 32);
+}
+// rows behind the last sequence: zero results
+template <typename T>
+__device__ __forceinline__ void zero_rows(const Args& a, const Seq& s, int kvh, int threads) {
+  const int64_t rows = s.q_end < a.nq ? a.nq - s.q_end : 0, per = (int64_t)a.g * a.dv, first = (int64_t)s.spare * threads + threadIdx.x,
+                step = (int64_t)s.spares * threads;
+  if (a.splits > 1) {  // no keys: the join writes zeros
+    const int w = a.dv + 4;
+    for (int64_t e = first; e < rows * a.g; e += step) {
+      float* p = a.part + (((int64_t)blockIdx.z * a.nq + s.q_end + e / a.g) * a.hk * a.g + kvh * a.g + e % a.g) * 2 * w;
+      p[0] = p[w] = -INFINITY, p[1] = p[w + 1] = 0.f;
+    }
+    return;
+  }
+  for (int64_t e = first; e < rows * per; e += step) {
+    const int64_t i = e / per, o = ((s.q_end + i) * a.hk + kvh) * per + (e - i * per);
+    ((T*)a.out)[o] = (T)0.f;
+    if (a.o2) ((T*)a.o2)[o] = (T)0.f;
+  }
+  for (int64_t e = first; a.lse && e < rows * a.g; e += step) {
+    const int64_t at = stat_at(a, kvh, 0, s.q_end, 0) + e;
+    a.lse[at] = a.lse[at + a.nq * a.g] = INFINITY;
+  }
+}
+
+// Many rows: the waves are two maps x G groups of 32 packed rows; a wave owns 32 rows of ONE map, so it needs half the accumulators (three
+// waves to a SIMD unit at d = 64, v 128, where both maps in a wave leave one) and the maps meet in LDS at the end.  Tiles of 32 keys in two
+// buffers: the next one loads while this one is consumed.
+// The accumulators are rescaled only when a row's maximum grew by more than 2^8: weights stay below 2^8, sums are exact either way.
+template <typename T, int DB, int DVB, int G>
+__global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
-  constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>;
-  constexpr int kTileBytes64 = 64 * (CK + CV) * 16;
-  constexpr int BN = KEYS ? 32 : (kTileBytes64 <= 40960 ? 64 : 32);
-  constexpr int kTile = BN * (CK + CV) * 16;
-  constexpr int kJoin = KEYS ? (NW / 2) * 64 * (2 * NT * 16 + 4) * 4 : 0;
-  constexpr int kSmem = KEYS ? (kTile * NW > kJoin ? kTile * NW : kJoin) : 2 * kTile;
+  constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>, TILE = 32 * G;
+  constexpr int BN = 32, kTile = BN * (CK + CV) * 16, kJoin = G * NT * 16 * 64 * 4;
+  constexpr int kSmem = 2 * kTile > kJoin ? 2 * kTile : kJoin;
+  constexpr bool kAgain = NT * 16 + QS * 4 <= 80;  // registers left for computing scores again
   __shared__ __attribute__((aligned(1024))) char smem[kSmem];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-  constexpr int TILE = KEYS ? 32 : 32 * NW;
+  const int map = wave & 1, group = wave >> 1;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const int t = a.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y;  // causal: the longest rows first
+  const int t = tile_order(a, blockIdx.y, gridDim.y, gridDim.x);
   const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
-  T* const out = (T*)a.out;
-  T* const o2 = (T*)a.o2;
-  if (s.tile < 0) {  // rows behind the last sequence: zero results
-    const int64_t rows = s.q_end < a.nq ? a.nq - s.q_end : 0, per = (int64_t)a.g * a.dv;
-    if (a.splits > 1) {  // no keys: the join writes zeros
-      const int w = a.dv + 4;
-      for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * a.g; e += (int64_t)s.spares * (NW * 64)) {
-        float* p = a.part + (((int64_t)blockIdx.z * a.nq + s.q_end + e / a.g) * a.hk * a.g + kvh * a.g + e % a.g) * 2 * w;
-        p[0] = p[w] = -INFINITY, p[1] = p[w + 1] = 0.f;
-      }
-      return;
-    }
-    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * per; e += (int64_t)s.spares * (NW * 64)) {
-      const int64_t i = e / per, o = ((s.q_end + i) * a.hk + kvh) * per + (e - i * per);
-      out[o] = (T)0.f;
-      if (o2) o2[o] = (T)0.f;
-    }
-    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; a.lse && e < rows * a.g; e += (int64_t)s.spares * (NW * 64)) {
-      const int64_t at = stat_at(a, kvh, 0, s.q_end, 0) + e;
-      a.lse[at] = a.lse[at + a.nq * a.g] = INFINITY;
-    }
+  if (s.tile < 0) {
+    zero_rows<T>(a, s, kvh, 128 * G);
     return;
   }
   const int row_base = s.tile * TILE;
   const int rows_here = a.stacked ? s.n : a.n;  // batch mode: rows beyond the length get zeros
   if (row_base >= rows_here * a.g) return;
-  const int r = row_base + (KEYS ? 0 : 32 * wave) + col;
+
+  // Q: B operand, lane = row, straight from global memory
+  const Row row = row_of(a, s, row_base + 32 * group + col);
+  Frag q[QS];
+  {
+    const int i0 = row_base / a.g;
+    const auto rq = buffer((const T*)a.q.data + s.b * a.q.batch_stride + ((a.stacked ? s.q0 : 0) + i0) * a.q.row_stride +
+                           ((int64_t)kvh * 2 * a.g + map) * a.q.head_stride);
+    const int o = (int)(((row.i - i0) * a.q.row_stride + 2 * row.h * a.q.head_stride) * (int)sizeof(T));
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      const int c = (2 * i + half) * kE<T>;
+      q[i] = load_frag<T>(rq, row.in && c < a.d ? o + c * (int)sizeof(T) : kOutside);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < QS; ++i) arrived(q[i]);
+  f32x16 acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = zero16();
+  float m = -INFINITY, l = 0.f;
+  bool huge = false;
+
+  const T* const kp = (const T*)a.k.data + s.b * a.k.batch_stride + (a.stacked ? s.k0 : 0) * a.k.row_stride + (int64_t)kvh * 2 * a.k.head_stride;
+  const T* const vp = (const T*)a.v.data + s.b * a.v.batch_stride + (a.stacked ? s.k0 : 0) * a.v.row_stride + (int64_t)kvh * a.v.head_stride;
+  const int off = s.m - s.n;  // causal: key j for query i iff j <= i + off
+  int begin = 0, end = s.m, seen = 0x7fffffff;  // seen: keys that all rows of this wave see
+  if (a.causal) {  // no key beyond the last row's limit
+    const int last = min(row_base + TILE, s.n * a.g) - 1;
+    end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
+    seen = (row_base + 32 * group) / a.g + off + 1;
+  }
+  if (a.splits > 1) split_keys(a, begin, end);
+
+  const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
+  // four waves load K, four (from the other end) V
+  const Stage<T, BN, 2, DB, 4> kst(a.d, krs, (int)(a.k.head_stride * sizeof(T)), wave, lane);
+  const Stage<T, BN, 1, DVB, 4> vst(a.dv, vrs, 0, 2 * G - 1 - wave, lane);
+  auto fill = [&](unsigned tile, int key0, uint64_t bits) GEOTR_INLINE {
+    if (G == 2 || wave < 4) kst.load(tile, words(kp + (int64_t)key0 * a.k.row_stride), krs, wave, bits);
+    if (G == 2 || wave >= 2 * G - 4) vst.load(tile + BN * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), vrs, 2 * G - 1 - wave, bits);
+  };
+
+  const Rows<T, CK, CK / 2> krow(col, half, map * (CK / 2));
+  const Cols<T, CV> vcol(lane);
+  const unsigned base = lds_at(smem);
+  auto scores = [&](unsigned tile, int key0, unsigned there) GEOTR_INLINE {
+    f32x16 x = zero16();
+#pragma unroll
+    for (int i = 0; i < QS; ++i) Ops<T>::mma(x, krow.get(tile, 0, i), q[i]);
+    if (there != 0xffffffffu || key0 + 32 > seen) {
+      const int above = a.causal ? row.i + off - key0 : 31;  // keys of the tile up to this one
+      unsigned lo = there;
+      if (above < 31) lo = above < 0 ? 0u : lo & ((2u << above) - 1);
+      lo >>= 4 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = (lo >> (8 * (i / 4) + i % 4)) & 1 ? x[i] : -INFINITY;
+    }
+    return x;
+  };
+  auto sum = [&](const f32x16& x) GEOTR_INLINE {
+    float u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = (x[i] + x[4 + i]) + (x[8 + i] + x[12 + i]);
+    return (u[0] + u[1]) + (u[2] + u[3]);
+  };
+  auto raise = [&](const f32x16& x) GEOTR_INLINE {  // the reference b to the maximum of scores x
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+    top = fmaxf(m, swap_max(top) * a.scale_log2);
+    const float c = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    m = top, l *= c;
+    huge = __any(fabsf(m) > kHuge && m > -INFINITY);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[i][j] *= c;
+  };
+  auto consume = [&](unsigned tile, int key0, unsigned there) GEOTR_INLINE {
+    const unsigned vt = tile + BN * CK * 16;
+    f32x16 p = scores(tile, key0, there);
+    float u;
+    if constexpr (kAgain) {
+      exponents(p, a.scale_log2, [&](int) { return m; }, huge);  // no reference yet: infinite
+      u = sum(p);
+      if (!__all(u < 256.f)) {
+        p = scores(tile, key0, there);
+        raise(p);
+        const float from = m == -INFINITY ? 0.f : m;  // no key yet: the weights are zero
+        exponents(p, a.scale_log2, [&](int) { return from; }, huge);
+        u = sum(p);
+      }
+    } else {
+      float top = p[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, p[i]);
+      if (__any(swap_max(top) * a.scale_log2 > m + 8.f)) raise(p);
+      const float from = m == -INFINITY ? 0.f : m;
+      exponents(p, a.scale_log2, [&](int) { return from; }, huge);
+      u = sum(p);
+    }
+    l += u;
+#pragma unroll
+    for (int x = 0; x < kPSteps<T>; ++x) {
+      const Frag w = pack<T>(p, x);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) Ops<T>::mma(acc[i], vcol.get(vt, 0, x, i), w);
+    }
+  };
+
+  // Tiles without a missing or masked row (the first `whole` keys) are loaded from descriptors that run along; the others look at every row
+  const int whole = a.masks ? begin : begin + (end - begin) / BN * BN;
+  i32x4 rk = words(kp + (int64_t)begin * a.k.row_stride), rv = words(vp + (int64_t)begin * a.v.row_stride);
+  uint64_t bits = 0;
+  auto next = [&](int key0, unsigned tile) GEOTR_INLINE {
+    if (key0 < whole) {
+      if (G == 2 || wave < 4) kst.load_all(tile, rk, krs, wave);
+      if (G == 2 || wave >= 2 * G - 4) vst.load_all(tile + BN * CK * 16, rv, vrs, 2 * G - 1 - wave);
+      rk = advance(rk, BN * krs), rv = advance(rv, BN * vrs);
+      return (uint64_t)0xffffffffull;
+    }
+    const uint64_t x = key0 < end ? key_bits(a, s, key0, end, lane) & 0xffffffffull : 0;
+    if (key0 < end) fill(tile, key0, x);
+    return x;
+  };
+  auto step = [&](int key0, unsigned tile, unsigned other) GEOTR_INLINE {
+    tile_ready();
+    __syncthreads();  // the tile is complete, and nobody reads the other buffer any more
+    const uint64_t now = bits;
+    bits = next(key0 + BN, other);
+    if (now) consume(tile, key0, (unsigned)now);
+  };
+  bits = next(begin, base);
+  for (int key0 = begin; key0 < end; key0 += 2 * BN) {  // two tiles: the buffers are constants of the addresses
+    step(key0, base, base + kTile);
+    if (key0 + BN < end) step(key0 + BN, base + kTile, base);
+  }
+
+  l = swap_add(l);
+  if (!row.in) m = -INFINITY, l = 0.f;
+  const int head = kvh * a.g + row.h;
+  if (a.splits > 1) {  // unnormalised, with its maximum and sum: (split, row, head, 2, 4 + dv)
+    if (row.i >= rows_here) return;
+    float* p = a.part + ((((int64_t)blockIdx.z * a.nq + s.q0 + row.i) * a.hk * a.g + head) * 2 + map) * (a.dv + 4);
+    if (half == 0) p[0] = m, p[1] = l;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = 32 * i + 8 * j + 4 * half;
+        if (c < a.dv) store4<float>(p + 4 + c, acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
+      }
+    return;
+  }
+  __syncthreads();
+  float* const box = (float*)smem + group * NT * 16 * 64 + lane;
+  const bool some = l != 0.f;  // false: no key, zero rows; a NaN stays one
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[i][j] = some ? acc[i][j] * inv : 0.f;
+  const int64_t at = s.q0 + row.i;
+  if (row.i < rows_here) {
+    if (a.lse && half == 0) a.lse[stat_at(a, kvh, map, at, row.h)] = some ? m + log2f(l) : INFINITY;
+    if (map == 1 && a.o2) {
+      T* const p = (T*)a.o2 + (at * a.hk * a.g + head) * a.dv;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = 32 * i + 8 * j + 4 * half;
+          if (c < a.dv) store4<T>(p + c, acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
+        }
+    }
+  }
+  if (map == 1) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) box[(i * 16 + j) * 64] = acc[i][j];
+  }
+  __syncthreads();
+  if (map == 1 || row.i >= rows_here) return;
+  const float lam = a.lam[head];
+  T* const p = (T*)a.out + (at * a.hk * a.g + head) * a.dv;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 32 * i + 8 * j + 4 * half;
+      if (c < a.dv) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = fmaf(-lam, box[(i * 16 + 4 * j + e) * 64], acc[i][4 * j + e]);
+        store4<T>(p + c, y[0], y[1], y[2], y[3]);
+      }
+    }
+}
+
+// Few rows (a token over a cache): the NW waves own the same 32 packed rows, both maps, and every wave streams key tiles of its own (no
+// barrier), joined at the end; with a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next launch.
+template <typename T, int DB, int DVB, int NW>
+__global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel(Args a) {
+  using Frag = typename Ops<T>::Frag;
+  constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>;
+  constexpr int BN = 32, TILE = 32, kTile = BN * (CK + CV) * 16, kJoin = (NW / 2) * 64 * (2 * NT * 16 + 4) * 4;
+  constexpr int kSmem = kTile * NW > kJoin ? kTile * NW : kJoin;
+  __shared__ __attribute__((aligned(1024))) char smem[kSmem];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+  const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
+  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
+  T* const out = (T*)a.out;
+  T* const o2 = (T*)a.o2;
+  if (s.tile < 0) {
+    zero_rows<T>(a, s, kvh, NW * 64);
+    return;
+  }
+  const int row_base = s.tile * TILE;
+  const int rows_here = a.stacked ? s.n : a.n;  // batch mode: rows beyond the length get zeros
+  if (row_base >= rows_here * a.g) return;
+  const int r = row_base + col;
   const Row row = row_of(a, s, r);
 
   // Q: B operand, lane = row, straight from global memory
@@ -374,6 +685,8 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_kernel(Args
       q2[i] = load_frag<T>(rq, in ? o + hs + c * (int)sizeof(T) : kOutside);
     }
   }
+#pragma unroll
+  for (int i = 0; i < QS; ++i) arrived(q1[i]), arrived(q2[i]);
   f32x16 acc1[NT], acc2[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc1[i] = zero16(), acc2[i] = zero16();
@@ -390,32 +703,24 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_kernel(Args
     end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
   }
   int begin = 0;
-  if (a.splits > 1) {
-    const int tiles = (end + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
-    begin = min(end, (int)blockIdx.z * per * 32);
-    end = min(end, begin + per * 32);
-  }
+  if (a.splits > 1) split_keys(a, begin, end);
 
-  constexpr int SHARE = KEYS ? 1 : NW;
-  const int w = KEYS ? 0 : wave;
-  auto fill = [&](char* tile, int key0, uint64_t bits) {
-    const auto rk = buffer(kp + (int64_t)key0 * a.k.row_stride);
-    const auto rv = buffer(vp + (int64_t)key0 * a.v.row_stride);
-    const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
-    const int hs = (int)(a.k.head_stride * sizeof(T));
-    if (bits == (BN == 64 ? ~0ull : 0xffffffffull)) {
-      stage<T, BN, 2, DB, SHARE, true>(tile, rk, a.d, hs, w, lane, [&](int x) { return x * krs; });
-      stage<T, BN, 1, DVB, SHARE, true>(tile + BN * CK * 16, rv, a.dv, 0, w, lane, [&](int x) { return x * vrs; });
+  const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T)), hs = (int)(a.k.head_stride * sizeof(T));
+  auto fill = [&](unsigned tile, int key0, uint64_t bits) GEOTR_INLINE {
+    const auto rk = words(kp + (int64_t)key0 * a.k.row_stride), rv = words(vp + (int64_t)key0 * a.v.row_stride);
+    if (bits == 0xffffffffull) {
+      stage_at<T, 32, 2, DB, 1>(tile, rk, a.d, hs, 0, lane, [&](int x) { return x * krs; });
+      stage_at<T, 32, 1, DVB, 1>(tile + BN * CK * 16, rv, a.dv, 0, 0, lane, [&](int x) { return x * vrs; });
     } else {
-      stage<T, BN, 2, DB, SHARE, false>(tile, rk, a.d, hs, w, lane, [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
-      stage<T, BN, 1, DVB, SHARE, false>(tile + BN * CK * 16, rv, a.dv, 0, w, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
+      stage_at<T, 32, 2, DB, 1>(tile, rk, a.d, hs, 0, lane, [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
+      stage_at<T, 32, 1, DVB, 1>(tile + BN * CK * 16, rv, a.dv, 0, 0, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
     }
   };
 
   const Rows<T, CK> krow(col, half);
   const Cols<T, CV> vcol(lane);
   // 32 keys of a staged tile
-  auto consume = [&](const char* at, int sub, int key0, uint64_t bits) {
+  auto consume = [&](const char* at, int sub, int key0, uint64_t bits) GEOTR_INLINE {
     const unsigned tile = lds_at(at), vt = tile + BN * CK * 16;
     f32x16 s1 = zero16(), s2 = zero16();
 #pragma unroll
@@ -468,39 +773,18 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_kernel(Args
     }
   };
 
-  if constexpr (KEYS) {
-    char* const mine = smem + wave * kTile;
-    for (int key0 = begin + 32 * wave; key0 < end; key0 += 32 * NW) {
-      const uint64_t bits = key_bits(a, s, key0, end, lane) & 0xffffffffull;
-      if (!bits) continue;
-      fill(mine, key0, bits);
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile is this wave's own
-      asm volatile("" ::: "memory");
-      consume(mine, 0, key0, bits);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-  } else {
-    int which = 0;
-    constexpr uint64_t kKeys = BN == 64 ? ~0ull : 0xffffffffull;
-    uint64_t bits = key_bits(a, s, begin, end, lane) & kKeys;
-    if (begin < end) fill(smem, begin, bits);
-    for (int key0 = begin; key0 < end; key0 += BN) {
-      __syncthreads();  // waits for this wave's loads: the tile is complete, and nobody reads the other buffer any more
-      uint64_t next = 0;
-      if (key0 + BN < end) {
-        next = key_bits(a, s, key0 + BN, end, lane) & kKeys;
-        fill(smem + (which ^ 1) * kTile, key0 + BN, next);
-      }
-#pragma unroll
-      for (int sub = 0; sub < BN / 32; ++sub)
-        if ((unsigned)(bits >> (32 * sub))) consume(smem + which * kTile, sub, key0, bits);
-      bits = next;
-      which ^= 1;
-    }
+  char* const mine = smem + wave * kTile;
+  for (int key0 = begin + 32 * wave; key0 < end; key0 += 32 * NW) {
+    const uint64_t bits = key_bits(a, s, key0, end, lane) & 0xffffffffull;
+    if (!bits) continue;
+    fill(lds_at(mine), key0, bits);
+    tile_ready();  // this wave's own: no barrier
+    consume(mine, 0, key0, bits);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 
   l1 = swap_add(l1), l2 = swap_add(l2);
-  if constexpr (KEYS) {  // join the waves' partials, the upper half of them through LDS, twice
+  {  // join the waves' partials, the upper half of them through LDS, twice
 #pragma unroll
     for (int step = NW / 2; step >= 1; step /= 2) {
       __syncthreads();
@@ -612,7 +896,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
   __shared__ __attribute__((aligned(1024))) char smem[NB * kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const int t = a.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
+  const int t = tile_order(a, blockIdx.y, gridDim.y, gridDim.x);
   const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
   T* const dq = (T*)a.gq;
   if (s.tile < 0) {
@@ -661,6 +945,11 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
     const int64_t st = stat_at(a, kvh, 0, at, row.h);
     lse1 = a.lse[st], lse2 = a.lse[st + a.nq * a.g], del1 = a.del[st], del2 = a.del[st + a.nq * a.g], lam = a.lam[head];
   }
+  arrived(lse1), arrived(lse2), arrived(del1), arrived(del2), arrived(lam);
+#pragma unroll
+  for (int i = 0; i < QS; ++i) arrived(q1[i]), arrived(q2[i]);
+#pragma unroll
+  for (int i = 0; i < VS; ++i) arrived(go[i]);
   const bool huge = __any((fabsf(lse1) > kHuge && lse1 < INFINITY) || (fabsf(lse2) > kHuge && lse2 < INFINITY));
   f32x16 acc1[ND], acc2[ND];
 #pragma unroll
@@ -676,23 +965,17 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
     const int last = min(row_base + TILE, s.n * a.g) - 1;
     end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
   }
-  auto fill = [&](char* tile, int key0, uint64_t bits) {
-    const auto rk = buffer(kp + (int64_t)key0 * a.k.row_stride);
-    const auto rv = buffer(vp + (int64_t)key0 * a.v.row_stride);
-    const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
-    const int hs = (int)(a.k.head_stride * sizeof(T));
-    if (bits == 0xffffffffull) {
-      stage<T, 32, 2, DB, NW, true>(tile, rk, a.d, hs, wave, lane, [&](int x) { return x * krs; });
-      stage<T, 32, 1, DVB, NW, true>(tile + 32 * CK * 16, rv, a.dv, 0, wave, lane, [&](int x) { return x * vrs; });
-    } else {
-      stage<T, 32, 2, DB, NW, false>(tile, rk, a.d, hs, wave, lane, [&](int x) { return (bits >> x) & 1 ? x * krs : kOutside; });
-      stage<T, 32, 1, DVB, NW, false>(tile + 32 * CK * 16, rv, a.dv, 0, wave, lane, [&](int x) { return (bits >> x) & 1 ? x * vrs : kOutside; });
-    }
+  const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
+  const Stage<T, 32, 2, DB, NW> kst(a.d, krs, (int)(a.k.head_stride * sizeof(T)), wave, lane);
+  const Stage<T, 32, 1, DVB, NW> vst(a.dv, vrs, 0, wave, lane);
+  auto fill = [&](unsigned tile, int key0, uint64_t bits) GEOTR_INLINE {
+    kst.load(tile, words(kp + (int64_t)key0 * a.k.row_stride), krs, wave, bits);
+    vst.load(tile + 32 * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), vrs, wave, bits);
   };
   const Rows<T, CK> krow(col, half);
   const Rows<T, CV> vrow(col, half);
   const Cols<T, CK> kcol(lane);
-  auto consume = [&](const char* at, int key0, uint64_t bits) {
+  auto consume = [&](const char* at, int key0, uint64_t bits) GEOTR_INLINE {
     const unsigned tile = lds_at(at), vt = tile + 32 * CK * 16;
     f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
 #pragma unroll
@@ -736,13 +1019,14 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
   if constexpr (NB == 2) {
     int which = 0;
     uint64_t bits = key_bits(a, s, 0, end, lane) & 0xffffffffull;
-    if (0 < end) fill(smem, 0, bits);
+    if (0 < end) fill(lds_at(smem), 0, bits);
     for (int key0 = 0; key0 < end; key0 += 32) {
+      tile_ready();
       __syncthreads();
       uint64_t next = 0;
       if (key0 + 32 < end) {
         next = key_bits(a, s, key0 + 32, end, lane) & 0xffffffffull;
-        fill(smem + (which ^ 1) * kTile, key0 + 32, next);
+        fill(lds_at(smem) + (which ^ 1) * kTile, key0 + 32, next);
       }
       if (bits) consume(smem + which * kTile, key0, bits);
       bits = next;
@@ -753,7 +1037,8 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       const uint64_t bits = key_bits(a, s, key0, end, lane) & 0xffffffffull;
       if (!bits) continue;
       __syncthreads();
-      fill(smem, key0, bits);
+      fill(lds_at(smem), key0, bits);
+      tile_ready();
       __syncthreads();
       consume(smem, key0, bits);
     }
@@ -824,11 +1109,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
                          (int64_t)kvh * a.v.head_stride);
   const int ok = (int)((32 * wave + col) * a.k.row_stride * (int)sizeof(T)), hs = (int)(a.k.head_stride * sizeof(T));
   const int ov = (int)((32 * wave + col) * a.v.row_stride * (int)sizeof(T));
-  auto k_frag = [&](int map, int i) {
+  auto k_frag = [&](int map, int i) GEOTR_INLINE {
     const int c = (2 * i + half) * kE<T>;
     return load_frag<T>(rk, in && c < a.d ? ok + map * hs + c * (int)sizeof(T) : kOutside);
   };
-  auto v_frag = [&](int i) {
+  auto v_frag = [&](int i) GEOTR_INLINE {
     const int c = (2 * i + half) * kE<T>;
     return load_frag<T>(rv, in && c < a.dv ? ov + c * (int)sizeof(T) : kOutside);
   };
@@ -838,6 +1123,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
     for (int i = 0; i < QS; ++i) k1[i] = k_frag(0, i), k2[i] = k_frag(1, i);
 #pragma unroll
     for (int i = 0; i < VS; ++i) vv[i] = v_frag(i);
+#pragma unroll
+    for (int i = 0; i < QS; ++i) arrived(k1[i]), arrived(k2[i]);
+#pragma unroll
+    for (int i = 0; i < VS; ++i) arrived(vv[i]);
   }
   f32x16 ak1[ND], ak2[ND], av[NV];
 #pragma unroll
@@ -859,15 +1148,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
   for (int r0 = first; r0 < rows; r0 += 32) {
     __syncthreads();
     const int i0 = a.g == 1 ? r0 : r0 / a.g;
-    const auto rq = buffer(qp + (int64_t)i0 * a.q.row_stride);
-    const auto ro = buffer(op + (int64_t)i0 * a.dout.row_stride);
-    auto q_off = [&](int x, int64_t rs, int64_t hstr) {
+    const auto rq = words(qp + (int64_t)i0 * a.q.row_stride);
+    const auto ro = words(op + (int64_t)i0 * a.dout.row_stride);
+    auto q_off = [&](int x, int64_t rs, int64_t hstr) GEOTR_INLINE {
       const int r = r0 + x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
       return r < rows ? (int)(((i - i0) * rs + h * hstr) * (int)sizeof(T)) : kOutside;
     };
-    stage<T, 32, 2, DB, NW, false>(smem, rq, a.d, (int)(a.q.head_stride * sizeof(T)), wave, lane,
+    stage_at<T, 32, 2, DB, NW>(lds_at(smem), rq, a.d, (int)(a.q.head_stride * sizeof(T)), wave, lane,
                         [&](int x) { return q_off(x, a.q.row_stride, 2 * a.q.head_stride); });
-    stage<T, 32, 1, DVB, NW, false>(smem + 32 * CQ * 16, ro, a.dv, 0, wave, lane,
+    stage_at<T, 32, 1, DVB, NW>(lds_at(smem) + 32 * CQ * 16, ro, a.dv, 0, wave, lane,
                          [&](int x) { return q_off(x, a.dout.row_stride, a.dout.head_stride); });
     if (threadIdx.x < 32) {
       const int r = r0 + threadIdx.x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
@@ -894,7 +1183,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
     for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, orow.get(ot, 0, i), kHold ? vv[i % (kHold ? VS : 1)] : v_frag(i));
     const bool huge = __builtin_amdgcn_readfirstlane(((const int*)st)[192]) != 0;
     f32x16 pj;
-    auto stat = [&](int which, int i) { return st[32 * which + 8 * (i / 4) + 4 * half + i % 4]; };
+    auto stat = [&](int which, int i) GEOTR_INLINE { return st[32 * which + 8 * (i / 4) + 4 * half + i % 4]; };
     exponents(s1, a.scale_log2, [&](int i) { return stat(0, i); }, huge);
     exponents(s2, a.scale_log2, [&](int i) { return stat(1, i); }, huge);
     if (a.causal && r0 < (key_base + TILE - 1 - off) * a.g) {  // a tile that some key of the block is not seen by
@@ -933,7 +1222,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
   T* const pk = dk + (at * a.hk + kvh) * 2 * a.d;
   T* const pv = dv + (at * a.hk + kvh) * a.dv;
   // a key that is masked or does not exist: zero, whatever its lane accumulated
-  auto out4 = [&](T* p, const f32x16& x, int j, float f) {
+  auto out4 = [&](T* p, const f32x16& x, int j, float f) GEOTR_INLINE {
     if (in) store4<T>(p, x[4 * j] * f, x[4 * j + 1] * f, x[4 * j + 2] * f, x[4 * j + 3] * f);
     else store4<T>(p, 0.f, 0.f, 0.f, 0.f);
   };
@@ -965,12 +1254,13 @@ template <typename T, int DB, int DVB>
 int launch_dims(const Args& a, Which which, hipStream_t s) {
   constexpr int NWK = 32 * (2 * DB + DVB) * (int)sizeof(T) * 4 <= 131072 ? 4 : 2;  // KEYS: a tile for every wave
   const bool fwd = which == kForward || which == kForwardKeys;
-  const int64_t tiles = tiles_of(a, which == kBackwardKV, which == kForwardKeys ? 32 : 128), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
+  constexpr int G = kGroups<T, DB, DVB>;
+  const int64_t tiles = tiles_of(a, which == kBackwardKV, which == kForwardKeys ? 32 : which == kForward ? 32 * G : 128), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
   if (tiles == 0 || x == 0) return GEOTR_OK;
   if (tiles > 65535 || x > 0x7fffffff) return fail(GEOTR_E_INVALID, "differential attention: %lld tiles of rows in one call", (long long)tiles);
   const dim3 grid((unsigned)x, (unsigned)tiles, fwd ? (unsigned)a.splits : 1u);
-  if (which == kForward) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, 4, false>), grid, dim3(256), 0, s, a);
-  else if (which == kForwardKeys) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, NWK, true>), grid, dim3(64 * NWK), 0, s, a);
+  if (which == kForward) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, G>), grid, dim3(128 * G), 0, s, a);
+  else if (which == kForwardKeys) hipLaunchKernelGGL((fwd_keys_kernel<T, DB, DVB, NWK>), grid, dim3(64 * NWK), 0, s, a);
   else if (which == kBackwardQ) hipLaunchKernelGGL((dq_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
   GEOTR_CHECK_LAUNCH("differential attention");
