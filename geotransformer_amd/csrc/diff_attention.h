@@ -15,8 +15,8 @@
 // accumulator a lane holds (16 of 32 contraction indices of ONE row) is the B operand of the next product as it stands: no exchange
 // between lanes and no LDS round trip for P and dS.  The other operand of that product is read transposed from LDS (ds_read_b64_tr_b16;
 // 32-bit: ds_read_b32 along the row), contraction indices in the same order: 8 (r / 4) + 4 half + r % 4 for accumulator register r.
-// A row of a head group: with g query heads to a key head the g heads of a query are g consecutive rows r = i g + h of the tile, so they
-// share every K and V fragment, and one query row over a long cache still fills g rows of the tile.
+// A row of a head group: with g query heads to a key head the heads of a query are consecutive rows r = (i << gsh) + h of the tile (g rounded
+// up to a power of two), so they share every K and V fragment, and one query row over a long cache still fills g rows of the tile.
 // Tiles go global -> LDS by 16-byte buffer loads (no registers), rows that do not exist or are masked and channels beyond D / Dv at an
 // offset past the buffer's end: the hardware writes zeros, so what a masked row holds (NaN included) never enters a product.  The chunk
 // order inside a row is permuted by the row (swizzle): row reads and transposed reads both spread over all banks.
@@ -31,18 +31,21 @@ using f32x16 = __attribute__((ext_vector_type(16))) float;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 #define GEOTR_LDS __attribute__((address_space(3)))
 #define GEOTR_INLINE __attribute__((always_inline))
+// LDS reads are not moved ahead over this (registers)
+#define GEOTR_FENCE __builtin_amdgcn_sched_barrier(0)
 
 struct Args {
   geotr_heads q, k, v, dout;             // dout: backward only
   void *out, *o2, *gq, *gk, *gv;         // contiguous (rows, heads, channels)
-  float *lse, *del, *part, *drow;        // (hk, 2, nq, g), (hk, 2, nq, g), split partials, (hk, nq, g)
+  float *lse, *part, *drow;              // (hk, 2, nq, g), split partials, (hk, nq, g)
+  float* rows;                           // backward, (hk, 5, nq, g): lse1, lse2 - log2 |lam|, del1, del2, sign of lam
   const float* amax;                     // 16-bit floats of narrow range: largest |dout| (backward), else null
   const float* lam;
   const int64_t *q_len, *k_len;
   const uint8_t* masks;                  // (nk) 1 = ignored key
   int64_t nq, nk;                        // all rows
   int batch, stacked, n, m;              // batch mode: n, m rows per sequence
-  int hk, g, d, dv, causal, splits;
+  int hk, g, gsh, d, dv, causal, splits; // query heads to a key head; packed rows r = (i << gsh) + h, h < g <= 1 << gsh
   float scale, scale_log2;
 };
 
@@ -80,8 +83,6 @@ template <typename T, int DB, int DVB>
 constexpr int kWaves = sizeof(T) * DB <= 128 ? 2 : 1;
 template <typename T, int DB, int DVB>
 constexpr int kWavesRows = sizeof(T) == 4 ? (DB <= 32 ? 3 : DB <= 64 ? 2 : 1) : DVB <= 64 ? 4 : DVB <= 128 ? 3 : 2;
-template <typename T, int DB, int DVB>
-constexpr int kGroups = 2;
 
 // fragment t of the accumulator's 32 contraction indices: registers E t .. E t + E - 1 (rounded to T: the one rounding of P and dS)
 template <typename T>
@@ -201,46 +202,43 @@ __device__ __forceinline__ typename Ops<T>::Frag load_frag(__amdgpu_buffer_rsrc_
   return __builtin_bit_cast(typename Ops<T>::Frag, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
 }
 
-// ROWS rows of NM maps of `width` channels (bucket DB) from rows of rs bytes into a tile, dealt over the SHARE waves that use it (wave w of
-// them).  A step of the waves covers S rows; the swizzle repeats after 16 (and is linear over xor), so a lane keeps one offset for each of
-// NB steps and reaches the others by a scalar: no vector arithmetic per load where every row exists.
+// ROWS rows of NM maps of `width` channels (bucket DB) into a tile, dealt over the SHARE waves that use it (wave w of them).  row_at(row)
+// is a row's byte offset, and 16 rows further on it is rs16 more.  A step of the waves covers S rows; the swizzle repeats after 16 (and is
+// linear over xor), so a lane keeps one offset for each of NB steps and reaches the others by a scalar: no vector arithmetic per load
+// where every row exists.
 template <typename T, int ROWS, int NM, int DB, int SHARE>
 struct Stage {
   static constexpr int CM = DB * (int)sizeof(T) / 16, C = NM * CM, N = ROWS * C / 64, S = SHARE * 64 / C > 0 ? SHARE * 64 / C : 1;
   static constexpr int NS = (N + SHARE - 1) / SHARE, NB = C < 16 || S >= 16 ? 1 : 16 / S < NS ? 16 / S : NS;
   static_assert(ROWS * C % 64 == 0 && C <= 64, "whole wave loads");
   int base[NB], row0;
-  __device__ __forceinline__ Stage(int width, int rs, int map_bytes, int w, int lane) {
+  template <class At>
+  __device__ __forceinline__ Stage(int width, int map_bytes, int w, int lane, At row_at) {
     const int p = w * 64 + lane;
     row0 = p / C;
     const int pos = (p % C) ^ swz<C>(row0);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int c = pos ^ swz<C>(j * S), map = NM == 1 ? 0 : c / CM, cc = NM == 1 ? c : c % CM;
-      base[j] = cc * kE<T> >= width ? kOutside : (j * S + row0) * rs + map * map_bytes + cc * 16;
+      base[j] = cc * kE<T> >= width ? kOutside : row_at(j * S + row0) + map * map_bytes + cc * 16;
     }
   }
   template <class Row>
-  __device__ __forceinline__ void load(unsigned tile, i32x4 r, int rs, int w, Row row) const {
+  __device__ __forceinline__ void load_some(unsigned tile, i32x4 r, int rs16, int w, Row row) const {
 #pragma unroll
     for (int it = 0; it < NS; ++it) {
       if (N % SHARE != 0 && it * SHARE + w >= N) break;
-      const int j = it % NB;
-      load_lds(r, tile + (it * SHARE + w) * 1024, row(it * S + row0) ? base[j] : kOutside, (it - j) * S * rs);
+      load_lds(r, tile + (it * SHARE + w) * 1024, row(it * S + row0) ? base[it % NB] : kOutside, (it - it % NB) * S * (rs16 / 16));
     }
   }
-  // every row exists; the descriptor's base runs along
-  __device__ __forceinline__ void load_all(unsigned tile, i32x4 r, int rs, int w) const {
-#pragma unroll
-    for (int it = 0; it < NS; ++it) {
-      if (N % SHARE != 0 && it * SHARE + w >= N) break;
-      load_lds(r, tile + (it * SHARE + w) * 1024, base[it % NB], (it - it % NB) * S * rs);
-    }
+  // every row exists
+  __device__ __forceinline__ void load_all(unsigned tile, i32x4 r, int rs16, int w) const {
+    load_some(tile, r, rs16, w, [](int) { return true; });
   }
   // rows `bits` of the tile
-  __device__ __forceinline__ void load(unsigned tile, i32x4 r, int rs, int w, uint64_t bits) const {
-    if (bits == (ROWS == 64 ? ~0ull : 0xffffffffull)) load(tile, r, rs, w, [](int) { return true; });
-    else load(tile, r, rs, w, [&](int x) { return (bits >> x) & 1; });
+  __device__ __forceinline__ void load(unsigned tile, i32x4 r, int rs16, int w, uint64_t bits) const {
+    if (bits == (ROWS == 64 ? ~0ull : 0xffffffffull)) load_all(tile, r, rs16, w);
+    else load_some(tile, r, rs16, w, [&](int x) { return (bits >> x) & 1; });
   }
 };
 
@@ -291,7 +289,7 @@ __device__ __forceinline__ Seq find_seq(const Args& a, int b, int t, int tiles) 
     const int i = b0 + lane;
     int ql = i < a.batch ? clamp_len(a.q_len[i], a.nq) : 0, kl = i < a.batch ? clamp_len(a.k_len[i], a.nk) : 0;
     const int ql0 = ql, kl0 = kl;
-    int tl = KEYS ? (kl + TILE - 1) / TILE : (int)(((int64_t)ql * a.g + TILE - 1) / TILE);
+    int tl = KEYS ? (kl + TILE - 1) / TILE : (int)((((int64_t)ql << a.gsh) + TILE - 1) / TILE);
     const int tl0 = tl;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -360,20 +358,25 @@ __device__ __forceinline__ void exponents(f32x16& s, float c, B b, bool huge) {
   for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
 }
 
-// One packed query row of a lane: its query, head within the group, and whether it exists
+// One packed query row of a lane: its query, head within the group, whether it exists and whether it is written (batch mode: rows beyond
+// their sequence's length get zeros)
 struct Row {
   int i, h;
-  bool in;
+  bool in, out;
 };
 __device__ __forceinline__ Row row_of(const Args& a, const Seq& s, int r) {
   Row x;
-  x.i = a.g == 1 ? r : r / a.g;
-  x.h = a.g == 1 ? 0 : r - x.i * a.g;
-  x.in = r < s.n * a.g;
+  x.i = r >> a.gsh, x.h = r & ((1 << a.gsh) - 1);
+  x.in = x.i < s.n && x.h < a.g;
+  x.out = x.i < (a.stacked ? s.n : a.n) && x.h < a.g;
   return x;
 }
 __device__ __forceinline__ int64_t stat_at(const Args& a, int kvh, int map, int64_t row, int h) {
   return (((int64_t)kvh * 2 + map) * a.nq + row) * a.g + h;
+}
+
+__device__ __forceinline__ int64_t row_stat_at(const Args& a, int kvh, int which, int64_t row, int h) {
+  return (((int64_t)kvh * 5 + which) * a.nq + row) * a.g + h;
 }
 
 // four consecutive channels of an output row
@@ -425,16 +428,17 @@ __device__ __forceinline__ void zero_rows(const Args& a, const Seq& s, int kvh, 
 // waves to a SIMD unit at d = 64, v 128, where both maps in a wave leave one) and the maps meet in LDS at the end.  Tiles of 32 keys in two
 // buffers: the next one loads while this one is consumed.
 // The accumulators are rescaled only when a row's maximum grew by more than 2^8: weights stay below 2^8, sums are exact either way.
-template <typename T, int DB, int DVB, int G>
+// FEW (a token over a cache, wide heads): the G groups share 32 rows and take 32 keys each of every tile, joined at the end.
+template <typename T, int DB, int DVB, int G, bool FEW>
 __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
-  constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>, TILE = 32 * G;
-  constexpr int BN = 32, kTile = BN * (CK + CV) * 16, kJoin = G * NT * 16 * 64 * 4;
+  constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>, TILE = FEW ? 32 : 32 * G;
+  constexpr int BN = FEW ? 32 * G : 32, kTile = BN * (CK + CV) * 16, kJoin = G * (NT * 16 + 2) * 64 * 4;
   constexpr int kSmem = 2 * kTile > kJoin ? 2 * kTile : kJoin;
   constexpr bool kAgain = NT * 16 + QS * 4 <= 80;  // registers left for computing scores again
   __shared__ __attribute__((aligned(1024))) char smem[kSmem];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-  const int map = wave & 1, group = wave >> 1;
+  const int map = wave & 1, group = wave >> 1, rows_at = FEW ? 0 : 32 * group;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
   const int t = tile_order(a, blockIdx.y, gridDim.y, gridDim.x);
   const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
@@ -443,14 +447,13 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
     return;
   }
   const int row_base = s.tile * TILE;
-  const int rows_here = a.stacked ? s.n : a.n;  // batch mode: rows beyond the length get zeros
-  if (row_base >= rows_here * a.g) return;
+  if (row_base >> a.gsh >= (a.stacked ? s.n : a.n)) return;
 
   // Q: B operand, lane = row, straight from global memory
-  const Row row = row_of(a, s, row_base + 32 * group + col);
+  const Row row = row_of(a, s, row_base + rows_at + col);
   Frag q[QS];
   {
-    const int i0 = row_base / a.g;
+    const int i0 = row_base >> a.gsh;
     const auto rq = buffer((const T*)a.q.data + s.b * a.q.batch_stride + ((a.stacked ? s.q0 : 0) + i0) * a.q.row_stride +
                            ((int64_t)kvh * 2 * a.g + map) * a.q.head_stride);
     const int o = (int)(((row.i - i0) * a.q.row_stride + 2 * row.h * a.q.head_stride) * (int)sizeof(T));
@@ -473,19 +476,19 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
   const int off = s.m - s.n;  // causal: key j for query i iff j <= i + off
   int begin = 0, end = s.m, seen = 0x7fffffff;  // seen: keys that all rows of this wave see
   if (a.causal) {  // no key beyond the last row's limit
-    const int last = min(row_base + TILE, s.n * a.g) - 1;
-    end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
-    seen = (row_base + 32 * group) / a.g + off + 1;
+    const int last = min((row_base + TILE - 1) >> a.gsh, s.n - 1);
+    end = min(end, max(0, last + off + 1));
+    seen = ((row_base + rows_at) >> a.gsh) + off + 1;
   }
   if (a.splits > 1) split_keys(a, begin, end);
 
   const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
   // four waves load K, four (from the other end) V
-  const Stage<T, BN, 2, DB, 4> kst(a.d, krs, (int)(a.k.head_stride * sizeof(T)), wave, lane);
-  const Stage<T, BN, 1, DVB, 4> vst(a.dv, vrs, 0, 2 * G - 1 - wave, lane);
+  const Stage<T, BN, 2, DB, 4> kst(a.d, (int)(a.k.head_stride * sizeof(T)), wave, lane, [&](int x) { return x * krs; });
+  const Stage<T, BN, 1, DVB, 4> vst(a.dv, 0, 2 * G - 1 - wave, lane, [&](int x) { return x * vrs; });
   auto fill = [&](unsigned tile, int key0, uint64_t bits) GEOTR_INLINE {
-    if (G == 2 || wave < 4) kst.load(tile, words(kp + (int64_t)key0 * a.k.row_stride), krs, wave, bits);
-    if (G == 2 || wave >= 2 * G - 4) vst.load(tile + BN * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), vrs, 2 * G - 1 - wave, bits);
+    if (G == 2 || wave < 4) kst.load(tile, words(kp + (int64_t)key0 * a.k.row_stride), 16 * krs, wave, bits);
+    if (G == 2 || wave >= 2 * G - 4) vst.load(tile + BN * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), 16 * vrs, 2 * G - 1 - wave, bits);
   };
 
   const Rows<T, CK, CK / 2> krow(col, half, map * (CK / 2));
@@ -524,8 +527,7 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[i][j] *= c;
   };
-  auto consume = [&](unsigned tile, int key0, unsigned there) GEOTR_INLINE {
-    const unsigned vt = tile + BN * CK * 16;
+  auto consume = [&](unsigned tile, unsigned vt, int key0, unsigned there) GEOTR_INLINE {
     f32x16 p = scores(tile, key0, there);
     float u;
     if constexpr (kAgain) {
@@ -559,15 +561,16 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
   // Tiles without a missing or masked row (the first `whole` keys) are loaded from descriptors that run along; the others look at every row
   const int whole = a.masks ? begin : begin + (end - begin) / BN * BN;
   i32x4 rk = words(kp + (int64_t)begin * a.k.row_stride), rv = words(vp + (int64_t)begin * a.v.row_stride);
+  constexpr uint64_t kAll = BN == 64 ? ~0ull : 0xffffffffull;
   uint64_t bits = 0;
   auto next = [&](int key0, unsigned tile) GEOTR_INLINE {
     if (key0 < whole) {
-      if (G == 2 || wave < 4) kst.load_all(tile, rk, krs, wave);
-      if (G == 2 || wave >= 2 * G - 4) vst.load_all(tile + BN * CK * 16, rv, vrs, 2 * G - 1 - wave);
+      if (G == 2 || wave < 4) kst.load_all(tile, rk, 16 * krs, wave);
+      if (G == 2 || wave >= 2 * G - 4) vst.load_all(tile + BN * CK * 16, rv, 16 * vrs, 2 * G - 1 - wave);
       rk = advance(rk, BN * krs), rv = advance(rv, BN * vrs);
-      return (uint64_t)0xffffffffull;
+      return kAll;
     }
-    const uint64_t x = key0 < end ? key_bits(a, s, key0, end, lane) & 0xffffffffull : 0;
+    const uint64_t x = key0 < end ? key_bits(a, s, key0, end, lane) & kAll : 0;
     if (key0 < end) fill(tile, key0, x);
     return x;
   };
@@ -576,7 +579,11 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
     __syncthreads();  // the tile is complete, and nobody reads the other buffer any more
     const uint64_t now = bits;
     bits = next(key0 + BN, other);
-    if (now) consume(tile, key0, (unsigned)now);
+    if constexpr (FEW) {
+      if ((unsigned)(now >> (32 * group))) consume(tile + group * 32 * CK * 16, tile + BN * CK * 16 + group * 32 * CV * 16, key0 + 32 * group, (unsigned)(now >> (32 * group)));
+    } else {
+      if (now) consume(tile, tile + BN * CK * 16, key0, (unsigned)now);
+    }
   };
   bits = next(begin, base);
   for (int key0 = begin; key0 < end; key0 += 2 * BN) {  // two tiles: the buffers are constants of the addresses
@@ -585,10 +592,34 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
   }
 
   l = swap_add(l);
+  if constexpr (FEW) {  // the other groups' sums and accumulators through LDS
+    static_assert(!FEW || G == 2, "one other group");
+    float* const box = (float*)smem + map * (NT * 16 + 2) * 64 + lane;
+    __syncthreads();
+    if (group == 1) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) box[(i * 16 + j) * 64] = acc[i][j];
+      box[NT * 16 * 64] = m, box[(NT * 16 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (group == 0) {
+      const float om = box[NT * 16 * 64], n = fmaxf(m, om), u = n == -INFINITY ? 0.f : n;
+      const float c = __builtin_amdgcn_exp2f(m - u), o = __builtin_amdgcn_exp2f(om - u);
+      l = l * c + box[(NT * 16 + 1) * 64] * o;
+      m = n;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[i][j] = acc[i][j] * c + box[(i * 16 + j) * 64] * o;
+    }
+  }
   if (!row.in) m = -INFINITY, l = 0.f;
+  const bool mine = !FEW || group == 0;
   const int head = kvh * a.g + row.h;
   if (a.splits > 1) {  // unnormalised, with its maximum and sum: (split, row, head, 2, 4 + dv)
-    if (row.i >= rows_here) return;
+    if (!row.out || !mine) return;
     float* p = a.part + ((((int64_t)blockIdx.z * a.nq + s.q0 + row.i) * a.hk * a.g + head) * 2 + map) * (a.dv + 4);
     if (half == 0) p[0] = m, p[1] = l;
 #pragma unroll
@@ -601,7 +632,7 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
     return;
   }
   __syncthreads();
-  float* const box = (float*)smem + group * NT * 16 * 64 + lane;
+  float* const box = (float*)smem + (FEW ? 0 : group) * NT * 16 * 64 + lane;
   const bool some = l != 0.f;  // false: no key, zero rows; a NaN stays one
   const float inv = 1.f / l;
 #pragma unroll
@@ -609,7 +640,7 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i][j] = some ? acc[i][j] * inv : 0.f;
   const int64_t at = s.q0 + row.i;
-  if (row.i < rows_here) {
+  if (row.out && mine) {
     if (a.lse && half == 0) a.lse[stat_at(a, kvh, map, at, row.h)] = some ? m + log2f(l) : INFINITY;
     if (map == 1 && a.o2) {
       T* const p = (T*)a.o2 + (at * a.hk * a.g + head) * a.dv;
@@ -622,14 +653,14 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
         }
     }
   }
-  if (map == 1) {
+  if (map == 1 && mine) {
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) box[(i * 16 + j) * 64] = acc[i][j];
   }
   __syncthreads();
-  if (map == 1 || row.i >= rows_here) return;
+  if (map == 1 || !row.out || !mine) return;
   const float lam = a.lam[head];
   T* const p = (T*)a.out + (at * a.hk * a.g + head) * a.dv;
 #pragma unroll
@@ -665,8 +696,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
     return;
   }
   const int row_base = s.tile * TILE;
-  const int rows_here = a.stacked ? s.n : a.n;  // batch mode: rows beyond the length get zeros
-  if (row_base >= rows_here * a.g) return;
+  if (row_base >> a.gsh >= (a.stacked ? s.n : a.n)) return;
   const int r = row_base + col;
   const Row row = row_of(a, s, r);
 
@@ -674,8 +704,8 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
   Frag q1[QS], q2[QS];
   {
     const auto rq = buffer((const T*)a.q.data + s.b * a.q.batch_stride + (a.stacked ? s.q0 : 0) * a.q.row_stride +
-                           (int64_t)kvh * 2 * a.g * a.q.head_stride + (int64_t)(row_base / a.g) * a.q.row_stride);
-    const int o = (int)(((row.i - row_base / a.g) * a.q.row_stride + 2 * row.h * a.q.head_stride) * (int)sizeof(T));
+                           (int64_t)kvh * 2 * a.g * a.q.head_stride + (int64_t)(row_base >> a.gsh) * a.q.row_stride);
+    const int o = (int)(((row.i - (row_base >> a.gsh)) * a.q.row_stride + 2 * row.h * a.q.head_stride) * (int)sizeof(T));
     const int hs = (int)(a.q.head_stride * sizeof(T));
 #pragma unroll
     for (int i = 0; i < QS; ++i) {
@@ -699,8 +729,8 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
   const int limit = a.causal ? row.i + off : 0x7fffffff;
   int end = s.m;
   if (a.causal) {  // no key beyond the last row's limit
-    const int last = min(row_base + TILE, s.n * a.g) - 1;
-    end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
+    const int last = min((row_base + TILE - 1) >> a.gsh, s.n - 1);
+    end = min(end, max(0, last + off + 1));
   }
   int begin = 0;
   if (a.splits > 1) split_keys(a, begin, end);
@@ -818,7 +848,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
     if (wave) return;
   }
 
-  if (r >= rows_here * a.g) return;
+  if (!row.out) return;
   if (!row.in) m1 = m2 = -INFINITY, l1 = l2 = 0.f;
   const int64_t at = s.q0 + row.i;
   const int head = kvh * a.g + row.h;
@@ -910,8 +940,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
     return;
   }
   const int row_base = s.tile * TILE;
-  const int rows_here = a.stacked ? s.n : a.n;
-  if (row_base >= rows_here * a.g) return;
+  if (row_base >> a.gsh >= (a.stacked ? s.n : a.n)) return;
   const int r = row_base + 32 * wave + col;
   const Row row = row_of(a, s, r);
   const int64_t at = s.q0 + row.i;
@@ -920,7 +949,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
 
   Frag q1[QS], q2[QS], go[VS];
   {
-    const int i0 = row_base / a.g;
+    const int i0 = row_base >> a.gsh;
     const auto rq = buffer((const T*)a.q.data + s.b * a.q.batch_stride + ((a.stacked ? s.q0 : 0) + i0) * a.q.row_stride +
                            (int64_t)kvh * 2 * a.g * a.q.head_stride);
     const auto ro = buffer((const T*)a.dout.data + s.b * a.dout.batch_stride + ((a.stacked ? s.q0 : 0) + i0) * a.dout.row_stride +
@@ -943,7 +972,9 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
   float lse1 = INFINITY, lse2 = INFINITY, del1 = 0.f, del2 = 0.f, lam = 0.f;
   if (row.in) {
     const int64_t st = stat_at(a, kvh, 0, at, row.h);
-    lse1 = a.lse[st], lse2 = a.lse[st + a.nq * a.g], del1 = a.del[st], del2 = a.del[st + a.nq * a.g], lam = a.lam[head];
+    lse1 = a.lse[st], lse2 = a.lse[st + a.nq * a.g], lam = a.lam[head];
+    const int64_t rs = row_stat_at(a, kvh, 2, at, row.h);
+    del1 = a.rows[rs], del2 = a.rows[rs + a.nq * a.g];
   }
   arrived(lse1), arrived(lse2), arrived(del1), arrived(del2), arrived(lam);
 #pragma unroll
@@ -962,15 +993,15 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
   const int limit = a.causal ? row.i + off : 0x7fffffff;
   int end = s.m;
   if (a.causal) {
-    const int last = min(row_base + TILE, s.n * a.g) - 1;
-    end = min(end, max(0, (last < 0 ? -1 : last / a.g) + off + 1));
+    const int last = min((row_base + TILE - 1) >> a.gsh, s.n - 1);
+    end = min(end, max(0, last + off + 1));
   }
   const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
-  const Stage<T, 32, 2, DB, NW> kst(a.d, krs, (int)(a.k.head_stride * sizeof(T)), wave, lane);
-  const Stage<T, 32, 1, DVB, NW> vst(a.dv, vrs, 0, wave, lane);
+  const Stage<T, 32, 2, DB, NW> kst(a.d, (int)(a.k.head_stride * sizeof(T)), wave, lane, [&](int x) { return x * krs; });
+  const Stage<T, 32, 1, DVB, NW> vst(a.dv, 0, wave, lane, [&](int x) { return x * vrs; });
   auto fill = [&](unsigned tile, int key0, uint64_t bits) GEOTR_INLINE {
-    kst.load(tile, words(kp + (int64_t)key0 * a.k.row_stride), krs, wave, bits);
-    vst.load(tile + 32 * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), vrs, wave, bits);
+    kst.load(tile, words(kp + (int64_t)key0 * a.k.row_stride), 16 * krs, wave, bits);
+    vst.load(tile + 32 * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), 16 * vrs, wave, bits);
   };
   const Rows<T, CK> krow(col, half);
   const Rows<T, CV> vrow(col, half);
@@ -1003,7 +1034,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
     for (int i = 0; i < 16; ++i) {
       const float p1 = s1[i], p2 = s2[i];
       dsum = fmaf(p2, dp[i], dsum);
-      s1[i] = p1 * (dp[i] - del1), s2[i] = -lam * p2 * (dp[i] - del2);
+      s1[i] = p1 * (dp[i] - del1), s2[i] = p2 * (dp[i] - del2);
       if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs;
     }
 #pragma unroll
@@ -1043,11 +1074,11 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       consume(smem, key0, bits);
     }
   }
-  if (r >= rows_here * a.g) return;
+  if (!row.out) return;
   dsum = swap_add(dsum);
   if (!row.in) dsum = 0.f;
   if (half == 0) a.drow[((int64_t)kvh * a.nq + at) * a.g + row.h] = dsum;
-  const float f = a.scale / gs;
+  const float f = a.scale / gs, f2 = -lam * f;
   T* const p1 = dq + (at * a.hk * a.g + head) * 2 * a.d;
 #pragma unroll
   for (int i = 0; i < ND; ++i)
@@ -1057,7 +1088,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       if (c < a.d) {
         if (row.in) {
           store4<T>(p1 + c, acc1[i][4 * j] * f, acc1[i][4 * j + 1] * f, acc1[i][4 * j + 2] * f, acc1[i][4 * j + 3] * f);
-          store4<T>(p1 + a.d + c, acc2[i][4 * j] * f, acc2[i][4 * j + 1] * f, acc2[i][4 * j + 2] * f, acc2[i][4 * j + 3] * f);
+          store4<T>(p1 + a.d + c, acc2[i][4 * j] * f2, acc2[i][4 * j + 1] * f2, acc2[i][4 * j + 2] * f2, acc2[i][4 * j + 3] * f2);
         } else {
           store4<T>(p1 + c, 0.f, 0.f, 0.f, 0.f);
           store4<T>(p1 + a.d + c, 0.f, 0.f, 0.f, 0.f);
@@ -1067,17 +1098,27 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
 }
 
 // ---- backward: keys (dK, dV) --------------------------------------------------------------------------------------------------------------
-// A wave owns 32 keys; K and V are the B operands (lane = key), in registers where they fit beside the accumulators (16-bit types), else
-// read again from memory for every tile of 32 packed query rows (32-bit: a product takes 16 times as long as its operand's load).
-template <typename T, int DB, int DVB, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_kernel(Args a) {
+// A wave owns 32 keys; K and V are the B operands (lane = key).  They stay in registers as far as two waves to a SIMD unit allow, V else in
+// LDS; 32-bit wide heads read them again from memory for every tile of 32 packed query rows (a product takes 16 times as long as the load).
+// Where both gradients' accumulators leave no registers (16-bit heads of 128, values of 256) dK and dV are two launches, the scores twice:
+// 20 instead of 16 products of d, 334 instead of 462 us at 2 x 2 048 rows and 4 heads.  Narrower heads lose by it (64, 128: 370 against
+// 274 us at 2 x 4 096 causal rows and 8 heads).
+enum Part { kBoth, kKeysOnly, kValuesOnly };
+template <typename T, int DVB>
+constexpr bool kSplitKV = sizeof(T) == 2 && DVB == 256;
+template <typename T, int DB, int DVB, int PART>
+constexpr int kWavesKV = DB <= 32 ? 2 : 1;
+template <typename T, int DB, int DVB, int NW, int PART>
+__global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CQ = 2 * DB * (int)sizeof(T) / 16, CO = DVB * (int)sizeof(T) / 16, ND = DB / 32, NV = DVB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
-  constexpr bool kHold = sizeof(T) == 2;
-  constexpr int kStats = 32 * 6 * 4 + 16;  // lse1, lse2, del1, del2, lam, limit of a tile's rows; whether a score is huge
-  constexpr int kTile = 32 * (CQ + CO) * 16, TILE = 32 * NW;
-  __shared__ __attribute__((aligned(1024))) char smem[kTile + kStats];
-  float* const st = (float*)(smem + kTile);
+  constexpr bool kHold = sizeof(T) == 2, kHoldV = PART != kValuesOnly && kHold && (int)sizeof(T) * DB <= 128,
+                 kLdsV = PART != kValuesOnly && kHold && !kHoldV;
+  constexpr bool DK = PART != kValuesOnly, DV = PART != kKeysOnly;
+  constexpr int kRowBytes = 32 * (CQ + CO) * 16, kTile = kRowBytes + 1024, TILE = 32 * NW;  // 6 x 32 numbers of the rows behind them
+  constexpr int NB = 2 * kTile <= 140000 ? 2 : 1;
+
+  __shared__ __attribute__((aligned(1024))) char smem[NB * kTile + (kLdsV ? TILE * CO * 16 : 0)];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
   const Seq s = find_seq<TILE, true>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
@@ -1085,11 +1126,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
   T* const dv = (T*)a.gv;
   if (s.tile < 0) {
     const int64_t rows = s.k_end < a.nk ? a.nk - s.k_end : 0;
-    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * (2 * a.d); e += (int64_t)s.spares * (NW * 64)) {
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; DK && e < rows * (2 * a.d); e += (int64_t)s.spares * (NW * 64)) {
       const int64_t i = e / (2 * a.d);
       dk[((s.k_end + i) * a.hk + kvh) * 2 * a.d + (e - i * 2 * a.d)] = (T)0.f;
     }
-    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; e < rows * a.dv; e += (int64_t)s.spares * (NW * 64)) {
+    for (int64_t e = (int64_t)s.spare * (NW * 64) + threadIdx.x; DV && e < rows * a.dv; e += (int64_t)s.spares * (NW * 64)) {
       const int64_t i = e / a.dv;
       dv[((s.k_end + i) * a.hk + kvh) * a.dv + (e - i * a.dv)] = (T)0.f;
     }
@@ -1117,103 +1158,175 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
     const int c = (2 * i + half) * kE<T>;
     return load_frag<T>(rv, in && c < a.dv ? ov + c * (int)sizeof(T) : kOutside);
   };
-  Frag k1[kHold ? QS : 1], k2[kHold ? QS : 1], vv[kHold ? VS : 1];
+  Frag k1[kHold ? QS : 1], k2[kHold ? QS : 1], vv[kHoldV ? VS : 1];
   if constexpr (kHold) {
 #pragma unroll
     for (int i = 0; i < QS; ++i) k1[i] = k_frag(0, i), k2[i] = k_frag(1, i);
 #pragma unroll
-    for (int i = 0; i < VS; ++i) vv[i] = v_frag(i);
-#pragma unroll
     for (int i = 0; i < QS; ++i) arrived(k1[i]), arrived(k2[i]);
+  }
+  if constexpr (kHoldV) {
+#pragma unroll
+    for (int i = 0; i < VS; ++i) vv[i] = v_frag(i);
 #pragma unroll
     for (int i = 0; i < VS; ++i) arrived(vv[i]);
   }
-  f32x16 ak1[ND], ak2[ND], av[NV];
+  const unsigned vt = lds_at(smem) + NB * kTile + wave * 32 * CO * 16;  // this wave's keys of V
+  if constexpr (kLdsV) {
+    const i32x4 r = words((const T*)a.v.data + s.b * a.v.batch_stride + ((a.stacked ? s.k0 : 0) + key_base + 32 * wave) * a.v.row_stride +
+                          (int64_t)kvh * a.v.head_stride);
+    const unsigned there = (unsigned)__ballot(in);
+    stage_at<T, 32, 1, DVB, 1>(vt, r, a.dv, 0, 0, lane, [&](int x) GEOTR_INLINE {
+      return (there >> x) & 1 ? x * (int)(a.v.row_stride * sizeof(T)) : kOutside;
+    });
+  }
+  f32x16 ak1[DK ? ND : 1], ak2[DK ? ND : 1], av[DV ? NV : 1];
+  if constexpr (DK) {
 #pragma unroll
-  for (int i = 0; i < ND; ++i) ak1[i] = zero16(), ak2[i] = zero16();
+    for (int i = 0; i < ND; ++i) ak1[i] = zero16(), ak2[i] = zero16();
+  }
+  if constexpr (DV) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) av[i] = zero16();
+    for (int i = 0; i < NV; ++i) av[i] = zero16();
+  }
 
   const int off = s.m - s.n;
-  const int rows = s.n * a.g;
+  const int rows = s.n << a.gsh;
   int first = 0;
-  if (a.causal) first = min(s.n, max(0, key_base - off)) * a.g / 32 * 32;  // rows before see none of these keys
+  if (a.causal) first = (min(s.n, max(0, key_base - off)) << a.gsh) / 32 * 32;  // rows before see none of these keys
+  // key j is seen by query i iff j <= i + off, by packed row r iff (j - off) << gsh <= r
+  const int from = a.causal ? min(key - off, s.n) * (1 << a.gsh) : 0, last = a.causal ? min(key_base + TILE - 1 - off, s.n) * (1 << a.gsh) : 0;
+  bool minus = false;
+  for (int h = 0; h < a.g; ++h) minus |= a.lam[kvh * a.g + h] < 0.f;
+
   const T* const qp = (const T*)a.q.data + s.b * a.q.batch_stride + (a.stacked ? s.q0 : 0) * a.q.row_stride + (int64_t)kvh * 2 * a.g * a.q.head_stride;
   const T* const op = (const T*)a.dout.data + s.b * a.dout.batch_stride + (a.stacked ? s.q0 : 0) * a.dout.row_stride +
                       (int64_t)kvh * a.g * a.dout.head_stride;
+  const float* const sp = a.rows + row_stat_at(a, kvh, 0, s.q0, 0);
+  const int qrs = (int)(a.q.row_stride * sizeof(T)), qhs = (int)(a.q.head_stride * sizeof(T)), ors = (int)(a.dout.row_stride * sizeof(T)),
+            ohs = (int)(a.dout.head_stride * sizeof(T));
+  const int group = 1 << a.gsh, q16 = group <= 16 ? (16 >> a.gsh) * qrs : 32 * qhs, o16 = group <= 16 ? (16 >> a.gsh) * ors : 16 * ohs;
+  const Stage<T, 32, 2, DB, NW> qst(a.d, qhs, wave, lane, [&](int x) { return (x >> a.gsh) * qrs + (x & (group - 1)) * 2 * qhs; });
+  const Stage<T, 32, 1, DVB, NW> ost(a.dv, 0, wave, lane, [&](int x) { return (x >> a.gsh) * ors + (x & (group - 1)) * ohs; });
+  // numbers of the rows: a wave load takes two of the six kinds, lane = kind and row
+  const int so = (int)((half * a.nq + (col >> a.gsh)) * a.g + (col & (group - 1))) * 4;
+  auto fill = [&](unsigned tile, int r0) GEOTR_INLINE {
+    const int i0 = r0 >> a.gsh, h0 = r0 & (group - 1);
+    const i32x4 rq = words(qp + i0 * a.q.row_stride + 2 * h0 * a.q.head_stride), ro = words(op + i0 * a.dout.row_stride + h0 * a.dout.head_stride);
+    auto there = [&](int x) GEOTR_INLINE { return r0 + x < rows && ((r0 + x) & (group - 1)) < a.g; };
+    if (r0 + 32 <= rows && a.g == group) {
+      qst.load_all(tile, rq, q16, wave);
+      ost.load_all(tile + 32 * CQ * 16, ro, o16, wave);
+    } else {
+      qst.load_some(tile, rq, q16, wave, there);
+      ost.load_some(tile + 32 * CQ * 16, ro, o16, wave, there);
+    }
+    // rows that do not exist: zeros, and their products are zero because q and dout are
+    for (int x = wave; x < 3; x += NW) {
+      const i32x4 rs = words(sp + ((int64_t)(2 * x) * a.nq + i0) * a.g + h0);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                   :
+                   : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) && 2 * x + half < 5 ? so : kOutside), "s"(rs)
+                   : "memory");
+    }
+  };
   const Rows<T, CQ> qrow(col, half);
   const Rows<T, CO> orow(col, half);
   const Cols<T, CQ> qcol(lane);
   const Cols<T, CO> ocol(lane);
-  for (int r0 = first; r0 < rows; r0 += 32) {
-    __syncthreads();
-    const int i0 = a.g == 1 ? r0 : r0 / a.g;
-    const auto rq = words(qp + (int64_t)i0 * a.q.row_stride);
-    const auto ro = words(op + (int64_t)i0 * a.dout.row_stride);
-    auto q_off = [&](int x, int64_t rs, int64_t hstr) GEOTR_INLINE {
-      const int r = r0 + x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
-      return r < rows ? (int)(((i - i0) * rs + h * hstr) * (int)sizeof(T)) : kOutside;
-    };
-    stage_at<T, 32, 2, DB, NW>(lds_at(smem), rq, a.d, (int)(a.q.head_stride * sizeof(T)), wave, lane,
-                        [&](int x) { return q_off(x, a.q.row_stride, 2 * a.q.head_stride); });
-    stage_at<T, 32, 1, DVB, NW>(lds_at(smem) + 32 * CQ * 16, ro, a.dv, 0, wave, lane,
-                         [&](int x) { return q_off(x, a.dout.row_stride, a.dout.head_stride); });
-    if (threadIdx.x < 32) {
-      const int r = r0 + threadIdx.x, i = a.g == 1 ? r : r / a.g, h = r - i * a.g;
-      const bool there = r < rows;
-      const int64_t p = stat_at(a, kvh, 0, s.q0 + i, h);
-      const float e1 = there ? a.lse[p] : INFINITY, e2 = there ? a.lse[p + a.nq * a.g] : INFINITY;
-      st[threadIdx.x] = e1, st[32 + threadIdx.x] = e2;
-      const bool big = __any((fabsf(e1) > kHuge && e1 < INFINITY) || (fabsf(e2) > kHuge && e2 < INFINITY));
-      if (threadIdx.x == 0) ((int*)st)[192] = big;
-      st[64 + threadIdx.x] = there ? a.del[p] : 0.f;
-      st[96 + threadIdx.x] = there ? a.del[p + a.nq * a.g] : 0.f;
-      st[128 + threadIdx.x] = there ? a.lam[kvh * a.g + h] : 0.f;
-      ((int*)st)[160 + threadIdx.x] = a.causal ? i + off : 0x7fffffff;
-    }
-    __syncthreads();
-    const unsigned qt = lds_at(smem), ot = qt + 32 * CQ * 16;
-    f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
+  auto consume = [&](unsigned qt, int r0) GEOTR_INLINE {
+    const unsigned ot = qt + 32 * CQ * 16, st = qt + kRowBytes + 16 * half;
+    auto stat = [&](int which, int j) GEOTR_INLINE { return lds_load<f32x4>(st + 128 * which + 32 * j); };
+    f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();  // scores, then P1 and |lam| P2
 #pragma unroll
     for (int i = 0; i < QS; ++i) {
       Ops<T>::mma(s1, qrow.get(qt, 0, i), kHold ? k1[i % (kHold ? QS : 1)] : k_frag(0, i));
       Ops<T>::mma(s2, qrow.get(qt, 0, CQ / 4 + i), kHold ? k2[i % (kHold ? QS : 1)] : k_frag(1, i));
     }
+    if constexpr (PART == kKeysOnly) GEOTR_FENCE;
+    auto weights = [&](auto from) GEOTR_INLINE {  // beside the products of dP
+      if constexpr (DK) {
 #pragma unroll
-    for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, orow.get(ot, 0, i), kHold ? vv[i % (kHold ? VS : 1)] : v_frag(i));
-    const bool huge = __builtin_amdgcn_readfirstlane(((const int*)st)[192]) != 0;
-    f32x16 pj;
-    auto stat = [&](int which, int i) GEOTR_INLINE { return st[32 * which + 8 * (i / 4) + 4 * half + i % 4]; };
-    exponents(s1, a.scale_log2, [&](int i) { return stat(0, i); }, huge);
-    exponents(s2, a.scale_log2, [&](int i) { return stat(1, i); }, huge);
-    if (a.causal && r0 < (key_base + TILE - 1 - off) * a.g) {  // a tile that some key of the block is not seen by
+        for (int i = 0; i < VS; ++i) {
+          if (PART == kKeysOnly && i % 2 == 0) GEOTR_FENCE;
+          Ops<T>::mma(dp, orow.get(ot, 0, i), kHoldV ? vv[i % (kHoldV ? VS : 1)] : kLdsV ? orow.get(vt, 0, i) : v_frag(i));
+        }
+        if constexpr (PART == kKeysOnly) GEOTR_FENCE;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 e1 = stat(0, j), e2 = stat(1, j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * j + e;
+          s1[i] = __builtin_amdgcn_exp2f(from(s1[i], e1[e])), s2[i] = __builtin_amdgcn_exp2f(from(s2[i], e2[e]));
+        }
+          }
+    };
+    const float own = fabsf(lds_load<float>(qt + kRowBytes + 128 * half + 4 * col));  // lane: row and map
+    if (__builtin_expect(__any(own > kHuge && own < INFINITY), 0)) weights([&](float x, float e) { return x * a.scale_log2 - e; });
+    else weights([&](float x, float e) { return fmaf(x, a.scale_log2, -e); });
+    if (a.causal && r0 < last) {  // rows that do not see some key of the block
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (key > __float_as_int(stat(5, i))) s1[i] = 0.f, s2[i] = 0.f;
+        if (r0 + 8 * (i / 4) + 4 * half + i % 4 < from) s1[i] = 0.f, s2[i] = 0.f;
+    }
+    if (minus) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 sg = stat(4, j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s2[4 * j + e] *= sg[e];
+      }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int x = 8 * j + 4 * half;
-      const f32x4 d1 = *(const f32x4*)(st + 64 + x), d2 = *(const f32x4*)(st + 96 + x), lm = *(const f32x4*)(st + 128 + x);
+      f32x4 d1 = {}, d2 = {};
+      if constexpr (DK) d1 = stat(2, j), d2 = stat(3, j);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * j + e;
-        const float p1 = s1[i], p2 = s2[i];
-        pj[i] = fmaf(-lm[e], p2, p1) * kBoost;
-        s1[i] = p1 * (dp[i] - d1[e]), s2[i] = -lm[e] * p2 * (dp[i] - d2[e]);
-        if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs;
+        const float p1 = s1[i], p2 = s2[i], g = dp[i];
+        if constexpr (DK) s1[i] = p1 * (g - d1[e]), s2[i] = p2 * (d2[e] - g);
+        if constexpr (DV) dp[i] = p1 - p2;
+        if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs, dp[i] *= kBoost;
       }
     }
 #pragma unroll
     for (int p = 0; p < kPSteps<T>; ++p) {
-      const Frag fp = pack<T>(pj, p), f1 = pack<T>(s1, p), f2 = pack<T>(s2, p);
+      if constexpr (DV) {
+        const Frag f = pack<T>(dp, p);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) Ops<T>::mma(av[i], ocol.get(ot, 0, p, i), fp);
-#pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        Ops<T>::mma(ak1[i], qcol.get(qt, 0, p, i), f1);
-        Ops<T>::mma(ak2[i], qcol.get(qt, 0, p, ND + i), f2);
+        for (int i = 0; i < NV; ++i) Ops<T>::mma(av[i], ocol.get(ot, 0, p, i), f);
       }
+      if constexpr (DK) {
+        const Frag f1 = pack<T>(s1, p), f2 = pack<T>(s2, p);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          Ops<T>::mma(ak1[i], qcol.get(qt, 0, p, i), f1);
+          Ops<T>::mma(ak2[i], qcol.get(qt, 0, p, ND + i), f2);
+        }
+      }
+    }
+  };
+  const unsigned base = lds_at(smem);
+  if constexpr (NB == 2) {
+    if (first < rows) fill(base, first);
+    int which = 0;
+    for (int r0 = first; r0 < rows; r0 += 32) {
+      tile_ready();
+      __syncthreads();
+      if (r0 + 32 < rows) fill(base + (kTile - which), r0 + 32);
+      consume(base + which, r0);
+      which = kTile - which;
+    }
+  } else {
+    for (int r0 = first; r0 < rows; r0 += 32) {
+      __syncthreads();
+      fill(base, r0);
+      tile_ready();
+      __syncthreads();
+      consume(base, r0);
     }
   }
   if (key >= keys_here) return;
@@ -1228,15 +1341,19 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * DB <= 64 ? 2 : 1) void dkv_ker
   };
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
+    if constexpr (DK) {
 #pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      const int c = 32 * i + 8 * j + 4 * half;
-      if (c < a.d) out4(pk + c, ak1[i], j, fk), out4(pk + a.d + c, ak2[i], j, fk);
+      for (int i = 0; i < ND; ++i) {
+        const int c = 32 * i + 8 * j + 4 * half;
+        if (c < a.d) out4(pk + c, ak1[i], j, fk), out4(pk + a.d + c, ak2[i], j, fk);
+      }
     }
+    if constexpr (DV) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = 32 * i + 8 * j + 4 * half;
-      if (c < a.dv) out4(pv + c, av[i], j, fv);
+      for (int i = 0; i < NV; ++i) {
+        const int c = 32 * i + 8 * j + 4 * half;
+        if (c < a.dv) out4(pv + c, av[i], j, fv);
+      }
     }
   }
 }
@@ -1246,23 +1363,33 @@ enum Which { kForward, kForwardKeys, kBackwardQ, kBackwardKV };
 
 // stack mode: every sequence may end inside a tile, and one block more takes the rows behind the last
 inline int64_t tiles_of(const Args& a, bool keys, int tile) {
-  const int64_t rows = keys ? (a.stacked ? a.nk : a.m) : (a.stacked ? a.nq : a.n) * (int64_t)a.g;
+  const int64_t rows = keys ? (a.stacked ? a.nk : a.m) : (a.stacked ? a.nq : a.n) << a.gsh;
   return (rows + tile - 1) / tile + (a.stacked ? a.batch + 1 : 0);
 }
 
 template <typename T, int DB, int DVB>
 int launch_dims(const Args& a, Which which, hipStream_t s) {
-  constexpr int NWK = 32 * (2 * DB + DVB) * (int)sizeof(T) * 4 <= 131072 ? 4 : 2;  // KEYS: a tile for every wave
-  const bool fwd = which == kForward || which == kForwardKeys;
-  constexpr int G = kGroups<T, DB, DVB>;
-  const int64_t tiles = tiles_of(a, which == kBackwardKV, which == kForwardKeys ? 32 : which == kForward ? 32 * G : 128), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
+  constexpr int G = 2, NWB = 4, kWide = 64 * (2 * DB + DVB) * (int)sizeof(T);  // bytes of 64 keys
+  // few rows: narrow heads stream a tile per wave; wide ones share tiles of 64 keys, where two buffers of them fit
+  constexpr bool kNarrow = (int)sizeof(T) * DB < 256, kFew = !kNarrow && 2 * kWide <= 160 * 1024;
+  const bool keys = which == kForwardKeys && (kNarrow || kFew);
+  const int tile = which == kBackwardQ || which == kBackwardKV ? 32 * NWB : keys ? 32 : 32 * G;
+  const int64_t tiles = tiles_of(a, which == kBackwardKV, tile), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
   if (tiles == 0 || x == 0) return GEOTR_OK;
   if (tiles > 65535 || x > 0x7fffffff) return fail(GEOTR_E_INVALID, "differential attention: %lld tiles of rows in one call", (long long)tiles);
-  const dim3 grid((unsigned)x, (unsigned)tiles, fwd ? (unsigned)a.splits : 1u);
-  if (which == kForward) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, G>), grid, dim3(128 * G), 0, s, a);
-  else if (which == kForwardKeys) hipLaunchKernelGGL((fwd_keys_kernel<T, DB, DVB, NWK>), grid, dim3(64 * NWK), 0, s, a);
-  else if (which == kBackwardQ) hipLaunchKernelGGL((dq_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
+  const dim3 grid((unsigned)x, (unsigned)tiles, which == kForward || which == kForwardKeys ? (unsigned)a.splits : 1u);
+  if (which == kForward || which == kForwardKeys) {
+    if (!keys) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, G, false>), grid, dim3(128 * G), 0, s, a);
+    else if constexpr (kNarrow) hipLaunchKernelGGL((fwd_keys_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
+    else if constexpr (kFew) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, G, true>), grid, dim3(128 * G), 0, s, a);
+  } else if (which == kBackwardQ) {
+    hipLaunchKernelGGL((dq_kernel<T, DB, DVB, NWB>), grid, dim3(64 * NWB), 0, s, a);
+  } else if constexpr (kSplitKV<T, DVB>) {
+    hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, NWB, kKeysOnly>), grid, dim3(64 * NWB), 0, s, a);
+    hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, NWB, kValuesOnly>), grid, dim3(64 * NWB), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, NWB, kBoth>), grid, dim3(64 * NWB), 0, s, a);
+  }
   GEOTR_CHECK_LAUNCH("differential attention");
   return GEOTR_OK;
 }

@@ -10,14 +10,15 @@ namespace {
 
 constexpr int kMostSplits = 64;  // the join holds one split per lane
 
-// One wave per (row, head): maxima and sums of the splits in the lanes, channels over the lanes.  Bound: HBM / latency.
+// One block per (row, head): every wave holds the splits' maxima and sums in its lanes, four channels of both maps in a lane, and takes
+// every fourth split; the waves meet in LDS in a fixed order.  Bound: HBM where rows are many, latency for single tokens (a wave per row that
+// walked the splits took 82 us for 16 rows of 64 splits).
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
-  const int lane = threadIdx.x & 63, heads = a.hk * a.g;
-  const int64_t e = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (e >= a.nq * heads) return;
-  const int64_t row = e / heads;
-  const int head = (int)(e - row * heads), w = a.dv + 4;
+  __shared__ f32x4 box[4][2][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, heads = a.hk * a.g;
+  const int64_t e = blockIdx.x, row = e / heads;
+  const int head = (int)(e - row * heads), w = a.dv + 4, c = 4 * lane;
   const int64_t step = a.nq * heads * 2 * (int64_t)w;
   const float* p = a.part + e * 2 * w;
   float m[2], l[2], f[2];
@@ -34,20 +35,34 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
     m[x] = top, l[x] = sum;
   }
+  f32x4 y = {}, z = {};
+#pragma unroll 4
+  for (int s = wave; s < a.splits; s += 4) {
+    const float f1 = __shfl(f[0], s, 64), f2 = __shfl(f[1], s, 64);
+    if (c < a.dv) {
+      const f32x4 u = *(const f32x4*)(p + s * step + 4 + c), v = *(const f32x4*)(p + s * step + w + 4 + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a split without keys may have written nothing
+        if (f1 != 0.f) y[i] = fmaf(u[i], f1, y[i]);
+        if (f2 != 0.f) z[i] = fmaf(v[i], f2, z[i]);
+      }
+    }
+  }
+  box[wave][0][lane] = y, box[wave][1][lane] = z;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int x = 1; x < 4; ++x) y += box[x][0][lane], z += box[x][1][lane];
   const bool some = l[0] != 0.f;
   const float lam = a.lam[head];
-  for (int c = lane; c < a.dv; c += 64) {
-    float y = 0.f, z = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float f1 = __shfl(f[0], s, 64), f2 = __shfl(f[1], s, 64);
-      const float* q = p + s * step + 4 + c;
-      if (f1 != 0.f) y = fmaf(q[0], f1, y);
-      if (f2 != 0.f) z = fmaf(q[w], f2, z);
+  if (c < a.dv) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      z[i] = some ? z[i] / l[1] : 0.f;
+      y[i] = some ? fmaf(-lam, z[i], y[i] / l[0]) : 0.f;
     }
-    z = some ? z / l[1] : 0.f;
-    y = some ? fmaf(-lam, z, y / l[0]) : 0.f;
-    ((T*)a.out)[e * a.dv + c] = (T)y;
-    if (a.o2) ((T*)a.o2)[e * a.dv + c] = (T)z;
+    store4<T>((T*)a.out + e * a.dv + c, y[0], y[1], y[2], y[3]);
+    if (a.o2) store4<T>((T*)a.o2 + e * a.dv + c, z[0], z[1], z[2], z[3]);
   }
   if (a.lse && lane < 2) {
     const int kvh = head / a.g;
@@ -55,7 +70,8 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   }
 }
 
-// del_2 = dout . O2, del_1 = dout . O1 = dout . out + lam del_2; 16 lanes per (row, head).  fp16: the largest |dout| of the rows that
+// What the backward pass reads of a row: the sums, del_2 = dout . O2 and del_1 = dout . O1 = dout . out + lam del_2 (16 lanes per (row,
+// head)), |lam| folded into the second sum.  fp16: the largest |dout| of the rows that
 // exist (an order-free maximum).  Bound: HBM.
 template <typename T>
 __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
@@ -85,7 +101,10 @@ __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
   if (in && c0 == 0) {
     const int kvh = head / a.g;
     const int64_t at = stat_at(a, kvh, 0, row, head - kvh * a.g);
-    a.del[at] = fmaf(a.lam[head], z, x), a.del[at + a.nq * a.g] = z;
+    const int64_t to = row_stat_at(a, kvh, 0, row, head - kvh * a.g), step = a.nq * a.g;
+    const float lam = a.lam[head], e2 = a.lse[at + step];
+    a.rows[to] = a.lse[at], a.rows[to + step] = lam == 0.f ? INFINITY : e2 - log2f(fabsf(lam));
+    a.rows[to + 2 * step] = fmaf(lam, z, x), a.rows[to + 3 * step] = z, a.rows[to + 4 * step] = lam < 0.f ? -1.f : 1.f;
   }
   if constexpr (Narrow<T>::value) {
     if (a.q_len) {  // gradients of rows that do not exist say nothing
@@ -153,15 +172,17 @@ int make_args(const geotr_diff_attn* op, Args& a) {
   GEOTR_CHECK_ARG(!op->stacked || (op->q_lengths && op->k_lengths), "differential attention: stack mode needs both lengths");
   const int size = op->dtype == GEOTR_F32 ? 4 : 2;
   const int64_t g = h / hk;
+  a.gsh = 0;
+  while ((1 << a.gsh) < g) ++a.gsh;
   a.nq = op->stacked ? op->n : op->batch * op->n, a.nk = op->stacked ? op->m : op->batch * op->m;
-  GEOTR_CHECK_ARG(a.nq * g <= kMostRows && a.nk <= kMostRows, "differential attention: %lld query rows (x %lld heads) and %lld keys in one call",
+  GEOTR_CHECK_ARG((a.nq << a.gsh) <= kMostRows && a.nk <= kMostRows, "differential attention: %lld query rows (x %lld heads) and %lld keys in one call",
                   (long long)a.nq, (long long)g, (long long)a.nk);
   int rc;
   if ((rc = check_view(op->q, 2 * h, size, op->batch, op->n, "q")) || (rc = check_view(op->k, 2 * hk, size, op->batch, op->m, "k")) ||
       (rc = check_view(op->v, hk, size, op->batch, op->m, "v")))
     return rc;
   a.q = op->q, a.k = op->k, a.v = op->v, a.dout = geotr_heads{nullptr, 0, 0, 0, 0};
-  a.out = a.o2 = a.gq = a.gk = a.gv = nullptr, a.lse = a.del = a.part = a.drow = nullptr, a.amax = nullptr;
+  a.out = a.o2 = a.gq = a.gk = a.gv = nullptr, a.lse = a.part = a.drow = a.rows = nullptr, a.amax = nullptr;
   a.lam = op->lam, a.q_len = op->q_lengths, a.k_len = op->k_lengths, a.masks = op->key_masks;
   a.batch = (int)op->batch, a.stacked = op->stacked != 0, a.n = (int)op->n, a.m = (int)op->m;
   a.hk = (int)hk, a.g = (int)g, a.d = (int)op->dim, a.dv = (int)op->v_dim, a.causal = op->causal != 0, a.splits = 1;
@@ -173,11 +194,11 @@ int make_args(const geotr_diff_attn* op, Args& a) {
 // blocks until there are two for each compute unit, as long as every block keeps 256 keys.
 bool keys_form(const Args& a) {
   const int64_t rows = a.stacked ? (a.nq + a.batch - 1) / std::max(a.batch, 1) : a.n;
-  return rows * a.g <= 32;
+  return rows << a.gsh <= 32;
 }
 int choose_splits(const Args& a) {
   const int64_t per = a.stacked ? a.nk / std::max(a.batch, 1) : a.m, seqs = std::max(a.batch, 1);
-  const int64_t rows = (a.stacked ? (a.nq + seqs - 1) / seqs : a.n) * a.g, tile = keys_form(a) ? 32 : 128;
+  const int64_t rows = (a.stacked ? (a.nq + seqs - 1) / seqs : a.n) << a.gsh, tile = keys_form(a) ? 32 : 64;
   const int64_t blocks = seqs * a.hk * std::max<int64_t>(1, (rows + tile - 1) / tile);
   return (int)std::max<int64_t>(1, std::min<int64_t>({kMostSplits, 512 / blocks, per / 256}));
 }
@@ -217,7 +238,7 @@ int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, void* out2, fl
   hipStream_t s = (hipStream_t)stream;
   if (const int r = launch(op->dtype, a, keys_form(a) ? kForwardKeys : kForward, s)) return r;
   if (a.splits > 1) {
-    const dim3 grid((unsigned)((a.nq * a.hk * a.g + 3) / 4));
+    const dim3 grid((unsigned)(a.nq * a.hk * a.g));
     if (op->dtype == GEOTR_F32) hipLaunchKernelGGL((join_kernel<float>), grid, dim3(256), 0, s, a);
     else if (op->dtype == GEOTR_BF16) hipLaunchKernelGGL((join_kernel<__bf16>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((join_kernel<_Float16>), grid, dim3(256), 0, s, a);
@@ -230,7 +251,7 @@ size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op) {
   Args a;
   if (make_args(op, a) != GEOTR_OK) return 0;
   const size_t rows = (size_t)a.nq * a.hk * a.g;
-  return align_up(2 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(sizeof(float));
+  return align_up(5 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(sizeof(float));
 }
 
 int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const void* out, const void* out2, const float* lse,
@@ -247,7 +268,7 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
   const size_t rows = (size_t)a.nq * a.hk * a.g, need = geotr_diff_attn_backward_workspace_bytes(op);
   if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   Carver c(ws);
-  a.del = c.take<float>(2 * rows), a.drow = c.take<float>(rows);
+  a.rows = c.take<float>(5 * rows), a.drow = c.take<float>(rows);
   float* amax = c.take<float>(1);
   a.dout = *dout, a.out = const_cast<void*>(out), a.o2 = const_cast<void*>(out2), a.lse = const_cast<float*>(lse);
   a.gq = dq, a.gk = dk, a.gv = dv, a.amax = amax;
