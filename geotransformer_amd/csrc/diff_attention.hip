@@ -52,7 +52,11 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   __syncthreads();
   if (wave) return;
 #pragma unroll
-  for (int x = 1; x < 4; ++x) y += box[x][0][lane], z += box[x][1][lane];
+  for (int x = 1; x < 4; ++x) {
+    const f32x4 u = box[x][0][lane], v = box[x][1][lane];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] += u[i], z[i] += v[i];
+  }
   const bool some = l[0] != 0.f;
   const float lam = a.lam[head];
   if (c < a.dv) {

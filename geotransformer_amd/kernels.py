@@ -5,6 +5,7 @@ import ctypes
 import math
 
 import os
+import struct
 
 import torch
 
@@ -782,24 +783,41 @@ HEAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 
 
+_HEADS, _DIFF_ATTN = struct.Struct('5q'), struct.Struct('15q4i9qfi')  # the bytes of Heads and DiffAttn (a fifth of a ctypes structure's time)
+
+
 def _heads(t):
-    """geotr_heads of a (rows, heads, channels) or (batch, rows, heads, channels) tensor whose channels are contiguous; the stride of a
-    dimension of one element says nothing and is passed as 0."""
+    """The five words of geotr_heads of a (rows, heads, channels) or (batch, rows, heads, channels) tensor whose channels are contiguous; the
+    stride of a dimension of one element says nothing and is passed as 0."""
     if t is None:
-        return Heads(None, 0, 0, 0, 0)
-    size, stride = t.shape[-3:], [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
-    return Heads(t.data_ptr(), size[1], stride[0] if t.dim() == 4 else 0, stride[-3], stride[-2])
+        return 0, 0, 0, 0, 0
+    size, stride = t.shape, t.stride()
+    if len(size) == 4:
+        return (t.data_ptr(), size[2], stride[0] if size[0] > 1 else 0, stride[1] if size[1] > 1 else 0, stride[2] if size[2] > 1 else 0)
+    return t.data_ptr(), size[1], 0, stride[0] if size[0] > 1 else 0, stride[1] if size[1] > 1 else 0
 
 
 def _same_device(*tensors):
     """The one device of all given tensors; RuntimeError when it is not a GPU."""
-    device = next(t for t in tensors if t is not None).device
+    device = tensors[0].device
     for t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f'all tensors of a call live on one device: {t.device} and {device}')
     if device.type != 'cuda':
         raise RuntimeError('geotransformer_amd needs device tensors (MI355X / gfx950); no CPU fallback exists.')
     return device
+
+
+def _call(device, fn, name, *args):
+    """fn(*args, stream) on the current stream of `device`, which need not be the current device."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream without the object (3 us of a call's 23)
+    if device.index == torch.cuda.current_device():
+        code = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, stream)
+    if code:
+        _lib.check(code, name)
 
 
 def check_rotary_heads(q, k):
@@ -830,14 +848,12 @@ def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0
     k = k if k is None or k.stride(-1) == 1 else k.contiguous()
     q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
     k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
-    views = [_heads(t) for t in (q, q_out, k, k_out)]
+    pack = _HEADS.pack
     batch, rows = (1, lead[0]) if len(lead) == 1 else lead
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().geotr_rotary(ctypes.byref(views[0]), ctypes.byref(views[1]), None if k is None else ctypes.byref(views[2]),
-                                            None if k is None else ctypes.byref(views[3]), HEAD_TYPES[q.dtype], batch, rows, q.shape[-1],
-                                            int(rotary_dim), int(bool(interleaved)), _lib.ptr(pos), POSITION_TYPES[pos.dtype],
-                                            pos.stride(0) if len(lead) == 2 else 0, pos.stride(-2), pos.stride(-1), _lib.ptr(turns),
-                                            _lib.ptr(axis), float(gain), int(bool(inverse)), _lib.stream_ptr()), 'geotr_rotary')
+    _call(device, _lib.load().geotr_rotary, 'geotr_rotary', pack(*_heads(q)), pack(*_heads(q_out)), None if k is None else pack(*_heads(k)),
+          None if k is None else pack(*_heads(k_out)), HEAD_TYPES[q.dtype], batch, rows, q.shape[-1], rotary_dim, int(interleaved), pos.data_ptr(),
+          POSITION_TYPES[pos.dtype], pos.stride(0) if len(lead) == 2 else 0, pos.stride(-2), pos.stride(-1), turns.data_ptr(), axis.data_ptr(), gain,
+          int(inverse))
     return q_out, k_out
 
 
@@ -887,21 +903,22 @@ def _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale):
     """(descriptor, what it points into) of a call."""
     device = _same_device(q, k, v, lam, q_lengths, k_lengths, key_masks)
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    lam = lam.expand(q.shape[-2] // 2).contiguous()
-    q_lengths, k_lengths, key_masks = (None if t is None else t.contiguous() for t in (q_lengths, k_lengths, key_masks))
+    if lam.dim() == 0 or lam.shape[0] * 2 != q.shape[-2] or lam.stride(0) != 1:
+        lam = lam.expand(q.shape[-2] // 2).contiguous()
+    q_lengths, k_lengths, key_masks = (t if t is None else t.contiguous() for t in (q_lengths, k_lengths, key_masks))
     stacked = q.dim() == 3 and q_lengths is not None
     batch = q_lengths.shape[0] if stacked else 1 if q.dim() == 3 else q.shape[0]
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
-    op = DiffAttn(_heads(q), _heads(k), _heads(v), HEAD_TYPES[q.dtype], int(stacked), int(bool(causal)), 0, batch, q.shape[-3], k.shape[-3],
-                  q.shape[-1], v.shape[-1], lam.data_ptr(), *(None if t is None else t.data_ptr() for t in (q_lengths, k_lengths, key_masks)),
-                  scale, 0)
+    op = _DIFF_ATTN.pack(*_heads(q), *_heads(k), *_heads(v), HEAD_TYPES[q.dtype], stacked, bool(causal), 0, batch, q.shape[-3], k.shape[-3], q.shape[-1],
+                         v.shape[-1], lam.data_ptr(), *(0 if t is None else t.data_ptr() for t in (q_lengths, k_lengths, key_masks)), scale, 0)
     return op, (q, k, v, lam, q_lengths, k_lengths, key_masks), device
 
 
-def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None, want_state=False):
+def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None, want_state=False, checked=False):
     """out[i, h] = sum_j (softmax_j(scale q[i, 2h] . k[j, 2c]) - lam[h] softmax_j(scale q[i, 2h+1] . k[j, 2c+1])) v[j, c], c = h Hk / H
     (geotr_diff_attn_forward).  want_state: also what diff_attention_backward needs, (out, (out2, lse))."""
-    check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
+    if not checked:
+        check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
     lib, heads, kv_heads = _lib.load(), q.shape[-2] // 2, v.shape[-2]
     out = torch.empty(q.shape[:-2] + (heads, v.shape[-1]), dtype=q.dtype, device=device)
@@ -909,10 +926,10 @@ def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None,
     if want_state:
         out2 = torch.empty_like(out)
         lse = torch.empty((kv_heads, 2) + q.shape[:-2] + (heads // kv_heads,), dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        ws = _lib.workspace(lib.geotr_diff_attn_workspace_bytes(ctypes.byref(op)), device)
-        _lib.check(lib.geotr_diff_attn_forward(ctypes.byref(op), _lib.ptr(out), _lib.ptr(out2), _lib.ptr(lse), _lib.ptr(ws), ws.numel(),
-                                               _lib.stream_ptr()), 'geotr_diff_attn_forward')
+    need = lib.geotr_diff_attn_workspace_bytes(op)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call(device, lib.geotr_diff_attn_forward, 'geotr_diff_attn_forward', op, out.data_ptr(), out2 if out2 is None else out2.data_ptr(),
+          lse if lse is None else lse.data_ptr(), ws if ws is None else ws.data_ptr(), need)
     del keep
     return (out, (out2, lse)) if want_state else out
 
@@ -920,15 +937,16 @@ def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None,
 def diff_attention_backward(dout, q, k, v, lam, out, state, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None):
     """(dq, dk, dv, dlam (H)) for dout from diff_attention(..., want_state=True)'s results (geotr_diff_attn_backward)."""
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
+    if dout.shape != out.shape or dout.dtype != q.dtype:
+        raise ValueError(f'dout is {q.dtype} of the output\'s shape {tuple(out.shape)}: got {dout.dtype} {tuple(dout.shape)}')
+    _same_device(q, dout, out, *state)
     lib = _lib.load()
     dout = _aligned(dout)
-    view = _heads(dout)
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
     dlam = torch.empty(q.shape[-2] // 2, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        ws = _lib.workspace(lib.geotr_diff_attn_backward_workspace_bytes(ctypes.byref(op)), device)
-        _lib.check(lib.geotr_diff_attn_backward(ctypes.byref(op), ctypes.byref(view), _lib.ptr(out), _lib.ptr(state[0]), _lib.ptr(state[1]),
-                                                _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(dlam), _lib.ptr(ws), ws.numel(),
-                                                _lib.stream_ptr()), 'geotr_diff_attn_backward')
+    need = lib.geotr_diff_attn_backward_workspace_bytes(op)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _call(device, lib.geotr_diff_attn_backward, 'geotr_diff_attn_backward', op, _HEADS.pack(*_heads(dout)), out.data_ptr(), state[0].data_ptr(),
+          state[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), need)
     del keep
     return dq, dk, dv, dlam

@@ -19,7 +19,7 @@ from .rotary_embedding import RotaryPositionalEmbedding
 class _DifferentialAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale):
-        out, state = kernels.diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale, want_state=True)
+        out, state = kernels.diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale, want_state=True, checked=True)
         ctx.save_for_backward(q, k, v, lam, out, *state, q_lengths, k_lengths, key_masks)
         ctx.causal, ctx.scale = causal, scale
         return out
@@ -48,7 +48,7 @@ def differential_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_mas
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
         lam = lam.expand(q.shape[-2] // 2)  # the gradient of a shared value is the sum over its heads
         return _DifferentialAttention.apply(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
-    return kernels.diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
+    return kernels.diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale, checked=True)
 
 
 class DifferentialMultiHeadAttention(nn.Module):

@@ -54,7 +54,10 @@ class _Rotary(torch.autograd.Function):
         if dq is None and dk is None:
             return (None,) * 7
         first, second = (dk, None) if dq is None else (dq, dk)
-        first, second = _Rotary.apply(first, second, positions, turns, axis, ctx.how, not ctx.inverse)
+        if torch.is_grad_enabled():  # a graph of the gradient is wanted
+            first, second = _Rotary.apply(first, second, positions, turns, axis, ctx.how, not ctx.inverse)
+        else:
+            first, second = kernels.rotary(first, second, positions, turns, axis, *ctx.how, inverse=not ctx.inverse)
         return (None, first, None, None, None, None, None) if dq is None else (first, second, None, None, None, None, None)
 
 
@@ -92,5 +95,7 @@ class RotaryPositionalEmbedding(nn.Module):
             raise ValueError(f'positions {tuple(positions.shape)} of rows {tuple(lead)}, built for {self.num_axes} axes')
         if positions.requires_grad:
             raise NotImplementedError('rotary positions are not differentiable in the positions: pass positions.detach()')
-        return _Rotary.apply(q, k, positions, self.turn_bits.view(torch.float64), self.axis, (self.rotary_dim, self.interleaved, self.gain),
-                             False)
+        how, turns = (self.rotary_dim, self.interleaved, self.gain), self.turn_bits.view(torch.float64)
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            return _Rotary.apply(q, k, positions, turns, self.axis, how, False)
+        return kernels.rotary(q, k, positions, turns, self.axis, *how)
