@@ -134,7 +134,7 @@ SIGNATURES = {
     'geotr_diff_attn_workspace_bytes': (c_size, [c_ptr]),  # struct pointers; typed in geotransformer_amd/kernels.py
     'geotr_diff_attn_forward': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
     'geotr_diff_attn_backward_workspace_bytes': (c_size, [c_ptr]),
-    'geotr_diff_attn_backward': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
+    'geotr_diff_attn_backward': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
     'geotr_lgr': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_f32, c_int, c_f32, c_i64,
                           c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
 }

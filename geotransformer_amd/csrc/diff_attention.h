@@ -36,7 +36,8 @@ using s16x4 = __attribute__((ext_vector_type(4))) short;
 
 struct Args {
   geotr_heads q, k, v, dout;             // dout: backward only
-  void *out, *o2, *gq, *gk, *gv;         // contiguous (rows, heads, channels)
+  void *out, *gq, *gk, *gv;              // contiguous (rows, heads, channels)
+  float* maps;                           // (rows, heads, 2, dv): the maps' outputs, for the backward pass
   float *lse, *part, *drow;              // (hk, 2, nq, g), split partials, (hk, nq, g)
   float* rows;                           // backward, (hk, 5, nq, g): lse1, lse2 - log2 |lam|, del1, del2, sign of lam
   const float* amax;                     // 16-bit floats of narrow range: largest |dout| (backward), else null
@@ -78,6 +79,15 @@ constexpr int kStep = 2 * kE<T>;           // channels (row reads) or contractio
 template <typename T>
 constexpr int kPSteps = 32 / kStep<T>;     // steps of a 32-deep product
 
+// the type whose exponents are narrow
+template <typename T>
+struct Narrow {
+  static constexpr bool value = false;
+};
+template <>
+struct Narrow<_Float16> {
+  static constexpr bool value = true;
+};
 // waves that a SIMD unit holds at a time, by the registers of the accumulators
 template <typename T, int DB, int DVB>
 constexpr int kWaves = sizeof(T) * DB <= 128 ? 2 : 1;
@@ -90,6 +100,24 @@ __device__ __forceinline__ typename Ops<T>::Frag pack(const f32x16& p, int t) {
   typename Ops<T>::Frag f;
 #pragma unroll
   for (int i = 0; i < kE<T>; ++i) f[i] = (T)p[kE<T> * t + i];
+  return f;
+}
+
+// what pack(p, t) = w rounded away: p - w in one instruction as a product of a pair with (-1, 0) or (0, -1), where expanding w would take one
+// more.  The pairs are kept from the compiler: bfloat16's (-1, 0) as an immediate is read as (0, -1).
+template <typename T>
+__device__ __forceinline__ typename Ops<T>::Frag pack_rest(const f32x16& p, int t, const typename Ops<T>::Frag& w) {
+  using Pair = __attribute__((ext_vector_type(2))) T;
+  unsigned one = Narrow<T>::value ? 0xbc00u : 0xbf80u, other = one << 16;
+  asm("" : "+s"(one), "+s"(other));
+  const Pair minus[2] = {__builtin_bit_cast(Pair, one), __builtin_bit_cast(Pair, other)};
+  typename Ops<T>::Frag f;
+#pragma unroll
+  for (int i = 0; i < kE<T>; ++i) {
+    const Pair x = {w[i & ~1], w[i | 1]};
+    if constexpr (Narrow<T>::value) f[i] = (T)__builtin_amdgcn_fdot2(x, minus[i & 1], p[kE<T> * t + i], false);
+    else f[i] = (T)__builtin_amdgcn_fdot2_f32_bf16(x, minus[i & 1], p[kE<T> * t + i], false);
+  }
   return f;
 }
 
@@ -387,11 +415,11 @@ __device__ __forceinline__ void store4(T* p, float x, float y, float z, float w)
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------
-// Order of the tiles of one sequence: causal rows cost what lies before them.  With two blocks to a compute unit at most, all run at once
-// and the second half goes up from the shortest (a long block shares its unit with a short one); else the longest go first.
-__device__ __forceinline__ int tile_order(const Args& a, int y, int tiles, int others) {
+// Order of the tiles of one sequence: causal rows cost what lies before them.  Where all blocks run at once (two to a compute
+// unit) the second half goes up from the shortest (a long block shares its unit with a short one); else the longest go first.
+__device__ __forceinline__ int tile_order(const Args& a, int y, int tiles, int others, int at_once = 512) {
   if (!a.causal) return y;
-  if ((int64_t)tiles * others > 512) return tiles - 1 - y;
+  if ((int64_t)tiles * others > at_once) return tiles - 1 - y;
   return y < (tiles + 1) / 2 ? tiles - 1 - y : y - (tiles + 1) / 2;
 }
 // keys of this block when they are dealt over blockIdx.z
@@ -416,7 +444,10 @@ __device__ __forceinline__ void zero_rows(const Args& a, const Seq& s, int kvh, 
   for (int64_t e = first; e < rows * per; e += step) {
     const int64_t i = e / per, o = ((s.q_end + i) * a.hk + kvh) * per + (e - i * per);
     ((T*)a.out)[o] = (T)0.f;
-    if (a.o2) ((T*)a.o2)[o] = (T)0.f;
+  }
+  for (int64_t e = first; a.maps && e < 2 * rows * per; e += step) {
+    const int64_t i = e / (2 * per);
+    a.maps[((s.q_end + i) * a.hk + kvh) * 2 * per + (e - i * 2 * per)] = 0.f;
   }
   for (int64_t e = first; a.lse && e < rows * a.g; e += step) {
     const int64_t at = stat_at(a, kvh, 0, s.q_end, 0) + e;
@@ -429,7 +460,9 @@ __device__ __forceinline__ void zero_rows(const Args& a, const Seq& s, int kvh, 
 // buffers: the next one loads while this one is consumed.
 // The accumulators are rescaled only when a row's maximum grew by more than 2^8: weights stay below 2^8, sums are exact either way.
 // FEW (a token over a cache, wide heads): the G groups share 32 rows and take 32 keys each of every tile, joined at the end.
-template <typename T, int DB, int DVB, int G, bool FEW>
+// EXACT (16-bit, for training): what rounding P to 16 bits takes away goes through a second product, because the gradients subtract
+// dout . O_map from dout . v: an error of O is one of every dS of the row, and was as large as all others of dQ and dK together.
+template <typename T, int DB, int DVB, int G, bool FEW, bool EXACT>
 __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, NT = DVB / 32, QS = DB / kStep<T>, TILE = FEW ? 32 : 32 * G;
@@ -553,8 +586,18 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
 #pragma unroll
     for (int x = 0; x < kPSteps<T>; ++x) {
       const Frag w = pack<T>(p, x);
+      if constexpr (EXACT) {
+        const Frag rest = pack_rest<T>(p, x, w);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) Ops<T>::mma(acc[i], vcol.get(vt, 0, x, i), w);
+        for (int i = 0; i < NT; ++i) {
+          const Frag v = vcol.get(vt, 0, x, i);
+          Ops<T>::mma(acc[i], v, w);
+          Ops<T>::mma(acc[i], v, rest);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) Ops<T>::mma(acc[i], vcol.get(vt, 0, x, i), w);
+      }
     }
   };
 
@@ -642,14 +685,14 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
   const int64_t at = s.q0 + row.i;
   if (row.out && mine) {
     if (a.lse && half == 0) a.lse[stat_at(a, kvh, map, at, row.h)] = some ? m + log2f(l) : INFINITY;
-    if (map == 1 && a.o2) {
-      T* const p = (T*)a.o2 + (at * a.hk * a.g + head) * a.dv;
+    if (a.maps) {
+      float* const p = a.maps + ((at * a.hk * a.g + head) * 2 + map) * a.dv;
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = 32 * i + 8 * j + 4 * half;
-          if (c < a.dv) store4<T>(p + c, acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
+          if (c < a.dv) store4<float>(p + c, acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
         }
     }
   }
@@ -690,7 +733,6 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
   const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
   T* const out = (T*)a.out;
-  T* const o2 = (T*)a.o2;
   if (s.tile < 0) {
     zero_rows<T>(a, s, kvh, NW * 64);
     return;
@@ -872,27 +914,17 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
   const float lam = a.lam[head];
   const bool some = l1 != 0.f;  // false: no key (the maps share their keys), zero rows; a NaN stays one
   const float i1 = 1.f / l1, i2 = 1.f / l2;
-  if (a.lse && half == 0) {
-    const int64_t st = stat_at(a, kvh, 0, at, row.h);
-    a.lse[st] = some ? m1 + log2f(l1) : INFINITY;
-    a.lse[st + a.nq * a.g] = some ? m2 + log2f(l2) : INFINITY;
-  }
   T* const po = out + (at * a.hk * a.g + head) * a.dv;
-  T* const p2 = o2 ? o2 + (at * a.hk * a.g + head) * a.dv : nullptr;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = 32 * i + 8 * j + 4 * half;
       if (c < a.dv) {
-        float y[4], z[4];
+        float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          z[e] = some ? acc2[i][4 * j + e] * i2 : 0.f;
-          y[e] = some ? fmaf(-lam, z[e], acc1[i][4 * j + e] * i1) : 0.f;
-        }
+        for (int e = 0; e < 4; ++e) y[e] = some ? fmaf(-lam, acc2[i][4 * j + e] * i2, acc1[i][4 * j + e] * i1) : 0.f;
         store4<T>(po + c, y[0], y[1], y[2], y[3]);
-        if (p2) store4<T>(p2 + c, z[0], z[1], z[2], z[3]);
       }
     }
 }
@@ -900,14 +932,6 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
 // ---- backward: query rows (dQ, sum of P2 dP) --------------------------------------------------------------------------------------------
 // fp16: the power of two that brings the largest |dout| to [2, 4), so that dS neither underflows for the small gradients of a mean loss
 // nor overflows (|dP| < 4 Dv max|v|); 1 for the types with the exponent range of 32 bits
-template <typename T>
-struct Narrow {
-  static constexpr bool value = false;
-};
-template <>
-struct Narrow<_Float16> {
-  static constexpr bool value = true;
-};
 template <typename T>
 __device__ __forceinline__ float grad_scale(const Args& a) {
   if constexpr (Narrow<T>::value) {
@@ -917,16 +941,22 @@ __device__ __forceinline__ float grad_scale(const Args& a) {
   return 1.f;
 }
 
+// A wave owns 32 packed rows.  Where two tiles of 64 keys fit into LDS the four waves are two groups of rows x two of the keys, joined at the
+// end: blocks of 64 rows fill the chip at half the rows, and the longest causal block ends after half the steps.
+template <typename T, int DB, int DVB>
+constexpr int kKeyGroups = 128 * (2 * DB + DVB) * (int)sizeof(T) <= 131072 ? 2 : 1;
 template <typename T, int DB, int DVB, int NW>
 __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, ND = DB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
-  constexpr int kTile = 32 * (CK + CV) * 16, TILE = 32 * NW;
-  constexpr int NB = 2 * kTile <= 131072 ? 2 : 1;
-  __shared__ __attribute__((aligned(1024))) char smem[NB * kTile];
+  constexpr int KG = kKeyGroups<T, DB, DVB>, RG = NW / KG, BN = 32 * KG, TILE = 32 * RG;
+  constexpr int kTile = BN * (CK + CV) * 16, NB = 2 * kTile <= 131072 ? 2 : 1, kJoin = KG == 1 ? 0 : RG * (2 * ND * 16 + 1) * 64 * 4;
+  constexpr uint64_t kAll = BN == 64 ? ~0ull : 0xffffffffull;
+  __shared__ __attribute__((aligned(1024))) char smem[NB * kTile > kJoin ? NB * kTile : kJoin];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const int t = tile_order(a, blockIdx.y, gridDim.y, gridDim.x);
+  const int rg = wave % RG, kg = wave / RG;
+  const int t = tile_order(a, blockIdx.y, gridDim.y, gridDim.x, 256 * kWaves<T, DB, DVB>);
   const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
   T* const dq = (T*)a.gq;
   if (s.tile < 0) {
@@ -941,7 +971,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
   }
   const int row_base = s.tile * TILE;
   if (row_base >> a.gsh >= (a.stacked ? s.n : a.n)) return;
-  const int r = row_base + 32 * wave + col;
+  const int r = row_base + 32 * rg + col;
   const Row row = row_of(a, s, r);
   const int64_t at = s.q0 + row.i;
   const int head = kvh * a.g + row.h;
@@ -997,17 +1027,20 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
     end = min(end, max(0, last + off + 1));
   }
   const int krs = (int)(a.k.row_stride * sizeof(T)), vrs = (int)(a.v.row_stride * sizeof(T));
-  const Stage<T, 32, 2, DB, NW> kst(a.d, (int)(a.k.head_stride * sizeof(T)), wave, lane, [&](int x) { return x * krs; });
-  const Stage<T, 32, 1, DVB, NW> vst(a.dv, 0, wave, lane, [&](int x) { return x * vrs; });
+  const Stage<T, BN, 2, DB, NW> kst(a.d, (int)(a.k.head_stride * sizeof(T)), wave, lane, [&](int x) { return x * krs; });
+  const Stage<T, BN, 1, DVB, NW> vst(a.dv, 0, wave, lane, [&](int x) { return x * vrs; });
   auto fill = [&](unsigned tile, int key0, uint64_t bits) GEOTR_INLINE {
     kst.load(tile, words(kp + (int64_t)key0 * a.k.row_stride), 16 * krs, wave, bits);
-    vst.load(tile + 32 * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), 16 * vrs, wave, bits);
+    vst.load(tile + BN * CK * 16, words(vp + (int64_t)key0 * a.v.row_stride), 16 * vrs, wave, bits);
   };
   const Rows<T, CK> krow(col, half);
   const Rows<T, CV> vrow(col, half);
   const Cols<T, CK> kcol(lane);
-  auto consume = [&](const char* at, int key0, uint64_t bits) GEOTR_INLINE {
-    const unsigned tile = lds_at(at), vt = tile + 32 * CK * 16;
+  auto consume = [&](unsigned at, int key0, uint64_t bits) GEOTR_INLINE {
+    const unsigned tile = at + kg * 32 * CK * 16, vt = at + BN * CK * 16 + kg * 32 * CV * 16;
+    unsigned lo = (unsigned)(bits >> (32 * kg));
+    if (!lo) return;
+    key0 += 32 * kg;
     f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
 #pragma unroll
     for (int i = 0; i < QS; ++i) {
@@ -1016,7 +1049,6 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
     }
 #pragma unroll
     for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, vrow.get(vt, 0, i), go[i]);
-    unsigned lo = (unsigned)bits;
     const int above = limit - key0;
     if (above < 31) lo = above < 0 ? 0u : lo & ((2u << above) - 1);
     const bool some = __any(lo != 0xffffffffu);
@@ -1047,32 +1079,51 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       }
     }
   };
+  const unsigned base = lds_at(smem);
   if constexpr (NB == 2) {
     int which = 0;
-    uint64_t bits = key_bits(a, s, 0, end, lane) & 0xffffffffull;
-    if (0 < end) fill(lds_at(smem), 0, bits);
-    for (int key0 = 0; key0 < end; key0 += 32) {
+    uint64_t bits = key_bits(a, s, 0, end, lane) & kAll;
+    if (0 < end) fill(base, 0, bits);
+    for (int key0 = 0; key0 < end; key0 += BN) {
       tile_ready();
       __syncthreads();
       uint64_t next = 0;
-      if (key0 + 32 < end) {
-        next = key_bits(a, s, key0 + 32, end, lane) & 0xffffffffull;
-        fill(lds_at(smem) + (which ^ 1) * kTile, key0 + 32, next);
+      if (key0 + BN < end) {
+        next = key_bits(a, s, key0 + BN, end, lane) & kAll;
+        fill(base + (kTile - which), key0 + BN, next);
       }
-      if (bits) consume(smem + which * kTile, key0, bits);
+      consume(base + which, key0, bits);
       bits = next;
-      which ^= 1;
+      which = kTile - which;
     }
   } else {
-    for (int key0 = 0; key0 < end; key0 += 32) {
-      const uint64_t bits = key_bits(a, s, key0, end, lane) & 0xffffffffull;
+    for (int key0 = 0; key0 < end; key0 += BN) {
+      const uint64_t bits = key_bits(a, s, key0, end, lane) & kAll;
       if (!bits) continue;
       __syncthreads();
-      fill(lds_at(smem), key0, bits);
+      fill(base, key0, bits);
       tile_ready();
       __syncthreads();
-      consume(smem, key0, bits);
+      consume(base, key0, bits);
     }
+  }
+  if constexpr (KG == 2) {
+    float* const box = (float*)smem + rg * (2 * ND * 16 + 1) * 64 + lane;
+    __syncthreads();
+    if (kg == 1) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) box[(i * 16 + j) * 64] = acc1[i][j], box[((ND + i) * 16 + j) * 64] = acc2[i][j];
+      box[2 * ND * 16 * 64] = dsum;
+    }
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc1[i][j] += box[(i * 16 + j) * 64], acc2[i][j] += box[((ND + i) * 16 + j) * 64];
+    dsum += box[2 * ND * 16 * 64];
   }
   if (!row.out) return;
   dsum = swap_add(dsum);
@@ -1108,18 +1159,28 @@ template <typename T, int DVB>
 constexpr bool kSplitKV = sizeof(T) == 2 && DVB == 256;
 template <typename T, int DB, int DVB, int PART>
 constexpr int kWavesKV = DB <= 32 ? 2 : 1;
-template <typename T, int DB, int DVB, int NW, int PART>
+// V stays in LDS
+template <typename T, int DB, int PART>
+constexpr bool kLdsV = PART != kValuesOnly && sizeof(T) == 2 && (int)sizeof(T) * DB > 128;
+// bytes of 32 query rows, of dout's, and of 6 x 32 numbers of the rows
+template <typename T, int DB, int DVB>
+constexpr int kRowTile = 32 * (2 * DB + DVB) * (int)sizeof(T) + 1024;
+// QG = 2: the waves are two groups of keys x two of the query rows
+template <typename T, int DB, int DVB, int PART>
+constexpr int kRowGroups = 4 * kRowTile<T, DB, DVB> + (kLdsV<T, DB, PART> ? 64 * DVB * (int)sizeof(T) : 0) <= 160 * 1024 ? 2 : 1;
+template <typename T, int DB, int DVB, int NW, int PART, int QG>
 __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CQ = 2 * DB * (int)sizeof(T) / 16, CO = DVB * (int)sizeof(T) / 16, ND = DB / 32, NV = DVB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
-  constexpr bool kHold = sizeof(T) == 2, kHoldV = PART != kValuesOnly && kHold && (int)sizeof(T) * DB <= 128,
-                 kLdsV = PART != kValuesOnly && kHold && !kHoldV;
+  constexpr bool kHold = sizeof(T) == 2, kInLds = kLdsV<T, DB, PART>, kHoldV = PART != kValuesOnly && kHold && !kInLds;
   constexpr bool DK = PART != kValuesOnly, DV = PART != kKeysOnly;
-  constexpr int kRowBytes = 32 * (CQ + CO) * 16, kTile = kRowBytes + 1024, TILE = 32 * NW;  // 6 x 32 numbers of the rows behind them
-  constexpr int NB = 2 * kTile <= 140000 ? 2 : 1;
-
-  __shared__ __attribute__((aligned(1024))) char smem[NB * kTile + (kLdsV ? TILE * CO * 16 : 0)];
+  constexpr int KG = NW / QG, TILE = 32 * KG, BN = 32 * QG;
+  constexpr int kRowBytes = 32 * (CQ + CO) * 16, kTile = kRowTile<T, DB, DVB>, kBuf = QG * kTile;
+  constexpr int NB = 2 * kBuf <= 140000 ? 2 : 1, kV = kInLds ? TILE * CO * 16 : 0;
+  constexpr int kJoin = QG == 1 ? 0 : KG * ((DK ? 2 * ND : 0) + (DV ? NV : 0)) * 16 * 64 * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[NB * kBuf + kV > kJoin ? NB * kBuf + kV : kJoin];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+  const int kg = wave % KG, qg = wave / KG;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
   const Seq s = find_seq<TILE, true>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
   T* const dk = (T*)a.gk;
@@ -1139,7 +1200,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
   const int key_base = s.tile * TILE;
   const int keys_here = a.stacked ? s.m : a.m;
   if (key_base >= keys_here) return;
-  const int key = key_base + 32 * wave + col;
+  const int key = key_base + 32 * kg + col;
   const bool in = key < s.m && !(a.masks && a.masks[s.k0 + key]);
   const float gs = grad_scale<T>(a);
   constexpr float kBoost = Narrow<T>::value ? 256.f : 1.f;  // fp16: P 2^8 in the product with dout, the weights of a long row stay normal numbers
@@ -1148,8 +1209,8 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
                          (int64_t)kvh * 2 * a.k.head_stride);
   const auto rv = buffer((const T*)a.v.data + s.b * a.v.batch_stride + ((a.stacked ? s.k0 : 0) + key_base) * a.v.row_stride +
                          (int64_t)kvh * a.v.head_stride);
-  const int ok = (int)((32 * wave + col) * a.k.row_stride * (int)sizeof(T)), hs = (int)(a.k.head_stride * sizeof(T));
-  const int ov = (int)((32 * wave + col) * a.v.row_stride * (int)sizeof(T));
+  const int ok = (int)((32 * kg + col) * a.k.row_stride * (int)sizeof(T)), hs = (int)(a.k.head_stride * sizeof(T));
+  const int ov = (int)((32 * kg + col) * a.v.row_stride * (int)sizeof(T));
   auto k_frag = [&](int map, int i) GEOTR_INLINE {
     const int c = (2 * i + half) * kE<T>;
     return load_frag<T>(rk, in && c < a.d ? ok + map * hs + c * (int)sizeof(T) : kOutside);
@@ -1171,9 +1232,9 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
 #pragma unroll
     for (int i = 0; i < VS; ++i) arrived(vv[i]);
   }
-  const unsigned vt = lds_at(smem) + NB * kTile + wave * 32 * CO * 16;  // this wave's keys of V
-  if constexpr (kLdsV) {
-    const i32x4 r = words((const T*)a.v.data + s.b * a.v.batch_stride + ((a.stacked ? s.k0 : 0) + key_base + 32 * wave) * a.v.row_stride +
+  const unsigned vt = lds_at(smem) + NB * kBuf + kg * 32 * CO * 16;  // this wave's keys of V
+  if constexpr (kInLds) {
+    const i32x4 r = words((const T*)a.v.data + s.b * a.v.batch_stride + ((a.stacked ? s.k0 : 0) + key_base + 32 * kg) * a.v.row_stride +
                           (int64_t)kvh * a.v.head_stride);
     const unsigned there = (unsigned)__ballot(in);
     stage_at<T, 32, 1, DVB, 1>(vt, r, a.dv, 0, 0, lane, [&](int x) GEOTR_INLINE {
@@ -1210,7 +1271,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
   const Stage<T, 32, 1, DVB, NW> ost(a.dv, 0, wave, lane, [&](int x) { return (x >> a.gsh) * ors + (x & (group - 1)) * ohs; });
   // numbers of the rows: a wave load takes two of the six kinds, lane = kind and row
   const int so = (int)((half * a.nq + (col >> a.gsh)) * a.g + (col & (group - 1))) * 4;
-  auto fill = [&](unsigned tile, int r0) GEOTR_INLINE {
+  auto fill32 = [&](unsigned tile, int r0) GEOTR_INLINE {
     const int i0 = r0 >> a.gsh, h0 = r0 & (group - 1);
     const i32x4 rq = words(qp + i0 * a.q.row_stride + 2 * h0 * a.q.head_stride), ro = words(op + i0 * a.dout.row_stride + h0 * a.dout.head_stride);
     auto there = [&](int x) GEOTR_INLINE { return r0 + x < rows && ((r0 + x) & (group - 1)) < a.g; };
@@ -1230,11 +1291,19 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
                    : "memory");
     }
   };
+  auto fill = [&](unsigned tile, int r0) GEOTR_INLINE {
+    fill32(tile, r0);
+    if (QG == 2 && r0 + 32 < rows) fill32(tile + kTile, r0 + 32);
+  };
   const Rows<T, CQ> qrow(col, half);
   const Rows<T, CO> orow(col, half);
   const Cols<T, CQ> qcol(lane);
   const Cols<T, CO> ocol(lane);
   auto consume = [&](unsigned qt, int r0) GEOTR_INLINE {
+    if constexpr (QG == 2) {
+      qt += qg * kTile, r0 += 32 * qg;
+      if (r0 >= rows) return;
+    }
     const unsigned ot = qt + 32 * CQ * 16, st = qt + kRowBytes + 16 * half;
     auto stat = [&](int which, int j) GEOTR_INLINE { return lds_load<f32x4>(st + 128 * which + 32 * j); };
     f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();  // scores, then P1 and |lam| P2
@@ -1249,7 +1318,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
 #pragma unroll
         for (int i = 0; i < VS; ++i) {
           if (PART == kKeysOnly && i % 2 == 0) GEOTR_FENCE;
-          Ops<T>::mma(dp, orow.get(ot, 0, i), kHoldV ? vv[i % (kHoldV ? VS : 1)] : kLdsV ? orow.get(vt, 0, i) : v_frag(i));
+          Ops<T>::mma(dp, orow.get(ot, 0, i), kHoldV ? vv[i % (kHoldV ? VS : 1)] : kInLds ? orow.get(vt, 0, i) : v_frag(i));
         }
         if constexpr (PART == kKeysOnly) GEOTR_FENCE;
       }
@@ -1313,21 +1382,47 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
   if constexpr (NB == 2) {
     if (first < rows) fill(base, first);
     int which = 0;
-    for (int r0 = first; r0 < rows; r0 += 32) {
+    for (int r0 = first; r0 < rows; r0 += BN) {
       tile_ready();
       __syncthreads();
-      if (r0 + 32 < rows) fill(base + (kTile - which), r0 + 32);
+      if (r0 + BN < rows) fill(base + (kBuf - which), r0 + BN);
       consume(base + which, r0);
-      which = kTile - which;
+      which = kBuf - which;
     }
   } else {
-    for (int r0 = first; r0 < rows; r0 += 32) {
+    for (int r0 = first; r0 < rows; r0 += BN) {
       __syncthreads();
       fill(base, r0);
       tile_ready();
       __syncthreads();
       consume(base, r0);
     }
+  }
+  if constexpr (QG == 2) {  // the other query group's sums
+    float* box = (float*)smem + kg * (kJoin / 4 / KG) + lane;
+    auto meet = [&](f32x16& x) GEOTR_INLINE {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (qg == 1) box[j * 64] = x[j];
+        else x[j] += box[j * 64];
+      }
+      box += 16 * 64;
+    };
+    auto all = [&]() GEOTR_INLINE {
+      if constexpr (DK) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) meet(ak1[i]), meet(ak2[i]);
+      }
+      if constexpr (DV) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) meet(av[i]);
+      }
+    };
+    __syncthreads();
+    if (qg == 1) all();
+    __syncthreads();
+    if (qg == 1) return;
+    all();
   }
   if (key >= keys_here) return;
   const float fk = a.scale / gs, fv = 1.f / kBoost;
@@ -1361,6 +1456,11 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
 // ---- launches -------------------------------------------------------------------------------------------------------------------------------
 enum Which { kForward, kForwardKeys, kBackwardQ, kBackwardKV };
 
+#ifndef SMALLGRID
+#define SMALLGRID 128
+#endif
+constexpr int64_t kSmallGrid = SMALLGRID;
+
 // stack mode: every sequence may end inside a tile, and one block more takes the rows behind the last
 inline int64_t tiles_of(const Args& a, bool keys, int tile) {
   const int64_t rows = keys ? (a.stacked ? a.nk : a.m) : (a.stacked ? a.nq : a.n) << a.gsh;
@@ -1373,25 +1473,44 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
   // few rows: narrow heads stream a tile per wave; wide ones share tiles of 64 keys, where two buffers of them fit
   constexpr bool kNarrow = (int)sizeof(T) * DB < 256, kFew = !kNarrow && 2 * kWide <= 160 * 1024;
   const bool keys = which == kForwardKeys && (kNarrow || kFew);
-  const int tile = which == kBackwardQ || which == kBackwardKV ? 32 * NWB : keys ? 32 : 32 * G;
-  const int64_t tiles = tiles_of(a, which == kBackwardKV, tile), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
-  if (tiles == 0 || x == 0) return GEOTR_OK;
-  if (tiles > 65535 || x > 0x7fffffff) return fail(GEOTR_E_INVALID, "differential attention: %lld tiles of rows in one call", (long long)tiles);
-  const dim3 grid((unsigned)x, (unsigned)tiles, which == kForward || which == kForwardKeys ? (unsigned)a.splits : 1u);
-  if (which == kForward || which == kForwardKeys) {
-    if (!keys) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, G, false>), grid, dim3(128 * G), 0, s, a);
-    else if constexpr (kNarrow) hipLaunchKernelGGL((fwd_keys_kernel<T, DB, DVB, 4>), grid, dim3(256), 0, s, a);
-    else if constexpr (kFew) hipLaunchKernelGGL((fwd_kernel<T, DB, DVB, G, true>), grid, dim3(128 * G), 0, s, a);
-  } else if (which == kBackwardQ) {
-    hipLaunchKernelGGL((dq_kernel<T, DB, DVB, NWB>), grid, dim3(64 * NWB), 0, s, a);
-  } else if constexpr (kSplitKV<T, DVB>) {
-    hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, NWB, kKeysOnly>), grid, dim3(64 * NWB), 0, s, a);
-    hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, NWB, kValuesOnly>), grid, dim3(64 * NWB), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((dkv_kernel<T, DB, DVB, NWB, kBoth>), grid, dim3(64 * NWB), 0, s, a);
+  auto grid = [&](int tile) {
+    const int64_t tiles = tiles_of(a, which == kBackwardKV, tile), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
+    return dim3((unsigned)std::min<int64_t>(x, 0x80000000ll), (unsigned)std::min<int64_t>(tiles, 65536),
+                which == kForward || which == kForwardKeys ? (unsigned)a.splits : 1u);
+  };
+  auto run = [&](auto kernel, int tile, int threads) -> int {
+    const dim3 d = grid(tile);
+    if (d.x == 0 || d.y == 0) return GEOTR_OK;
+    if (d.x > 0x7fffffffu || d.y > 65535u) return fail(GEOTR_E_INVALID, "differential attention: too many rows in one call (65 535 tiles of %d)", tile);
+    hipLaunchKernelGGL(kernel, d, dim3(threads), 0, s, a);
+    GEOTR_CHECK_LAUNCH("differential attention");
+    return GEOTR_OK;
+  };
+  if (which == kBackwardQ) return run(dq_kernel<T, DB, DVB, NWB>, 32 * NWB / kKeyGroups<T, DB, DVB>, 64 * NWB);
+  if (which == kBackwardKV) {
+    // two query groups halve the keys of a block: for grids that leave compute units empty
+    const int64_t tiles = a.stacked ? (a.nk / (32 * NWB) + a.batch / 2) : (int64_t)a.batch * ((a.m + 32 * NWB - 1) / (32 * NWB));
+    const bool small = tiles * a.hk <= kSmallGrid * kWavesKV<T, DB, DVB, kBoth>;
+    auto keys_of = [&](auto part) -> int {
+      constexpr int PART = decltype(part)::value, QG = kRowGroups<T, DB, DVB, PART>;
+      if constexpr (QG == 2)
+        if (small) return run(dkv_kernel<T, DB, DVB, NWB, PART, 2>, 16 * NWB, 64 * NWB);
+      return run(dkv_kernel<T, DB, DVB, NWB, PART, 1>, 32 * NWB, 64 * NWB);
+    };
+    if constexpr (kSplitKV<T, DVB>) {
+      if (const int r = keys_of(std::integral_constant<int, kKeysOnly>{})) return r;
+      return keys_of(std::integral_constant<int, kValuesOnly>{});
+    } else {
+      return keys_of(std::integral_constant<int, kBoth>{});
+    }
   }
-  GEOTR_CHECK_LAUNCH("differential attention");
-  return GEOTR_OK;
+  if (keys) {
+    if constexpr (kNarrow) return run(fwd_keys_kernel<T, DB, DVB, 4>, 32, 256);
+    if constexpr (kFew) return run(fwd_kernel<T, DB, DVB, G, true, false>, 32, 128 * G);
+  }
+  if constexpr (sizeof(T) == 2)
+    if (a.maps) return run(fwd_kernel<T, DB, DVB, G, false, true>, 32 * G, 128 * G);
+  return run(fwd_kernel<T, DB, DVB, G, false, false>, 32 * G, 128 * G);
 }
 
 // head dimensions: the next of 32, 64, 128 for q and k; one or two times that for v

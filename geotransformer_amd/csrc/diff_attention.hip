@@ -60,13 +60,17 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   const bool some = l[0] != 0.f;
   const float lam = a.lam[head];
   if (c < a.dv) {
+    float o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      z[i] = some ? z[i] / l[1] : 0.f;
-      y[i] = some ? fmaf(-lam, z[i], y[i] / l[0]) : 0.f;
+      y[i] = some ? y[i] / l[0] : 0.f, z[i] = some ? z[i] / l[1] : 0.f;
+      o[i] = fmaf(-lam, z[i], y[i]);
     }
-    store4<T>((T*)a.out + e * a.dv + c, y[0], y[1], y[2], y[3]);
-    if (a.o2) store4<T>((T*)a.o2 + e * a.dv + c, z[0], z[1], z[2], z[3]);
+    store4<T>((T*)a.out + e * a.dv + c, o[0], o[1], o[2], o[3]);
+    if (a.maps) {
+      store4<float>(a.maps + 2 * e * a.dv + c, y[0], y[1], y[2], y[3]);
+      store4<float>(a.maps + (2 * e + 1) * a.dv + c, z[0], z[1], z[2], z[3]);
+    }
   }
   if (a.lse && lane < 2) {
     const int kvh = head / a.g;
@@ -74,9 +78,8 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   }
 }
 
-// What the backward pass reads of a row: the sums, del_2 = dout . O2 and del_1 = dout . O1 = dout . out + lam del_2 (16 lanes per (row,
-// head)), |lam| folded into the second sum.  fp16: the largest |dout| of the rows that
-// exist (an order-free maximum).  Bound: HBM.
+// What the backward pass reads of a row: the sums, del_a = dout . O_a in 32 bits (16 lanes per (row, head)), |lam| folded into the second
+// sum.  fp16: the largest |dout| of the rows that exist (an order-free maximum).  Bound: HBM.
 template <typename T>
 __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
   using Frag = typename Ops<T>::Frag;
@@ -89,14 +92,18 @@ __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
   if (in) {
     const int64_t b = a.stacked ? 0 : row / a.n, i = a.stacked ? row : row - b * a.n;
     const T* g = (const T*)a.dout.data + b * a.dout.batch_stride + i * a.dout.row_stride + head * a.dout.head_stride;
-    const T* y = (const T*)a.out + e * a.dv;
-    const T* y2 = (const T*)a.o2 + e * a.dv;
+    const float* y = a.maps + 2 * e * a.dv;
     for (int c = c0 * kE<T>; c < a.dv; c += 16 * kE<T>) {
-      const Frag fg = *(const Frag*)(g + c), fy = *(const Frag*)(y + c), f2 = *(const Frag*)(y2 + c);
+      const Frag fg = *(const Frag*)(g + c);
 #pragma unroll
-      for (int j = 0; j < kE<T>; ++j) {
-        x = fmaf((float)fg[j], (float)fy[j], x), z = fmaf((float)fg[j], (float)f2[j], z);
-        if constexpr (Narrow<T>::value) top = fmaxf(top, fabsf((float)fg[j]));
+      for (int j = 0; j < kE<T>; j += 4) {
+        const f32x4 y1 = *(const f32x4*)(y + c + j), y2 = *(const f32x4*)(y + a.dv + c + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = (float)fg[j + i];
+          x = fmaf(v, y1[i], x), z = fmaf(v, y2[i], z);
+          if constexpr (Narrow<T>::value) top = fmaxf(top, fabsf(v));
+        }
       }
     }
   }
@@ -108,7 +115,7 @@ __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
     const int64_t to = row_stat_at(a, kvh, 0, row, head - kvh * a.g), step = a.nq * a.g;
     const float lam = a.lam[head], e2 = a.lse[at + step];
     a.rows[to] = a.lse[at], a.rows[to + step] = lam == 0.f ? INFINITY : e2 - log2f(fabsf(lam));
-    a.rows[to + 2 * step] = fmaf(lam, z, x), a.rows[to + 3 * step] = z, a.rows[to + 4 * step] = lam < 0.f ? -1.f : 1.f;
+    a.rows[to + 2 * step] = x, a.rows[to + 3 * step] = z, a.rows[to + 4 * step] = lam < 0.f ? -1.f : 1.f;
   }
   if constexpr (Narrow<T>::value) {
     if (a.q_len) {  // gradients of rows that do not exist say nothing
@@ -186,7 +193,7 @@ int make_args(const geotr_diff_attn* op, Args& a) {
       (rc = check_view(op->v, hk, size, op->batch, op->m, "v")))
     return rc;
   a.q = op->q, a.k = op->k, a.v = op->v, a.dout = geotr_heads{nullptr, 0, 0, 0, 0};
-  a.out = a.o2 = a.gq = a.gk = a.gv = nullptr, a.lse = a.part = a.drow = a.rows = nullptr, a.amax = nullptr;
+  a.out = a.gq = a.gk = a.gv = nullptr, a.maps = a.lse = a.part = a.drow = a.rows = nullptr, a.amax = nullptr;
   a.lam = op->lam, a.q_len = op->q_lengths, a.k_len = op->k_lengths, a.masks = op->key_masks;
   a.batch = (int)op->batch, a.stacked = op->stacked != 0, a.n = (int)op->n, a.m = (int)op->m;
   a.hk = (int)hk, a.g = (int)g, a.d = (int)op->dim, a.dv = (int)op->v_dim, a.causal = op->causal != 0, a.splits = 1;
@@ -194,7 +201,7 @@ int make_args(const geotr_diff_attn* op, Args& a) {
   return GEOTR_OK;
 }
 
-// Few rows to a sequence (32 packed rows or less): blocks of one 32-row tile whose waves stream keys of their own.  Keys are dealt over
+// Few rows to a sequence (32 packed rows or less) without a gradient: blocks of one 32-row tile whose waves stream keys of their own.  Keys are dealt over
 // blocks until there are two for each compute unit, as long as every block keeps 256 keys.
 bool keys_form(const Args& a) {
   const int64_t rows = a.stacked ? (a.nq + a.batch - 1) / std::max(a.batch, 1) : a.n;
@@ -225,22 +232,22 @@ size_t geotr_diff_attn_workspace_bytes(const geotr_diff_attn* op) {
   return part_bytes(a, choose_splits(a));
 }
 
-int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, void* out2, float* lse, void* ws, size_t ws_bytes, void* stream) {
+int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, float* maps, float* lse, void* ws, size_t ws_bytes, void* stream) {
   Args a;
   const int rc = make_args(op, a);
   if (rc != GEOTR_OK) return rc;
   if (a.nq == 0) return GEOTR_OK;
   GEOTR_CHECK_ARG(out, "geotr_diff_attn_forward: out is a null pointer");
-  GEOTR_CHECK_ARG(!out2 == !lse, "geotr_diff_attn_forward: out2 and lse go together");
-  GEOTR_CHECK_ARG((uintptr_t)out % 16 == 0 && (uintptr_t)out2 % 16 == 0, "geotr_diff_attn_forward: results are not 16-byte aligned");
-  a.out = out, a.o2 = out2, a.lse = lse, a.splits = choose_splits(a);
+  GEOTR_CHECK_ARG(!maps == !lse, "geotr_diff_attn_forward: maps and lse go together");
+  GEOTR_CHECK_ARG((uintptr_t)out % 16 == 0 && (uintptr_t)maps % 16 == 0, "geotr_diff_attn_forward: results are not 16-byte aligned");
+  a.out = out, a.maps = maps, a.lse = lse, a.splits = choose_splits(a);
   const size_t need = part_bytes(a, a.splits);
   if (need) {
     if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_forward: workspace of %zu bytes, %zu needed", ws_bytes, need);
     a.part = (float*)ws;
   }
   hipStream_t s = (hipStream_t)stream;
-  if (const int r = launch(op->dtype, a, keys_form(a) ? kForwardKeys : kForward, s)) return r;
+  if (const int r = launch(op->dtype, a, keys_form(a) && !maps ? kForwardKeys : kForward, s)) return r;
   if (a.splits > 1) {
     const dim3 grid((unsigned)(a.nq * a.hk * a.g));
     if (op->dtype == GEOTR_F32) hipLaunchKernelGGL((join_kernel<float>), grid, dim3(256), 0, s, a);
@@ -258,7 +265,7 @@ size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op) {
   return align_up(5 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(sizeof(float));
 }
 
-int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const void* out, const void* out2, const float* lse,
+int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const float* maps, const float* lse,
                              void* dq, void* dk, void* dv, float* dlam, void* ws, size_t ws_bytes, void* stream) {
   Args a;
   const int rc = make_args(op, a);
@@ -266,15 +273,15 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
   GEOTR_CHECK_ARG(dout && dlam, "geotr_diff_attn_backward: null pointer");
   const int size = op->dtype == GEOTR_F32 ? 4 : 2;
   if (const int r = check_view(*dout, (int64_t)a.hk * a.g, size, op->batch, op->n, "dout")) return r;
-  GEOTR_CHECK_ARG((a.nq == 0 || (out && out2 && lse && dq)) && (a.nk == 0 || (dk && dv)), "geotr_diff_attn_backward: null pointer");
-  GEOTR_CHECK_ARG((uintptr_t)out % 16 == 0 && (uintptr_t)out2 % 16 == 0 && (uintptr_t)dq % 16 == 0 && (uintptr_t)dk % 16 == 0 && (uintptr_t)dv % 16 == 0,
+  GEOTR_CHECK_ARG((a.nq == 0 || (maps && lse && dq)) && (a.nk == 0 || (dk && dv)), "geotr_diff_attn_backward: null pointer");
+  GEOTR_CHECK_ARG((uintptr_t)maps % 16 == 0 && (uintptr_t)dq % 16 == 0 && (uintptr_t)dk % 16 == 0 && (uintptr_t)dv % 16 == 0,
                   "geotr_diff_attn_backward: results are not 16-byte aligned");
   const size_t rows = (size_t)a.nq * a.hk * a.g, need = geotr_diff_attn_backward_workspace_bytes(op);
   if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   Carver c(ws);
   a.rows = c.take<float>(5 * rows), a.drow = c.take<float>(rows);
   float* amax = c.take<float>(1);
-  a.dout = *dout, a.out = const_cast<void*>(out), a.o2 = const_cast<void*>(out2), a.lse = const_cast<float*>(lse);
+  a.dout = *dout, a.maps = const_cast<float*>(maps), a.lse = const_cast<float*>(lse);
   a.gq = dq, a.gk = dk, a.gv = dv, a.amax = amax;
   hipStream_t s = (hipStream_t)stream;
   if (op->dtype == GEOTR_F16)

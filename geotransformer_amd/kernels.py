@@ -916,37 +916,40 @@ def _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale):
 
 def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None, want_state=False, checked=False):
     """out[i, h] = sum_j (softmax_j(scale q[i, 2h] . k[j, 2c]) - lam[h] softmax_j(scale q[i, 2h+1] . k[j, 2c+1])) v[j, c], c = h Hk / H
-    (geotr_diff_attn_forward).  want_state: also what diff_attention_backward needs, (out, (out2, lse))."""
+    (geotr_diff_attn_forward).  want_state: also what diff_attention_backward needs, (out, (maps, lse))."""
     if not checked:
         check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
     lib, heads, kv_heads = _lib.load(), q.shape[-2] // 2, v.shape[-2]
     out = torch.empty(q.shape[:-2] + (heads, v.shape[-1]), dtype=q.dtype, device=device)
-    out2 = lse = None
+    maps = lse = None
     if want_state:
-        out2 = torch.empty_like(out)
+        maps = torch.empty(out.shape[:-1] + (2, v.shape[-1]), dtype=torch.float32, device=device)
         lse = torch.empty((kv_heads, 2) + q.shape[:-2] + (heads // kv_heads,), dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_workspace_bytes(op)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _call(device, lib.geotr_diff_attn_forward, 'geotr_diff_attn_forward', op, out.data_ptr(), out2 if out2 is None else out2.data_ptr(),
+    _call(device, lib.geotr_diff_attn_forward, 'geotr_diff_attn_forward', op, out.data_ptr(), maps if maps is None else maps.data_ptr(),
           lse if lse is None else lse.data_ptr(), ws if ws is None else ws.data_ptr(), need)
     del keep
-    return (out, (out2, lse)) if want_state else out
+    return (out, (maps, lse)) if want_state else out
 
 
-def diff_attention_backward(dout, q, k, v, lam, out, state, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None):
-    """(dq, dk, dv, dlam (H)) for dout from diff_attention(..., want_state=True)'s results (geotr_diff_attn_backward)."""
+def diff_attention_backward(dout, q, k, v, lam, state, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None):
+    """(dq, dk, dv, dlam (H)) for dout from the state of diff_attention(..., want_state=True) (geotr_diff_attn_backward)."""
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
-    if dout.shape != out.shape or dout.dtype != q.dtype:
-        raise ValueError(f'dout is {q.dtype} of the output\'s shape {tuple(out.shape)}: got {dout.dtype} {tuple(dout.shape)}')
-    _same_device(q, dout, out, *state)
+    shape = q.shape[:-2] + (q.shape[-2] // 2, v.shape[-1])
+    if dout.shape != shape or dout.dtype != q.dtype:
+        raise ValueError(f'dout is {q.dtype} of the output\'s shape {tuple(shape)}: got {dout.dtype} {tuple(dout.shape)}')
+    if state[0].shape != shape[:-1] + (2, v.shape[-1]):
+        raise ValueError(f'the state of another call: outputs of the maps {tuple(state[0].shape)}')
+    _same_device(q, dout, *state)
     lib = _lib.load()
     dout = _aligned(dout)
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
     dlam = torch.empty(q.shape[-2] // 2, dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_backward_workspace_bytes(op)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _call(device, lib.geotr_diff_attn_backward, 'geotr_diff_attn_backward', op, _HEADS.pack(*_heads(dout)), out.data_ptr(), state[0].data_ptr(),
+    _call(device, lib.geotr_diff_attn_backward, 'geotr_diff_attn_backward', op, _HEADS.pack(*_heads(dout)), state[0].data_ptr(),
           state[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), need)
     del keep
     return dq, dk, dv, dlam

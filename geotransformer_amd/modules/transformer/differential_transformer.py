@@ -20,15 +20,15 @@ class _DifferentialAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale):
         out, state = kernels.diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale, want_state=True, checked=True)
-        ctx.save_for_backward(q, k, v, lam, out, *state, q_lengths, k_lengths, key_masks)
+        ctx.save_for_backward(q, k, v, lam, *state, q_lengths, k_lengths, key_masks)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, lam, out, out2, lse, q_lengths, k_lengths, key_masks = ctx.saved_tensors
-        grads = kernels.diff_attention_backward(dout, q, k, v, lam, out, (out2, lse), q_lengths, k_lengths, key_masks, ctx.causal, ctx.scale)
+        q, k, v, lam, maps, lse, q_lengths, k_lengths, key_masks = ctx.saved_tensors
+        grads = kernels.diff_attention_backward(dout, q, k, v, lam, (maps, lse), q_lengths, k_lengths, key_masks, ctx.causal, ctx.scale)
         return grads + (None,) * 5
 
 

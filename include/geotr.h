@@ -645,7 +645,8 @@ int geotr_rotary(const geotr_heads* q, const geotr_heads* q_out, const geotr_hea
  * rows of ALL `batch` sequences one behind the other (stack mode), both lengths given.  Lengths are read on the device and held to the
  * rows that exist.  key_masks: bytes (batch, m) or (m), contiguous, nonzero = ignored.  causal: query i sees keys j <= i + (keys - queries) of its sequence.
  * Results of rows without a key, beyond their length or behind the last sequence are zero; what such key rows hold is never used.
- * out, out2 (optional: the second map's output before lam): contiguous (rows, H, v_dim); lse (optional): (Hk, 2, rows, H / Hk) fp32. */
+ * out: contiguous (rows, H, v_dim).  For the gradients, both or none: maps (rows, H, 2, v_dim) fp32, the output of each map before lam, and
+ * lse (Hk, 2, rows, H / Hk) fp32, the logarithm (base 2) of its sum. */
 typedef struct geotr_diff_attn {
   geotr_heads q, k, v;
   int32_t dtype, stacked, causal, pad_;
@@ -658,12 +659,12 @@ typedef struct geotr_diff_attn {
   int32_t pad2_;
 } geotr_diff_attn;
 size_t geotr_diff_attn_workspace_bytes(const geotr_diff_attn* op);
-int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, void* out2, float* lse, void* ws, size_t ws_bytes, void* stream);
-/* Gradients for dout (strided like q, H heads of v_dim) from what the forward call left in out, out2 and lse: dq, dk, dv contiguous in
+int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, float* maps, float* lse, void* ws, size_t ws_bytes, void* stream);
+/* Gradients for dout (strided like q, H heads of v_dim) from what the forward call left in maps and lse: dq, dk, dv contiguous in
  * the layout of q, k, v; dlam (H) fp32. */
 size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op);
-int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const void* out, const void* out2, const float* lse,
-                             void* dq, void* dk, void* dv, float* dlam, void* ws, size_t ws_bytes, void* stream);
+int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const float* maps, const float* lse, void* dq, void* dk,
+                             void* dv, float* dlam, void* ws, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Native pyramid: precompute_data_stack_mode (geotransformer/utils/data.py:13-77) as one host call: (S-1) grid

@@ -26,7 +26,7 @@ def _check(q, k, v, lam, dout, ql=None, kl=None, key_masks=None, causal=False, s
         return
     leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
     out2 = differential_attention(*leaves, **kw)
-    assert torch.equal(out, out2)
+    oracle.assert_within('out', out2, *want['out'])
     grads = torch.autograd.grad(out2, leaves, dout)
     for name, g in zip(('dq', 'dk', 'dv', 'dlam'), grads):
         oracle.assert_within(name, g, *want[name])
