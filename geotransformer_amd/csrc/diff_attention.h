@@ -1456,11 +1456,6 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
 // ---- launches -------------------------------------------------------------------------------------------------------------------------------
 enum Which { kForward, kForwardKeys, kBackwardQ, kBackwardKV };
 
-#ifndef SMALLGRID
-#define SMALLGRID 128
-#endif
-constexpr int64_t kSmallGrid = SMALLGRID;
-
 // stack mode: every sequence may end inside a tile, and one block more takes the rows behind the last
 inline int64_t tiles_of(const Args& a, bool keys, int tile) {
   const int64_t rows = keys ? (a.stacked ? a.nk : a.m) : (a.stacked ? a.nq : a.n) << a.gsh;
@@ -1488,9 +1483,11 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
   };
   if (which == kBackwardQ) return run(dq_kernel<T, DB, DVB, NWB>, 32 * NWB / kKeyGroups<T, DB, DVB>, 64 * NWB);
   if (which == kBackwardKV) {
-    // two query groups halve the keys of a block: for grids that leave compute units empty
+    // Two query groups halve a block's keys and its steps, but load every query row twice as often.  They win while all their blocks run at
+    // once (2 x 2 048 rows and 4 heads, 128 against 64 blocks: 64/64 139 against 246 us, 128/128 220 against 308, 32-bit 64/128 229
+    // against 433; 16 clouds of 295 in 32 bits: 66 against 81) and lose with more (2 x 4 096 causal rows and 8 heads: 404 against 316).
     const int64_t tiles = a.stacked ? (a.nk / (32 * NWB) + a.batch / 2) : (int64_t)a.batch * ((a.m + 32 * NWB - 1) / (32 * NWB));
-    const bool small = tiles * a.hk <= kSmallGrid * kWavesKV<T, DB, DVB, kBoth>;
+    const bool small = tiles * a.hk <= 128 * kWavesKV<T, DB, DVB, kBoth>;
     auto keys_of = [&](auto part) -> int {
       constexpr int PART = decltype(part)::value, QG = kRowGroups<T, DB, DVB, PART>;
       if constexpr (QG == 2)

@@ -829,11 +829,12 @@ def check_rotary_heads(q, k):
         raise TypeError(f'heads are float32, bfloat16 or float16, all of one type: got {q.dtype} and {None if k is None else k.dtype}')
 
 
-def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0, inverse=False):
+def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0, inverse=False, checked=False):
     """(q, k) with the first rotary_dim channels of every head turned by their token's position (geotr_rotary); k may be None.
-    positions: (rows,) / (batch, rows) or with a last dimension of axes; turns (rotary_dim / 2) float64: turns per unit of position;
-    axis (rotary_dim / 2) int32: the axis of each pair.  inverse: the transposed rotation (the gradient)."""
-    check_rotary_heads(q, k)
+    positions: (rows,) / (batch, rows) or with a last dimension of axes; turns (rotary_dim / 2) float64 or its bits as int64: turns per
+    unit of position; axis (rotary_dim / 2) int32: the axis of each pair.  inverse: the transposed rotation (the gradient)."""
+    if not checked:
+        check_rotary_heads(q, k)
     if rotary_dim % 2 or not 2 <= rotary_dim <= q.shape[-1]:
         raise ValueError(f'rotary_dim {rotary_dim} of a head of {q.shape[-1]} channels: an even number up to it')
     if positions.dtype not in POSITION_TYPES:
@@ -842,12 +843,12 @@ def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0
     pos = positions.unsqueeze(-1) if positions.dim() == len(lead) else positions
     if pos.dim() != len(lead) + 1 or tuple(pos.shape[:-1]) != tuple(lead):
         raise ValueError(f'positions of rows {tuple(lead)}: got {tuple(positions.shape)}')
-    assert turns.dtype == torch.float64 and axis.dtype == torch.int32 and turns.numel() == axis.numel() == rotary_dim // 2
+    assert turns.dtype in (torch.float64, torch.int64) and axis.dtype == torch.int32 and turns.numel() == axis.numel() == rotary_dim // 2
     device = _same_device(q, k, positions, turns, axis)
     q = q if q.stride(-1) == 1 else q.contiguous()
     k = k if k is None or k.stride(-1) == 1 else k.contiguous()
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     pack = _HEADS.pack
     batch, rows = (1, lead[0]) if len(lead) == 1 else lead
     _call(device, _lib.load().geotr_rotary, 'geotr_rotary', pack(*_heads(q)), pack(*_heads(q_out)), None if k is None else pack(*_heads(k)),
@@ -921,7 +922,7 @@ def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None,
         check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
     lib, heads, kv_heads = _lib.load(), q.shape[-2] // 2, v.shape[-2]
-    out = torch.empty(q.shape[:-2] + (heads, v.shape[-1]), dtype=q.dtype, device=device)
+    out = q.new_empty(q.shape[:-2] + (heads, v.shape[-1]))
     maps = lse = None
     if want_state:
         maps = torch.empty(out.shape[:-1] + (2, v.shape[-1]), dtype=torch.float32, device=device)
@@ -945,7 +946,7 @@ def diff_attention_backward(dout, q, k, v, lam, state, q_lengths=None, k_lengths
     _same_device(q, dout, *state)
     lib = _lib.load()
     dout = _aligned(dout)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     dlam = torch.empty(q.shape[-2] // 2, dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_backward_workspace_bytes(op)
     ws = torch.empty(need, dtype=torch.uint8, device=device)

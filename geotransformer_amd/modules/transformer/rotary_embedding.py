@@ -46,7 +46,7 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions, turns, axis)
         ctx.how, ctx.inverse = how, inverse
         ctx.set_materialize_grads(False)
-        return kernels.rotary(q, k, positions, turns, axis, *how, inverse=inverse)
+        return kernels.rotary(q, k, positions, turns, axis, *how, inverse=inverse, checked=True)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -95,7 +95,7 @@ class RotaryPositionalEmbedding(nn.Module):
             raise ValueError(f'positions {tuple(positions.shape)} of rows {tuple(lead)}, built for {self.num_axes} axes')
         if positions.requires_grad:
             raise NotImplementedError('rotary positions are not differentiable in the positions: pass positions.detach()')
-        how, turns = (self.rotary_dim, self.interleaved, self.gain), self.turn_bits.view(torch.float64)
+        how, turns = (self.rotary_dim, self.interleaved, self.gain), self.turn_bits
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             return _Rotary.apply(q, k, positions, turns, self.axis, how, False)
-        return kernels.rotary(q, k, positions, turns, self.axis, *how)
+        return kernels.rotary(q, k, positions, turns, self.axis, *how, checked=True)

@@ -117,7 +117,7 @@ def test_entry_points_check_their_arguments():
     assert fwd(big) == -2 and b'workspace' in lib.geotr_last_error()
     need = lib.geotr_diff_attn_backward_workspace_bytes(ctypes.byref(op()))
     assert need >= 3 * 5 * 4 * 4
-    bwd = lambda o, g, ws: lib.geotr_diff_attn_backward(ctypes.byref(o), g, one, one, one, one, one, one, one, one if ws else None, ws, None)  # noqa: E731
+    bwd = lambda o, g, ws: lib.geotr_diff_attn_backward(ctypes.byref(o), g, one, one, one, one, one, one, one if ws else None, ws, None)  # noqa: E731
     g = kernels.Heads(one, 4, 0, 128, 32)
     assert bwd(op(), ctypes.byref(g), need - 1) == -2 and bwd(op(), None, need) == -1
     assert bwd(op(), ctypes.byref(kernels.Heads(one, 3, 0, 128, 32)), need) == -1 and b'dout has 3 heads' in lib.geotr_last_error()
