@@ -225,6 +225,9 @@ template <class V>
 __device__ __forceinline__ void arrived(V& x) {
   asm volatile("" : "+v"(x));
 }
+// x lies in accumulation registers here: without it the compiler takes the same ones for the scores, 64 moves a tile (dK/dV 327 -> 276 us at
+// 2 x 4 096 causal rows and 8 heads; 128/128 at 2 x 2 048 and 4: 222 -> 129)
+__device__ __forceinline__ void held(f32x16& x) { asm volatile("" : "+a"(x)); }
 template <typename T>
 __device__ __forceinline__ typename Ops<T>::Frag load_frag(__amdgpu_buffer_rsrc_t r, int offset) {
   return __builtin_bit_cast(typename Ops<T>::Frag, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
@@ -1047,6 +1050,10 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       Ops<T>::mma(s1, krow.get(tile, 0, i), q1[i]);
       Ops<T>::mma(s2, krow.get(tile, 0, CK / 4 + i), q2[i]);
     }
+    if constexpr (kWaves<T, DB, DVB> == 1) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i) held(acc1[i]), held(acc2[i]);
+    }
 #pragma unroll
     for (int i = 0; i < VS; ++i) Ops<T>::mma(dp, vrow.get(vt, 0, i), go[i]);
     const int above = limit - key0;
@@ -1312,6 +1319,16 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
       Ops<T>::mma(s1, qrow.get(qt, 0, i), kHold ? k1[i % (kHold ? QS : 1)] : k_frag(0, i));
       Ops<T>::mma(s2, qrow.get(qt, 0, CQ / 4 + i), kHold ? k2[i % (kHold ? QS : 1)] : k_frag(1, i));
     }
+    if constexpr (kWavesKV<T, DB, DVB, PART> == 1) {
+      if constexpr (DK) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) held(ak1[i]), held(ak2[i]);
+      }
+      if constexpr (DV) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) held(av[i]);
+      }
+    }
     if constexpr (PART == kKeysOnly) GEOTR_FENCE;
     auto weights = [&](auto from) GEOTR_INLINE {  // beside the products of dP
       if constexpr (DK) {
@@ -1330,7 +1347,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
           const int i = 4 * j + e;
           s1[i] = __builtin_amdgcn_exp2f(from(s1[i], e1[e])), s2[i] = __builtin_amdgcn_exp2f(from(s2[i], e2[e]));
         }
-          }
+      }
     };
     const float own = fabsf(lds_load<float>(qt + kRowBytes + 128 * half + 4 * col));  // lane: row and map
     if (__builtin_expect(__any(own > kHuge && own < INFINITY), 0)) weights([&](float x, float e) { return x * a.scale_log2 - e; });

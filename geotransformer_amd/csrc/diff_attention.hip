@@ -10,14 +10,15 @@ namespace {
 
 constexpr int kMostSplits = 64;  // the join holds one split per lane
 
-// One block per (row, head): every wave holds the splits' maxima and sums in its lanes, four channels of both maps in a lane, and takes
-// every fourth split; the waves meet in LDS in a fixed order.  Bound: HBM where rows are many, latency for single tokens (a wave per row that
-// walked the splits took 82 us for 16 rows of 64 splits).
-template <typename T>
+// Every wave holds the splits' maxima and sums in its lanes and four channels of both maps in a lane.  W waves to a (row, head) take the
+// splits in turn and meet in LDS in a fixed order: four for many splits (single tokens, where latency counts: one wave took 82 us for 16
+// rows of 64 splits, four 6), one for few (many rows: 12 us against 28 at 16 384 rows of two splits).
+template <typename T, int W>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
-  __shared__ f32x4 box[4][2][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, heads = a.hk * a.g;
-  const int64_t e = blockIdx.x, row = e / heads;
+  __shared__ f32x4 box[W][2][64];
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, heads = a.hk * a.g;
+  const int64_t e = W == 1 ? blockIdx.x * 4ll + (threadIdx.x >> 6) : blockIdx.x, row = e / heads;
+  if (W == 1 && e >= a.nq * heads) return;
   const int head = (int)(e - row * heads), w = a.dv + 4, c = 4 * lane;
   const int64_t step = a.nq * heads * 2 * (int64_t)w;
   const float* p = a.part + e * 2 * w;
@@ -37,7 +38,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   }
   f32x4 y = {}, z = {};
 #pragma unroll 4
-  for (int s = wave; s < a.splits; s += 4) {
+  for (int s = wave; s < a.splits; s += W) {
     const float f1 = __shfl(f[0], s, 64), f2 = __shfl(f[1], s, 64);
     if (c < a.dv) {
       const f32x4 u = *(const f32x4*)(p + s * step + 4 + c), v = *(const f32x4*)(p + s * step + w + 4 + c);
@@ -48,14 +49,16 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
       }
     }
   }
-  box[wave][0][lane] = y, box[wave][1][lane] = z;
-  __syncthreads();
-  if (wave) return;
+  if constexpr (W > 1) {
+    box[wave][0][lane] = y, box[wave][1][lane] = z;
+    __syncthreads();
+    if (wave) return;
 #pragma unroll
-  for (int x = 1; x < 4; ++x) {
-    const f32x4 u = box[x][0][lane], v = box[x][1][lane];
+    for (int x = 1; x < W; ++x) {
+      const f32x4 u = box[x][0][lane], v = box[x][1][lane];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] += u[i], z[i] += v[i];
+      for (int i = 0; i < 4; ++i) y[i] += u[i], z[i] += v[i];
+    }
   }
   const bool some = l[0] != 0.f;
   const float lam = a.lam[head];
@@ -249,10 +252,13 @@ int geotr_diff_attn_forward(const geotr_diff_attn* op, void* out, float* maps, f
   hipStream_t s = (hipStream_t)stream;
   if (const int r = launch(op->dtype, a, keys_form(a) && !maps ? kForwardKeys : kForward, s)) return r;
   if (a.splits > 1) {
-    const dim3 grid((unsigned)(a.nq * a.hk * a.g));
-    if (op->dtype == GEOTR_F32) hipLaunchKernelGGL((join_kernel<float>), grid, dim3(256), 0, s, a);
-    else if (op->dtype == GEOTR_BF16) hipLaunchKernelGGL((join_kernel<__bf16>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((join_kernel<_Float16>), grid, dim3(256), 0, s, a);
+    const int64_t rows = a.nq * a.hk * a.g;
+    const bool many = a.splits > 4;
+    const dim3 grid((unsigned)(many ? rows : (rows + 3) / 4));
+    auto join = [&](auto one, auto four) { hipLaunchKernelGGL(many ? four : one, grid, dim3(256), 0, s, a); };
+    if (op->dtype == GEOTR_F32) join(join_kernel<float, 1>, join_kernel<float, 4>);
+    else if (op->dtype == GEOTR_BF16) join(join_kernel<__bf16, 1>, join_kernel<__bf16, 4>);
+    else join(join_kernel<_Float16, 1>, join_kernel<_Float16, 4>);
     GEOTR_CHECK_LAUNCH("geotr_diff_attn_forward");
   }
   return GEOTR_OK;
