@@ -38,8 +38,8 @@ struct Args {
   geotr_heads q, k, v, dout;             // dout: backward only
   void *out, *gq, *gk, *gv;              // contiguous (rows, heads, channels)
   float* maps;                           // (rows, heads, 2, dv): the maps' outputs, for the backward pass
-  float *lse, *part, *drow;              // (hk, 2, nq, g), split partials, (hk, nq, g)
-  float* rows;                           // backward, (hk, 5, nq, g): lse1, lse2 - log2 |lam|, del1, del2, sign of lam
+  float *lse, *part, *drow;              // (hk, 4, nq, g): see store_sums; split partials; (hk, nq, g)
+  float* rows;                           // backward, (hk, 7, nq, g): lse1, lse2 - log2 |lam|, del1, del2, sign of lam, rest of lse1, of lse2
   const float* amax;                     // 16-bit floats of narrow range: largest |dout| (backward), else null
   const float* lam;
   const int64_t *q_len, *k_len;
@@ -377,10 +377,10 @@ __device__ __forceinline__ f32x16 zero16() {
 // rounded maximum b grows with it until the exponential overflows; rounded alike, the largest score gives exactly 0.
 constexpr float kHuge = 1048576.f;
 template <class B>
-__device__ __forceinline__ void exponents(f32x16& s, float c, B b, bool huge) {
+__device__ __forceinline__ void exponents(f32x16& s, float c, B b, bool huge, float rest = 0.f) {
   if (__builtin_expect(huge, 0)) {  // a branch of the wave, not a choice per element
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = s[i] * c - b(i);
+    for (int i = 0; i < 16; ++i) s[i] = (s[i] * c - b(i)) - rest;
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], c, -b(i));
@@ -403,11 +403,20 @@ __device__ __forceinline__ Row row_of(const Args& a, const Seq& s, int r) {
   return x;
 }
 __device__ __forceinline__ int64_t stat_at(const Args& a, int kvh, int map, int64_t row, int h) {
-  return (((int64_t)kvh * 2 + map) * a.nq + row) * a.g + h;
+  return (((int64_t)kvh * 4 + map) * a.nq + row) * a.g + h;
 }
 
 __device__ __forceinline__ int64_t row_stat_at(const Args& a, int kvh, int which, int64_t row, int h) {
-  return (((int64_t)kvh * 5 + which) * a.nq + row) * a.g + h;
+  return (((int64_t)kvh * 7 + which) * a.nq + row) * a.g + h;
+}
+
+// What the backward pass takes weights from: log2 of the sum, m + log2 l.  Beyond 2^20 that would round log2 l away (weights off by 4 % at
+// 2^20, all 1 further on), so there m and log2 l are kept apart.  Rows without a key: infinity, weights of zero.
+__device__ __forceinline__ void store_sums(const Args& a, int64_t at, float m, float l, bool some) {
+  const float log = log2f(l);
+  const bool far = fabsf(m) > kHuge;
+  a.lse[at] = some ? (far ? m : m + log) : INFINITY;
+  a.lse[at + 2 * a.nq * a.g] = some && far ? log : 0.f;
 }
 
 // four consecutive channels of an output row
@@ -455,6 +464,7 @@ __device__ __forceinline__ void zero_rows(const Args& a, const Seq& s, int kvh, 
   for (int64_t e = first; a.lse && e < rows * a.g; e += step) {
     const int64_t at = stat_at(a, kvh, 0, s.q_end, 0) + e;
     a.lse[at] = a.lse[at + a.nq * a.g] = INFINITY;
+    a.lse[at + 2 * a.nq * a.g] = a.lse[at + 3 * a.nq * a.g] = 0.f;
   }
 }
 
@@ -687,7 +697,7 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
     for (int j = 0; j < 16; ++j) acc[i][j] = some ? acc[i][j] * inv : 0.f;
   const int64_t at = s.q0 + row.i;
   if (row.out && mine) {
-    if (a.lse && half == 0) a.lse[stat_at(a, kvh, map, at, row.h)] = some ? m + log2f(l) : INFINITY;
+    if (a.lse && half == 0) store_sums(a, stat_at(a, kvh, map, at, row.h), m, l, some);
     if (a.maps) {
       float* const p = a.maps + ((at * a.hk * a.g + head) * 2 + map) * a.dv;
 #pragma unroll
@@ -1002,14 +1012,14 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       go[i] = load_frag<T>(ro, row.in && c < a.dv ? oo + c * (int)sizeof(T) : kOutside);
     }
   }
-  float lse1 = INFINITY, lse2 = INFINITY, del1 = 0.f, del2 = 0.f, lam = 0.f;
+  float lse1 = INFINITY, lse2 = INFINITY, rest1 = 0.f, rest2 = 0.f, del1 = 0.f, del2 = 0.f, lam = 0.f;
   if (row.in) {
     const int64_t st = stat_at(a, kvh, 0, at, row.h);
-    lse1 = a.lse[st], lse2 = a.lse[st + a.nq * a.g], lam = a.lam[head];
+    lse1 = a.lse[st], lse2 = a.lse[st + a.nq * a.g], rest1 = a.lse[st + 2 * a.nq * a.g], rest2 = a.lse[st + 3 * a.nq * a.g], lam = a.lam[head];
     const int64_t rs = row_stat_at(a, kvh, 2, at, row.h);
     del1 = a.rows[rs], del2 = a.rows[rs + a.nq * a.g];
   }
-  arrived(lse1), arrived(lse2), arrived(del1), arrived(del2), arrived(lam);
+  arrived(lse1), arrived(lse2), arrived(rest1), arrived(rest2), arrived(del1), arrived(del2), arrived(lam);
 #pragma unroll
   for (int i = 0; i < QS; ++i) arrived(q1[i]), arrived(q2[i]);
 #pragma unroll
@@ -1060,8 +1070,8 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
     if (above < 31) lo = above < 0 ? 0u : lo & ((2u << above) - 1);
     const bool some = __any(lo != 0xffffffffu);
     lo >>= 4 * half;
-    exponents(s1, a.scale_log2, [&](int) { return lse1; }, huge);
-    exponents(s2, a.scale_log2, [&](int) { return lse2; }, huge);
+    exponents(s1, a.scale_log2, [&](int) { return lse1; }, huge, rest1);
+    exponents(s2, a.scale_log2, [&](int) { return lse2; }, huge, rest2);
     if (__builtin_expect(some, 0)) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -1169,7 +1179,7 @@ constexpr int kWavesKV = DB <= 32 ? 2 : 1;
 // V stays in LDS
 template <typename T, int DB, int PART>
 constexpr bool kLdsV = PART != kValuesOnly && sizeof(T) == 2 && (int)sizeof(T) * DB > 128;
-// bytes of 32 query rows, of dout's, and of 6 x 32 numbers of the rows
+// bytes of 32 query rows, of dout's, and of 8 x 32 numbers of the rows
 template <typename T, int DB, int DVB>
 constexpr int kRowTile = 32 * (2 * DB + DVB) * (int)sizeof(T) + 1024;
 // QG = 2: the waves are two groups of keys x two of the query rows
@@ -1276,7 +1286,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
   const int group = 1 << a.gsh, q16 = group <= 16 ? (16 >> a.gsh) * qrs : 32 * qhs, o16 = group <= 16 ? (16 >> a.gsh) * ors : 16 * ohs;
   const Stage<T, 32, 2, DB, NW> qst(a.d, qhs, wave, lane, [&](int x) { return (x >> a.gsh) * qrs + (x & (group - 1)) * 2 * qhs; });
   const Stage<T, 32, 1, DVB, NW> ost(a.dv, 0, wave, lane, [&](int x) { return (x >> a.gsh) * ors + (x & (group - 1)) * ohs; });
-  // numbers of the rows: a wave load takes two of the six kinds, lane = kind and row
+  // numbers of the rows: a wave load takes two of the seven kinds, lane = kind and row
   const int so = (int)((half * a.nq + (col >> a.gsh)) * a.g + (col & (group - 1))) * 4;
   auto fill32 = [&](unsigned tile, int r0) GEOTR_INLINE {
     const int i0 = r0 >> a.gsh, h0 = r0 & (group - 1);
@@ -1290,11 +1300,11 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
       ost.load_some(tile + 32 * CQ * 16, ro, o16, wave, there);
     }
     // rows that do not exist: zeros, and their products are zero because q and dout are
-    for (int x = wave; x < 3; x += NW) {
+    for (int x = wave; x < 4; x += NW) {
       const i32x4 rs = words(sp + ((int64_t)(2 * x) * a.nq + i0) * a.g + h0);
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                    :
-                   : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) && 2 * x + half < 5 ? so : kOutside), "s"(rs)
+                   : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) && 2 * x + half < 7 ? so : kOutside), "s"(rs)
                    : "memory");
     }
   };
@@ -1330,7 +1340,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
       }
     }
     if constexpr (PART == kKeysOnly) GEOTR_FENCE;
-    auto weights = [&](auto from) GEOTR_INLINE {  // beside the products of dP
+    auto weights = [&](auto from, auto far) GEOTR_INLINE {  // beside the products of dP
       if constexpr (DK) {
 #pragma unroll
         for (int i = 0; i < VS; ++i) {
@@ -1342,16 +1352,18 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const f32x4 e1 = stat(0, j), e2 = stat(1, j);
+        f32x4 r1 = {}, r2 = {};
+        if constexpr (decltype(far)::value) r1 = stat(5, j), r2 = stat(6, j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * j + e;
-          s1[i] = __builtin_amdgcn_exp2f(from(s1[i], e1[e])), s2[i] = __builtin_amdgcn_exp2f(from(s2[i], e2[e]));
+          s1[i] = __builtin_amdgcn_exp2f(from(s1[i], e1[e], r1[e])), s2[i] = __builtin_amdgcn_exp2f(from(s2[i], e2[e], r2[e]));
         }
       }
     };
     const float own = fabsf(lds_load<float>(qt + kRowBytes + 128 * half + 4 * col));  // lane: row and map
-    if (__builtin_expect(__any(own > kHuge && own < INFINITY), 0)) weights([&](float x, float e) { return x * a.scale_log2 - e; });
-    else weights([&](float x, float e) { return fmaf(x, a.scale_log2, -e); });
+    if (__builtin_expect(__any(own > kHuge && own < INFINITY), 0)) weights([&](float x, float e, float r) { return (x * a.scale_log2 - e) - r; }, std::true_type{});
+    else weights([&](float x, float e, float) { return fmaf(x, a.scale_log2, -e); }, std::false_type{});
     if (a.causal && r0 < last) {  // rows that do not see some key of the block
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -1501,15 +1513,17 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
   if (which == kBackwardQ) return run(dq_kernel<T, DB, DVB, NWB>, 32 * NWB / kKeyGroups<T, DB, DVB>, 64 * NWB);
   if (which == kBackwardKV) {
     // Two query groups halve a block's keys and its steps, but load every query row twice as often.  They win while all their blocks run at
-    // once (2 x 2 048 rows and 4 heads, 128 against 64 blocks: 64/64 139 against 246 us, 128/128 220 against 308, 32-bit 64/128 229
-    // against 433; 16 clouds of 295 in 32 bits: 66 against 81) and lose with more (2 x 4 096 causal rows and 8 heads: 404 against 316).
+    // once (2 x 2 048 rows and 4 heads, 128 against 64 blocks: 64/64 139 against 246 us, 128/128 220 against 308) and lose with more
+    // (2 x 4 096 causal rows and 8 heads: 404 against 316).  32-bit products take 16 times as long as the loads: always (32 clouds of 295
+    // rows: 119 against 128 us; 4 x 2 048 rows, 4 heads: 368 against 481).
     const int64_t tiles = a.stacked ? (a.nk / (32 * NWB) + a.batch / 2) : (int64_t)a.batch * ((a.m + 32 * NWB - 1) / (32 * NWB));
     const bool small = tiles * a.hk <= 128 * kWavesKV<T, DB, DVB, kBoth>;
     auto keys_of = [&](auto part) -> int {
       constexpr int PART = decltype(part)::value, QG = kRowGroups<T, DB, DVB, PART>;
       if constexpr (QG == 2)
-        if (small) return run(dkv_kernel<T, DB, DVB, NWB, PART, 2>, 16 * NWB, 64 * NWB);
-      return run(dkv_kernel<T, DB, DVB, NWB, PART, 1>, 32 * NWB, 64 * NWB);
+        if (sizeof(T) == 4 || small) return run(dkv_kernel<T, DB, DVB, NWB, PART, 2>, 16 * NWB, 64 * NWB);
+      if constexpr (QG == 1 || sizeof(T) == 2) return run(dkv_kernel<T, DB, DVB, NWB, PART, 1>, 32 * NWB, 64 * NWB);
+      return GEOTR_OK;
     };
     if constexpr (kSplitKV<T, DVB>) {
       if (const int r = keys_of(std::integral_constant<int, kKeysOnly>{})) return r;

@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   }
   if (a.lse && lane < 2) {
     const int kvh = head / a.g;
-    a.lse[stat_at(a, kvh, lane, row, head - kvh * a.g)] = some ? (lane ? m[1] + log2f(l[1]) : m[0] + log2f(l[0])) : INFINITY;
+    store_sums(a, stat_at(a, kvh, lane, row, head - kvh * a.g), lane ? m[1] : m[0], lane ? l[1] : l[0], some);
   }
 }
 
@@ -116,8 +116,10 @@ __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
     const int kvh = head / a.g;
     const int64_t at = stat_at(a, kvh, 0, row, head - kvh * a.g);
     const int64_t to = row_stat_at(a, kvh, 0, row, head - kvh * a.g), step = a.nq * a.g;
-    const float lam = a.lam[head], e2 = a.lse[at + step];
-    a.rows[to] = a.lse[at], a.rows[to + step] = lam == 0.f ? INFINITY : e2 - log2f(fabsf(lam));
+    const float lam = a.lam[head], e2 = a.lse[at + step], r2 = a.lse[at + 3 * step], log = log2f(fabsf(lam));
+    const bool far = fabsf(e2) > kHuge && e2 < INFINITY;
+    a.rows[to] = a.lse[at], a.rows[to + step] = lam == 0.f ? INFINITY : far ? e2 : e2 - log;
+    a.rows[to + 5 * step] = a.lse[at + 2 * step], a.rows[to + 6 * step] = far && lam != 0.f ? r2 - log : 0.f;
     a.rows[to + 2 * step] = x, a.rows[to + 3 * step] = z, a.rows[to + 4 * step] = lam < 0.f ? -1.f : 1.f;
   }
   if constexpr (Narrow<T>::value) {
@@ -268,7 +270,7 @@ size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op) {
   Args a;
   if (make_args(op, a) != GEOTR_OK) return 0;
   const size_t rows = (size_t)a.nq * a.hk * a.g;
-  return align_up(5 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(sizeof(float));
+  return align_up(7 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(sizeof(float));
 }
 
 int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const float* maps, const float* lse,
@@ -285,7 +287,7 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
   const size_t rows = (size_t)a.nq * a.hk * a.g, need = geotr_diff_attn_backward_workspace_bytes(op);
   if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   Carver c(ws);
-  a.rows = c.take<float>(5 * rows), a.drow = c.take<float>(rows);
+  a.rows = c.take<float>(7 * rows), a.drow = c.take<float>(rows);
   float* amax = c.take<float>(1);
   a.dout = *dout, a.maps = const_cast<float*>(maps), a.lse = const_cast<float*>(lse);
   a.gq = dq, a.gk = dk, a.gv = dv, a.amax = amax;

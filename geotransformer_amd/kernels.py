@@ -926,7 +926,7 @@ def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None,
     maps = lse = None
     if want_state:
         maps = torch.empty(out.shape[:-1] + (2, v.shape[-1]), dtype=torch.float32, device=device)
-        lse = torch.empty((kv_heads, 2) + q.shape[:-2] + (heads // kv_heads,), dtype=torch.float32, device=device)
+        lse = torch.empty((kv_heads, 4) + q.shape[:-2] + (heads // kv_heads,), dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_workspace_bytes(op)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call(device, lib.geotr_diff_attn_forward, 'geotr_diff_attn_forward', op, out.data_ptr(), maps if maps is None else maps.data_ptr(),

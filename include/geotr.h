@@ -646,7 +646,7 @@ int geotr_rotary(const geotr_heads* q, const geotr_heads* q_out, const geotr_hea
  * rows that exist.  key_masks: bytes (batch, m) or (m), contiguous, nonzero = ignored.  causal: query i sees keys j <= i + (keys - queries) of its sequence.
  * Results of rows without a key, beyond their length or behind the last sequence are zero; what such key rows hold is never used.
  * out: contiguous (rows, H, v_dim).  For the gradients, both or none: maps (rows, H, 2, v_dim) fp32, the output of each map before lam, and
- * lse (Hk, 2, rows, H / Hk) fp32, the logarithm (base 2) of its sum. */
+ * lse (Hk, 4, rows, H / Hk) fp32, the logarithms (base 2) of their sums in two parts. */
 typedef struct geotr_diff_attn {
   geotr_heads q, k, v;
   int32_t dtype, stacked, causal, pad_;

@@ -1,7 +1,8 @@
 """Plain 64-bit forms of the rotary positions and the differential attention, with the bounds their kernels have to keep.
 
 Bounds are worst cases of the roundings, u = half a step of the type: every P and dS is rounded once to the type before its product, every
-result once; what is held in 32 bits is off by rho relative to the sum of absolute values, rho = 2 (d + 4) 2^-24 max|s||q||k| (a score
+result once, and for the gradients the outputs of the maps are summed from P in two parts of the type (u^2 is left) and kept in 32
+bits; what is held in 32 bits is off by rho relative to the sum of absolute values, rho = 2 (d + 4) 2^-24 max|s||q||k| (a score
 enters a weight and its sum) + (keys + 16) 2^-23 (sums, exponentials)."""
 import math
 
@@ -85,11 +86,9 @@ def differential_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_mas
             gs = tiny * float(gf.abs().max()) if tiny else 0.0  # fp16: dS is scaled to the largest gradient before it is rounded
             dp = g @ val.t()
             e_dp = (dv + 2) * 2.0 ** -24 * (g.abs() @ val.abs().t())
-            e_o2 = e2 + u * (o2.abs() + e2) + tiny
+            x1, x2 = ((u * u + rho) * (p @ val.abs()) + tiny * val.abs().sum(0) + U[torch.float32] * o.abs() for p, o in zip(P, (o1, o2)))
             d1, d2 = (g * o1).sum(1, keepdim=True), (g * o2).sum(1, keepdim=True)
-            more = (dv + 4) * 2.0 ** -24 * (g.abs() * (out.abs() + 2 * o2.abs())).sum(1, keepdim=True)
-            e_d2 = (g.abs() * e_o2).sum(1, keepdim=True) + more
-            e_d1 = (g.abs() * (far['out'][qs, h] + lam[h].abs() * e_o2)).sum(1, keepdim=True) + more
+            e_d1, e_d2 = ((g.abs() * (x + (dv + 4) * 2.0 ** -24 * o.abs())).sum(1, keepdim=True) for x, o in ((x1, o1), (x2, o2)))
             weights = P[0] - lam[h] * P[1]
             absw = P[0] + lam[h].abs() * P[1]
             x1, x2 = P[0] * (dp - d1), -lam[h] * P[1] * (dp - d2)
