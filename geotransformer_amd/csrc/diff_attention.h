@@ -3,9 +3,8 @@
 //
 //   out_h = sum_j (P1_ij - lam_h P2_ij) v_j,   Pa_ij = softmax_j(s q_a,i . k_a,j),   heads 2h and 2h + 1 of q and k are the two maps.
 //
-// One pass over the keys with a running maximum and sum for each map and two accumulators (O1 and O2 share every fragment of V):
-//   4 D + 4 Dv products per (row, key).  Joining the weights first would need the sums before the pass: one V product less, but every
-//   score and exponential twice.
+// One pass over the keys with a running maximum and sum for each map and an accumulator for each map: 4 D + 4 Dv operations per (row, key).
+//   Joining the weights first would need the sums before the pass: one V product less, but every score and exponential twice.
 // Backward, from lse_a = log2 of the sums and del_a = dO . O_a (attention output of map a):
 //   dP = dO V^T;  dS1 = P1 (dP - del1);  dS2 = -lam P2 (dP - del2);  dQa = s dSa Ka;  dKa = s dSa^T Qa;  dV = (P1 - lam P2)^T dO;
 //   dlam = - sum_ij P2 dP.  Two kernels, one that owns query rows (dQ, dlam) and one that owns keys (dK, dV): the scores are computed
@@ -88,7 +87,7 @@ template <>
 struct Narrow<_Float16> {
   static constexpr bool value = true;
 };
-// waves that a SIMD unit holds at a time, by the registers of the accumulators
+// waves that a SIMD unit holds at a time, by the registers of the accumulators (rows: one map to a wave, half of them)
 template <typename T, int DB, int DVB>
 constexpr int kWaves = sizeof(T) * DB <= 128 ? 2 : 1;
 template <typename T, int DB, int DVB>
@@ -470,7 +469,9 @@ __device__ __forceinline__ void zero_rows(const Args& a, const Seq& s, int kvh, 
 
 // Many rows: the waves are two maps x G groups of 32 packed rows; a wave owns 32 rows of ONE map, so it needs half the accumulators (three
 // waves to a SIMD unit at d = 64, v 128, where both maps in a wave leave one) and the maps meet in LDS at the end.  Tiles of 32 keys in two
-// buffers: the next one loads while this one is consumed.
+// buffers: the next one loads while this one is consumed.  Bound: matrix and vector instructions of a SIMD unit issue one after the other
+// (12 products of 32 cycles and 58 vector instructions for 32 x 32 weights at 64, 128).  8 192 causal rows, 16 heads, 64, 128, bf16: 433 us,
+// 0.95 PFLOP/s of the four products where a large library product of this card reaches 1.2; 32 bits, 2 048 rows: 112 of 138 TFLOP/s.
 // The accumulators are rescaled only when a row's maximum grew by more than 2^8: weights stay below 2^8, sums are exact either way.
 // FEW (a token over a cache, wide heads): the G groups share 32 rows and take 32 keys each of every tile, joined at the end.
 // EXACT (16-bit, for training): what rounding P to 16 bits takes away goes through a second product, because the gradients subtract
@@ -735,6 +736,9 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
 
 // Few rows (a token over a cache): the NW waves own the same 32 packed rows, both maps, and every wave streams key tiles of its own (no
 // barrier), joined at the end; with a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next launch.
+// Bound: HBM.  8 tokens over caches of up to 32 768 keys, 16 heads on 4, 64, 128, bf16: 83 us, 4.9 of the 5.1 TB/s of a large copy, and 6 us
+// for the join (with the two maps' waves sharing tiles behind barriers, 103); one row of 257 keys in 32 bits: 18 us, three tiles of
+// products one after the other on each SIMD unit of one compute unit.
 template <typename T, int DB, int DVB, int NW>
 __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
@@ -955,7 +959,8 @@ __device__ __forceinline__ float grad_scale(const Args& a) {
 }
 
 // A wave owns 32 packed rows.  Where two tiles of 64 keys fit into LDS the four waves are two groups of rows x two of the keys, joined at the
-// end: blocks of 64 rows fill the chip at half the rows, and the longest causal block ends after half the steps.
+// end: blocks of 64 rows fill the chip at half the rows, and the longest causal block ends after half the steps (2 x 4 096 causal rows, 8
+// heads, 64, 128: 175 -> 157 us; 128, 256 at 2 x 2 048 and 4 heads: 187 -> 116).  Bound: latency of two waves to a SIMD unit, 0.65 PFLOP/s.
 template <typename T, int DB, int DVB>
 constexpr int kKeyGroups = 128 * (2 * DB + DVB) * (int)sizeof(T) <= 131072 ? 2 : 1;
 template <typename T, int DB, int DVB, int NW>
@@ -1166,10 +1171,11 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
 }
 
 // ---- backward: keys (dK, dV) --------------------------------------------------------------------------------------------------------------
-// A wave owns 32 keys; K and V are the B operands (lane = key).  They stay in registers as far as two waves to a SIMD unit allow, V else in
-// LDS; 32-bit wide heads read them again from memory for every tile of 32 packed query rows (a product takes 16 times as long as the load).
-// Where both gradients' accumulators leave no registers (16-bit heads of 128, values of 256) dK and dV are two launches, the scores twice:
-// 20 instead of 16 products of d, 334 instead of 462 us at 2 x 2 048 rows and 4 heads.  Narrower heads lose by it (64, 128: 370 against
+// A wave owns 32 keys; K and V are the B operands (lane = key).  16-bit K and V stay in registers, V of wide heads in LDS; in 32 bits they are
+// read again from memory for every tile of 32 packed query rows (a product takes 16 times as long as the load; held: 136 against 129 us at
+// 32 clouds of 295, spilled).  Bound: latency of one wave to a SIMD unit, 0.5 PFLOP/s at 2 x 4 096 causal rows, 8 heads, 64, 128 (270 us);
+// two waves spill (989 us).  Where both gradients' accumulators leave no registers (16-bit heads of 128, values of 256) dK and dV are two launches, the scores twice:
+// 20 instead of 16 products of d, 334 instead of 462 us at 2 x 2 048 rows and 4 heads (260 by now).  Narrower heads lose by it (64, 128: 370 against
 // 274 us at 2 x 4 096 causal rows and 8 heads).
 enum Part { kBoth, kKeysOnly, kValuesOnly };
 template <typename T, int DVB>

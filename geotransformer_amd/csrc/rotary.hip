@@ -7,7 +7,9 @@
 //
 // Bound: HBM, every element read once and written once (the trigonometry is one sine and cosine per (token, pair), shared by all heads
 // of the query and of the key, which one launch covers).  A thread owns one 16-byte chunk position of a token (two chunks in the half
-// layout), computes the E (half) or E / 2 (interleaved) angles once and walks the heads with four of them in flight.
+// layout), computes the E (half) or E / 2 (interleaved) angles once and walks the heads with four of them in flight.  32 768 tokens of 40
+// heads of 128, bf16: 157 us, 4.3 of the 5.1 TB/s of a large copy; 9 583 points of 16 heads of 32, 32 bits: 8.8 us (4.5 TB/s); one token: 6 us,
+// the launch.
 #include <algorithm>
 
 #include "common.h"

@@ -832,7 +832,7 @@ def check_rotary_heads(q, k):
 def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0, inverse=False, checked=False):
     """(q, k) with the first rotary_dim channels of every head turned by their token's position (geotr_rotary); k may be None.
     positions: (rows,) / (batch, rows) or with a last dimension of axes; turns (rotary_dim / 2) float64 or its bits as int64: turns per
-    unit of position; axis (rotary_dim / 2) int32: the axis of each pair.  inverse: the transposed rotation (the gradient)."""
+    unit of position; axis (rotary_dim / 2) int32: the axis of each pair, below the number of them.  inverse: the transposed rotation (the gradient)."""
     if not checked:
         check_rotary_heads(q, k)
     if rotary_dim % 2 or not 2 <= rotary_dim <= q.shape[-1]:
