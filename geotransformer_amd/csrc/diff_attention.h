@@ -39,7 +39,7 @@ struct Args {
   float* maps;                           // (rows, heads, 2, dv): the maps' outputs, for the backward pass
   float *lse, *part, *drow;              // (hk, 4, nq, g): see store_sums; split partials; (hk, nq, g)
   float* rows;                           // backward, (hk, 7, nq, g): lse1, lse2 - log2 |lam|, del1, del2, sign of lam, rest of lse1, of lse2
-  const float* amax;                     // 16-bit floats of narrow range: largest |dout| (backward), else null
+  const float* amax;                     // 16-bit floats of narrow range: largest |dout| and |v| (backward)
   const float* lam;
   const int64_t *q_len, *k_len;
   const uint8_t* masks;                  // (nk) 1 = ignored key
@@ -947,13 +947,13 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
 }
 
 // ---- backward: query rows (dQ, sum of P2 dP) --------------------------------------------------------------------------------------------
-// fp16: the power of two that brings the largest |dout| to [2, 4), so that dS neither underflows for the small gradients of a mean loss
-// nor overflows (|dP| < 4 Dv max|v|); 1 for the types with the exponent range of 32 bits
+// fp16: the power of two that brings |dP - del| <= 2 Dv max|dout| max|v| below 2^15, so that dS neither overflows nor underflows for the small
+// gradients of a mean loss; 1 for the types with the exponent range of 32 bits
 template <typename T>
 __device__ __forceinline__ float grad_scale(const Args& a) {
   if constexpr (Narrow<T>::value) {
-    const float m = *a.amax;
-    if (m > 0.f && m < INFINITY) return ldexpf(1.f, 1 - ilogbf(m));
+    const float top = 2.f * a.dv * a.amax[0] * a.amax[1];
+    if (top > 0.f && top < INFINITY) return ldexpf(1.f, 14 - ilogbf(top));
   }
   return 1.f;
 }
@@ -1225,8 +1225,14 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
   if (key_base >= keys_here) return;
   const int key = key_base + 32 * kg + col;
   const bool in = key < s.m && !(a.masks && a.masks[s.k0 + key]);
-  const float gs = grad_scale<T>(a);
-  constexpr float kBoost = Narrow<T>::value ? 256.f : 1.f;  // fp16: P 2^8 in the product with dout, the weights of a long row stay normal numbers
+  float gs = grad_scale<T>(a), boost = 1.f;
+  bool minus = false;
+  if constexpr (Narrow<T>::value) {  // fp16: P 2^8 in the product with dout, the weights of a long row stay normal numbers; less where |lam| > 2^6
+    float most = 1.f;
+    for (int h = 0; h < a.g; ++h) most = fmaxf(most, fabsf(a.lam[kvh * a.g + h]));
+    const int power = ilogbf(most) + (most > 1.f);
+    gs = ldexpf(gs, -power), boost = ldexpf(1.f, min(8, 14 - power));
+  }
 
   const auto rk = buffer((const T*)a.k.data + s.b * a.k.batch_stride + ((a.stacked ? s.k0 : 0) + key_base) * a.k.row_stride +
                          (int64_t)kvh * 2 * a.k.head_stride);
@@ -1280,7 +1286,6 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
   if (a.causal) first = (min(s.n, max(0, key_base - off)) << a.gsh) / 32 * 32;  // rows before see none of these keys
   // key j is seen by query i iff j <= i + off, by packed row r iff (j - off) << gsh <= r
   const int from = a.causal ? min(key - off, s.n) * (1 << a.gsh) : 0, last = a.causal ? min(key_base + TILE - 1 - off, s.n) * (1 << a.gsh) : 0;
-  bool minus = false;
   for (int h = 0; h < a.g; ++h) minus |= a.lam[kvh * a.g + h] < 0.f;
 
   const T* const qp = (const T*)a.q.data + s.b * a.q.batch_stride + (a.stacked ? s.q0 : 0) * a.q.row_stride + (int64_t)kvh * 2 * a.g * a.q.head_stride;
@@ -1393,7 +1398,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
         const float p1 = s1[i], p2 = s2[i], g = dp[i];
         if constexpr (DK) s1[i] = p1 * (g - d1[e]), s2[i] = p2 * (d2[e] - g);
         if constexpr (DV) dp[i] = p1 - p2;
-        if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs, dp[i] *= kBoost;
+        if constexpr (Narrow<T>::value) s1[i] *= gs, s2[i] *= gs, dp[i] *= boost;
       }
     }
 #pragma unroll
@@ -1460,7 +1465,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
     all();
   }
   if (key >= keys_here) return;
-  const float fk = a.scale / gs, fv = 1.f / kBoost;
+  const float fk = a.scale / gs, fv = 1.f / boost;
   const int64_t at = s.k0 + key;
   T* const pk = dk + (at * a.hk + kvh) * 2 * a.d;
   T* const pv = dv + (at * a.hk + kvh) * a.dv;

@@ -140,6 +140,32 @@ __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
   }
 }
 
+// fp16: the largest |v| of the keys that exist and are not masked
+__global__ __launch_bounds__(256) void v_max_kernel(Args a, float* amax) {
+  const int lane = threadIdx.x & 63, per = a.hk * (a.dv / 8);
+  int64_t end = a.nk;
+  if (a.stacked) {
+    int64_t sum = 0;
+    for (int b = lane; b < a.batch; b += 64) sum += clamp_len(a.k_len[b], a.nk);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    end = min(end, sum);
+  }
+  float top = 0.f;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < end * per; e += (int64_t)gridDim.x * 256) {
+    const int64_t row = e / per, b = a.stacked ? 0 : row / a.m, i = a.stacked ? row : row - b * a.m;
+    if ((a.masks && a.masks[row]) || (!a.stacked && a.k_len && i >= a.k_len[b])) continue;
+    const int rest = (int)(e - row * per), head = rest / (a.dv / 8);
+    const auto x = *(const typename Ops<_Float16>::Frag*)((const _Float16*)a.v.data + b * a.v.batch_stride + i * a.v.row_stride +
+                                                          head * a.v.head_stride + 8 * (rest - head * (a.dv / 8)));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)x[j]));
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if (lane == 0 && top > 0.f) atomicMax((int*)amax, __float_as_int(top));
+}
+
 // dlam_h = - sum over rows, in a fixed order: 1 024 partial sums in 64 bits, then a tree
 __global__ __launch_bounds__(1024) void dlam_kernel(const float* drow, int64_t nq, int g, float* dlam) {
   __shared__ double box[1024];
@@ -270,7 +296,7 @@ size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op) {
   Args a;
   if (make_args(op, a) != GEOTR_OK) return 0;
   const size_t rows = (size_t)a.nq * a.hk * a.g;
-  return align_up(7 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(sizeof(float));
+  return align_up(7 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(2 * sizeof(float));
 }
 
 int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const float* maps, const float* lse,
@@ -288,12 +314,16 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
   if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   Carver c(ws);
   a.rows = c.take<float>(7 * rows), a.drow = c.take<float>(rows);
-  float* amax = c.take<float>(1);
+  float* amax = c.take<float>(2);
   a.dout = *dout, a.maps = const_cast<float*>(maps), a.lse = const_cast<float*>(lse);
   a.gq = dq, a.gk = dk, a.gv = dv, a.amax = amax;
   hipStream_t s = (hipStream_t)stream;
-  if (op->dtype == GEOTR_F16)
-    if (const int r = zero_async(amax, sizeof(float), s)) return r;
+  if (op->dtype == GEOTR_F16) {
+    if (const int r = zero_async(amax, 2 * sizeof(float), s)) return r;
+    const int64_t chunks = a.nk * a.hk * (a.dv / 8);
+    if (chunks) hipLaunchKernelGGL(v_max_kernel, dim3((unsigned)std::min<int64_t>(1024, (chunks + 255) / 256)), dim3(256), 0, s, a, amax + 1);
+    GEOTR_CHECK_LAUNCH("geotr_diff_attn_backward");
+  }
   if (a.nq) {
     const dim3 grid((unsigned)((rows + 15) / 16));
     if (op->dtype == GEOTR_F32) hipLaunchKernelGGL((del_kernel<float>), grid, dim3(256), 0, s, a, amax);

@@ -83,7 +83,10 @@ def differential_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_mas
             if gf is None:
                 continue
             g = gf[qs, h]
-            gs = tiny * float(gf.abs().max()) if tiny else 0.0  # fp16: dS is scaled to the largest gradient before it is rounded
+            # fp16: dS is scaled by a power of two that keeps 2 Dv max|dout| max|v| (times |lam| beyond 1) between 2^14 and 2^15, P by 2^8
+            # (less where |lam| > 2^6: 2^14 over the power of two above it) before they are rounded
+            power = 2.0 ** max(0, math.ceil(math.log2(max(1.0, float(lam.abs().max())))))
+            gs = tiny * 2.0 ** -14 * 2 * dv * float(gf.abs().max()) * float(vf[torch.isfinite(vf)].abs().max()) * power if tiny and m else 0.0
             dp = g @ val.t()
             e_dp = (dv + 2) * 2.0 ** -24 * (g.abs() @ val.abs().t())
             x1, x2 = ((u * u + rho) * (p @ val.abs()) + tiny * val.abs().sum(0) + U[torch.float32] * o.abs() for p, o in zip(P, (o1, o2)))
@@ -108,7 +111,7 @@ def differential_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_mas
             far['dk'][ks, 2 * c + 1] += (n + 2) * 2.0 ** -24 * scale * (x2.abs().t() @ qf[qs, 2 * h + 1].abs())
             res['dv'][ks, c] += weights.t() @ g
             # the difference of the two weights is rounded once, relative to itself; each weight is off by rho of its own
-            far['dv'][ks, c] += (u * weights.abs() + (rho * (1 + u) + (n + 2) * 2.0 ** -24) * absw).t() @ g.abs() + tiny * 2.0 ** -8 * g.abs().sum(0)
+            far['dv'][ks, c] += (u * weights.abs() + (rho * (1 + u) + (n + 2) * 2.0 ** -24) * absw).t() @ g.abs() + tiny * max(2.0 ** -8, power * 2.0 ** -14) * g.abs().sum(0)
             res['dlam'][h] -= (P[1] * dp).sum()
             far['dlam'][h] += (P[1] * (e_dp + (rho + 2.0 ** -22 * (m + 2)) * dp.abs())).sum() * (1 + rho)
     for name in ('dq', 'dk', 'dv'):

@@ -153,3 +153,69 @@ def test_nothing_around_the_results_changes():
     for n, shape in (('out', (33, 2, 72)), ('dq', q.shape), ('dk', k.shape), ('dv', v.shape)):
         oracle.assert_within(n, room[n][e:-e].view(shape), *want[n])
     del keep
+
+
+@pytest.mark.parametrize('heads,kv,d,dv', [(2, 1, 32, 64), (2, 2, 64, 128), (4, 1, 128, 256)])
+def test_large_values_and_lam_in_fp16(heads, kv, d, dv):
+    """Gradients of 16-bit floats of narrow range: values up to the type's largest, outputs' gradients large and small, lam beyond 2^6.
+    Results beyond the type's largest number are infinite, as their rounding is."""
+    from geotransformer_amd.modules.transformer import differential_attention
+    for size, grad, lam0, keys in ((10000.0, 1e-3, 1.0, 7), (10000.0, 1e-3, 1.0, 200), (1e-3, 1e-3, 1.0, 100), (1.0, 1.0, 300.0, 90), (1e-3, 1e4, -70.0, 40)):
+        q, k, v, lam, dout = _make('f16', (50,), (keys,), heads, kv, d, dv)
+        with torch.no_grad():
+            v *= size
+            dout *= grad
+            lam *= lam0
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+        y = differential_attention(*leaves)
+        want = oracle.differential_attention(q, k, v, lam, dout=dout)
+        for name, got in zip(('out', 'dq', 'dk', 'dv', 'dlam'), (y,) + torch.autograd.grad(y, leaves, dout)):
+            value, bound = want[name]
+            got = got.detach().cpu().double()
+            beyond = (value.abs() - bound >= 65520) if name != 'dlam' else torch.zeros_like(value, dtype=torch.bool)  # rounds to infinity
+            near = (value.abs() + bound < 65520) | (name == 'dlam')
+            assert torch.equal(got[beyond], torch.copysign(torch.full_like(value[beyond], float('inf')), value[beyond])), name
+            oracle.assert_within(name, got[near], value[near], bound[near])
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('heads,kv,d,dv', [(4, 2, 32, 64), (2, 2, 64, 128), (2, 1, 128, 256)])
+def test_clouds_of_very_different_sizes(dtype, heads, kv, d, dv):
+    """Few rows on average, one cloud with many; rows behind the last; keys of one cloud are most of all keys."""
+    ql, kl = [150] + [1] * 30, [3] * 30 + [1500]
+    q, k, v, lam, _ = _make(dtype, (sum(ql) + 4,), (sum(kl) + 9,), heads, kv, d, dv)
+    _check(q, k, v, lam, None, ql, kl, train=False)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+def test_nothing_at_all(dtype):
+    """No rows, no keys, no sequences: zeros of the right shapes."""
+    from geotransformer_amd.modules.transformer import differential_attention
+    for lead_q, lead_k in (((0,), (5,)), ((5,), (0,)), ((0,), (0,)), ((2, 0), (2, 5)), ((2, 5), (2, 0)), ((0, 4), (0, 5))):
+        leaves = [t.requires_grad_() for t in _make(dtype, lead_q, lead_k, 4, 2, 32, 64)]
+        dout = leaves.pop()
+        with torch.no_grad():
+            assert not differential_attention(*leaves).any()
+        y = differential_attention(*leaves)
+        assert y.shape == lead_q + (4, 64) and not y.any()
+        for g, t in zip(torch.autograd.grad(y, leaves, dout.detach()), leaves):
+            assert g.shape == t.shape and not g.any()
+
+
+def test_the_same_tensor_in_several_places():
+    """q, k and v as slices of one buffer, k as v, dout an expanded value: reads only, gradients add up."""
+    from geotransformer_amd.modules.transformer import differential_attention
+    x = torch.randn(60, 12, 64, device='cuda', generator=torch.Generator('cuda').manual_seed(2))
+    lam = torch.rand(2, device='cuda')
+    for q, k, v in ((x[:, :4], x[:, 4:8], x[:, 8:10]), (x[:, :4], x[:, :4], x[:, :2]), (x[:, 3:7], x[:, 4:8], x[:, 4:6])):
+        one = differential_attention(q, k, v, lam)
+        assert torch.equal(one, differential_attention(q.clone(), k.clone(), v.clone(), lam))
+        oracle.assert_within('out', one, *oracle.differential_attention(q, k, v, lam)['out'])
+    leaf = x.clone().requires_grad_()
+    whole, = torch.autograd.grad(differential_attention(leaf[:, :4], leaf[:, :4], leaf[:, :2], lam).sum(), leaf)
+    parts = [t.clone().requires_grad_() for t in (x[:, :4], x[:, :4], x[:, :2])]
+    a, b, c = torch.autograd.grad(differential_attention(*parts, lam), parts, torch.ones(60, 2, 64, device='cuda'))
+    want = torch.zeros_like(x)
+    want[:, :4] += a + b
+    want[:, :2] += c
+    assert float((whole - want).abs().max()) <= 4 * 2.0 ** -24 * float((a.abs() + b.abs()).max() + c.abs().max())
