@@ -858,35 +858,53 @@ def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0
     return q_out, k_out
 
 
-def _aligned(t):
-    """Channels contiguous, addresses and strides multiples of 16 bytes (what the tiles are loaded in): t itself, or a contiguous copy."""
-    e = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % e == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _aligned_heads(t, e):
+    """(t, words of geotr_heads) with channels contiguous, addresses and strides multiples of 16 bytes (e elements: what the tiles are loaded
+    in); a contiguous copy where t's are not."""
+    size, stride = t.shape, t.stride()
+    if len(size) == 4:
+        batch, rows, heads, _ = size
+        b, r, h, c = stride
+        if batch == 1:  # the stride of a dimension of one element says nothing
+            b = 0
+    else:
+        rows, heads, _ = size
+        r, h, c = stride
+        b = 0
+    if rows == 1:
+        r = 0
+    if heads == 1:
+        h = 0
+    address = t.data_ptr()
+    if c != 1 or address & 15 or (b | r | h) & (e - 1):
+        return _aligned_heads(t.clone(memory_format=torch.contiguous_format), e)
+    return t, (address, heads, b, r, h)
 
 
 def check_diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None, scale=None):
     """Refuses what geotr_diff_attn_* does not compute, with the reason."""
-    if q.dim() not in (3, 4) or k.dim() != q.dim() or v.dim() != q.dim():
+    qs, ks, vs = q.shape, k.shape, v.shape
+    dims, dtype = len(qs), q.dtype
+    if not 3 <= dims <= 4 or len(ks) != dims or len(vs) != dims:
         raise ValueError('q, k and v are (rows, heads, channels) in stack mode or (batch, rows, heads, channels): got '
-                         f'{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
-    if q.dtype not in HEAD_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f'q, k and v are float32, bfloat16 or float16, all of one type: got {q.dtype}, {k.dtype}, {v.dtype}')
-    heads, kv_heads = q.shape[-2] // 2, v.shape[-2]
-    if q.shape[-2] % 2 or k.shape[-2] != 2 * kv_heads or kv_heads < 1 or heads < 1 or heads % kv_heads or heads // kv_heads > 64:
-        raise ValueError(f'q has 2 H heads, k 2 Hk, v Hk, H a multiple of Hk (up to 64 times): got {q.shape[-2]}, {k.shape[-2]}, {kv_heads}')
-    if k.shape[:-2] != v.shape[:-2] or (q.dim() == 4 and q.shape[0] != k.shape[0]):
-        raise ValueError(f'rows of q {tuple(q.shape[:-2])}, k {tuple(k.shape[:-2])} and v {tuple(v.shape[:-2])} do not fit')
-    dim, v_dim = q.shape[-1], v.shape[-1]
-    if k.shape[-1] != dim or dim % 8 or not 8 <= dim <= 128 or v_dim % 8 or not 8 <= v_dim <= 256:
-        raise ValueError(f'channels of a head are multiples of 8, q and k alike up to 128, v up to 256: got {dim}, {k.shape[-1]}, {v_dim}')
+                         f'{tuple(qs)}, {tuple(ks)}, {tuple(vs)}')
+    if dtype not in HEAD_TYPES or k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f'q, k and v are float32, bfloat16 or float16, all of one type: got {dtype}, {k.dtype}, {v.dtype}')
+    q_heads, kv_heads, dim, v_dim = qs[-2], vs[-2], qs[-1], vs[-1]
+    heads = q_heads // 2
+    if q_heads % 2 or ks[-2] != 2 * kv_heads or kv_heads < 1 or heads < 1 or heads % kv_heads or heads // kv_heads > 64:
+        raise ValueError(f'q has 2 H heads, k 2 Hk, v Hk, H a multiple of Hk (up to 64 times): got {q_heads}, {ks[-2]}, {kv_heads}')
+    if ks[0] != vs[0] or (dims == 4 and (ks[1] != vs[1] or qs[0] != ks[0])):
+        raise ValueError(f'rows of q {tuple(qs[:-2])}, k {tuple(ks[:-2])} and v {tuple(vs[:-2])} do not fit')
+    if ks[-1] != dim or dim % 8 or not 8 <= dim <= 128 or v_dim % 8 or not 8 <= v_dim <= 256:
+        raise ValueError(f'channels of a head are multiples of 8, q and k alike up to 128, v up to 256: got {dim}, {ks[-1]}, {v_dim}')
     if lam.dtype != torch.float32 or lam.dim() > 1 or lam.numel() not in (1, heads):
         raise ValueError(f'lam is a float32 tensor of 1 or {heads} values: got {lam.dtype} {tuple(lam.shape)}')
     if scale is not None and not 0.0 < float(scale) < 1e30:
         raise ValueError(f'scale is a positive number, not {scale}')
-    if q.dim() == 3 and (q_lengths is None) != (k_lengths is None):
+    if dims == 3 and (q_lengths is None) != (k_lengths is None):
         raise ValueError('stack mode takes both lengths (or none: one sequence)')
-    sequences = q.shape[0] if q.dim() == 4 else None
+    sequences = qs[0] if dims == 4 else None
     for name, t in (('q_lengths', q_lengths), ('k_lengths', k_lengths)):
         if t is None:
             continue
@@ -895,23 +913,33 @@ def check_diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks
         sequences = t.shape[0] if sequences is None else sequences
         if t.shape[0] != sequences:
             raise ValueError(f'{name} of {t.shape[0]} sequences, expected {sequences}')
-    if key_masks is not None and (key_masks.dtype != torch.bool or key_masks.shape != k.shape[:-2]):
-        raise ValueError(f'key_masks are truth values of the rows of k {tuple(k.shape[:-2])}, True = ignored: got {key_masks.dtype} '
+    if key_masks is not None and (key_masks.dtype != torch.bool or key_masks.shape != ks[:-2]):
+        raise ValueError(f'key_masks are truth values of the rows of k {tuple(ks[:-2])}, True = ignored: got {key_masks.dtype} '
                          f'{tuple(key_masks.shape)}')
 
 
 def _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale):
     """(descriptor, what it points into) of a call."""
     device = _same_device(q, k, v, lam, q_lengths, k_lengths, key_masks)
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    if lam.dim() == 0 or lam.shape[0] * 2 != q.shape[-2] or lam.stride(0) != 1:
-        lam = lam.expand(q.shape[-2] // 2).contiguous()
-    q_lengths, k_lengths, key_masks = (t if t is None else t.contiguous() for t in (q_lengths, k_lengths, key_masks))
-    stacked = q.dim() == 3 and q_lengths is not None
-    batch = q_lengths.shape[0] if stacked else 1 if q.dim() == 3 else q.shape[0]
-    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
-    op = _DIFF_ATTN.pack(*_heads(q), *_heads(k), *_heads(v), HEAD_TYPES[q.dtype], stacked, bool(causal), 0, batch, q.shape[-3], k.shape[-3], q.shape[-1],
-                         v.shape[-1], lam.data_ptr(), *(0 if t is None else t.data_ptr() for t in (q_lengths, k_lengths, key_masks)), scale, 0)
+    qs, dtype = q.shape, q.dtype
+    e = 4 if dtype == torch.float32 else 8
+    (q, q_view), (k, k_view), (v, v_view) = _aligned_heads(q, e), _aligned_heads(k, e), _aligned_heads(v, e)
+    if lam.dim() == 0 or lam.shape[0] * 2 != qs[-2] or lam.stride(0) != 1:
+        lam = lam.expand(qs[-2] // 2).contiguous()
+    ql = kl = masks = 0
+    if q_lengths is not None:
+        q_lengths = q_lengths.contiguous()
+        ql = q_lengths.data_ptr()
+    if k_lengths is not None:
+        k_lengths = k_lengths.contiguous()
+        kl = k_lengths.data_ptr()
+    if key_masks is not None:
+        key_masks = key_masks.contiguous()
+        masks = key_masks.data_ptr()
+    stacked = len(qs) == 3 and q_lengths is not None
+    batch = q_lengths.shape[0] if stacked else 1 if len(qs) == 3 else qs[0]
+    op = _DIFF_ATTN.pack(*q_view, *k_view, *v_view, HEAD_TYPES[dtype], stacked, bool(causal), 0, batch, qs[-3], k.shape[-3], qs[-1], v.shape[-1],
+                         lam.data_ptr(), ql, kl, masks, 1.0 / math.sqrt(qs[-1]) if scale is None else scale, 0)
     return op, (q, k, v, lam, q_lengths, k_lengths, key_masks), device
 
 
@@ -921,12 +949,12 @@ def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None,
     if not checked:
         check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
-    lib, heads, kv_heads = _lib.load(), q.shape[-2] // 2, v.shape[-2]
-    out = q.new_empty(q.shape[:-2] + (heads, v.shape[-1]))
+    lib, lead, heads, kv_heads, v_dim = _lib.load(), q.shape[:-2], q.shape[-2] // 2, v.shape[-2], v.shape[-1]
+    out = q.new_empty((*lead, heads, v_dim))
     maps = lse = None
     if want_state:
-        maps = torch.empty(out.shape[:-1] + (2, v.shape[-1]), dtype=torch.float32, device=device)
-        lse = torch.empty((kv_heads, 4) + q.shape[:-2] + (heads // kv_heads,), dtype=torch.float32, device=device)
+        maps = torch.empty((*lead, heads, 2, v_dim), dtype=torch.float32, device=device)
+        lse = torch.empty((kv_heads, 4, *lead, heads // kv_heads), dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_workspace_bytes(op)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call(device, lib.geotr_diff_attn_forward, 'geotr_diff_attn_forward', op, out.data_ptr(), maps if maps is None else maps.data_ptr(),
@@ -945,12 +973,12 @@ def diff_attention_backward(dout, q, k, v, lam, state, q_lengths=None, k_lengths
         raise ValueError(f'the state of another call: outputs of the maps {tuple(state[0].shape)}')
     _same_device(q, dout, *state)
     lib = _lib.load()
-    dout = _aligned(dout)
+    dout, dout_view = _aligned_heads(dout, 4 if dout.dtype == torch.float32 else 8)
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     dlam = torch.empty(q.shape[-2] // 2, dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_backward_workspace_bytes(op)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _call(device, lib.geotr_diff_attn_backward, 'geotr_diff_attn_backward', op, _HEADS.pack(*_heads(dout)), state[0].data_ptr(),
+    _call(device, lib.geotr_diff_attn_backward, 'geotr_diff_attn_backward', op, _HEADS.pack(*dout_view), state[0].data_ptr(),
           state[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), need)
     del keep
     return dq, dk, dv, dlam
