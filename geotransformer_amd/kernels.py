@@ -835,26 +835,26 @@ def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0
     unit of position; axis (rotary_dim / 2) int32: the axis of each pair, below the number of them.  inverse: the transposed rotation (the gradient)."""
     if not checked:
         check_rotary_heads(q, k)
-    if rotary_dim % 2 or not 2 <= rotary_dim <= q.shape[-1]:
-        raise ValueError(f'rotary_dim {rotary_dim} of a head of {q.shape[-1]} channels: an even number up to it')
+    qs, place = q.shape, positions.stride()
+    if rotary_dim % 2 or not 2 <= rotary_dim <= qs[-1]:
+        raise ValueError(f'rotary_dim {rotary_dim} of a head of {qs[-1]} channels: an even number up to it')
     if positions.dtype not in POSITION_TYPES:
         raise TypeError(f'positions are int32, int64, float32 or float64, not {positions.dtype}')
-    lead = q.shape[:-2]
-    pos = positions.unsqueeze(-1) if positions.dim() == len(lead) else positions
-    if pos.dim() != len(lead) + 1 or tuple(pos.shape[:-1]) != tuple(lead):
-        raise ValueError(f'positions of rows {tuple(lead)}: got {tuple(positions.shape)}')
+    lead = len(qs) - 2
+    if not lead <= len(place) <= lead + 1 or positions.shape[:lead] != qs[:lead]:
+        raise ValueError(f'positions of rows {tuple(qs[:lead])}: got {tuple(positions.shape)}')
     assert turns.dtype in (torch.float64, torch.int64) and axis.dtype == torch.int32 and turns.numel() == axis.numel() == rotary_dim // 2
     device = _same_device(q, k, positions, turns, axis)
     q = q if q.stride(-1) == 1 else q.contiguous()
-    k = k if k is None or k.stride(-1) == 1 else k.contiguous()
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
-    pack = _HEADS.pack
-    batch, rows = (1, lead[0]) if len(lead) == 1 else lead
-    _call(device, _lib.load().geotr_rotary, 'geotr_rotary', pack(*_heads(q)), pack(*_heads(q_out)), None if k is None else pack(*_heads(k)),
-          None if k is None else pack(*_heads(k_out)), HEAD_TYPES[q.dtype], batch, rows, q.shape[-1], rotary_dim, int(interleaved), pos.data_ptr(),
-          POSITION_TYPES[pos.dtype], pos.stride(0) if len(lead) == 2 else 0, pos.stride(-2), pos.stride(-1), turns.data_ptr(), axis.data_ptr(), gain,
-          int(inverse))
+    pack, k_out, k_view, k_out_view = _HEADS.pack, None, None, None
+    if k is not None:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_view, k_out_view = pack(*_heads(k)), pack(*_heads(k_out))
+    _call(device, _lib.load().geotr_rotary, 'geotr_rotary', pack(*_heads(q)), pack(*_heads(q_out)), k_view, k_out_view, HEAD_TYPES[q.dtype],
+          1 if lead == 1 else qs[0], qs[lead - 1], qs[-1], rotary_dim, int(interleaved), positions.data_ptr(), POSITION_TYPES[positions.dtype],
+          place[0] if lead == 2 else 0, place[lead - 1], place[lead] if len(place) > lead else 0, turns.data_ptr(), axis.data_ptr(), gain, int(inverse))
     return q_out, k_out
 
 

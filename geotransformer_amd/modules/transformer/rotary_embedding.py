@@ -87,12 +87,11 @@ class RotaryPositionalEmbedding(nn.Module):
 
     def forward(self, q, k, positions):
         kernels.check_rotary_heads(q, k)
+        lead = q.dim() - 2
         if q.shape[-1] != self.head_dim:
             raise ValueError(f'heads of {q.shape[-1]} channels, built for {self.head_dim}')
-        lead = q.shape[:-2]
-        axes = positions.shape[-1] if positions.dim() == len(lead) + 1 else 1
-        if axes != self.num_axes:
-            raise ValueError(f'positions {tuple(positions.shape)} of rows {tuple(lead)}, built for {self.num_axes} axes')
+        if (positions.shape[-1] if positions.dim() == lead + 1 else 1) != self.num_axes:
+            raise ValueError(f'positions {tuple(positions.shape)} of rows {tuple(q.shape[:lead])}, built for {self.num_axes} axes')
         if positions.requires_grad:
             raise NotImplementedError('rotary positions are not differentiable in the positions: pass positions.detach()')
         how, turns = (self.rotary_dim, self.interleaved, self.gain), self.turn_bits
