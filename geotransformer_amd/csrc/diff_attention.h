@@ -734,11 +734,10 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
     }
 }
 
-// Few rows (a token over a cache): the NW waves own the same 32 packed rows, both maps, and every wave streams key tiles of its own (no
+// Few rows (a token over a cache; in 32 bits five rows and more): the NW waves own the same 32 packed rows, both maps, and every wave streams key tiles of its own (no
 // barrier), joined at the end; with a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next launch.
 // Bound: HBM.  8 tokens over caches of up to 32 768 keys, 16 heads on 4, 64, 128, bf16: 83 us, 4.9 of the 5.1 TB/s of a large copy, and 6 us
-// for the join (with the two maps' waves sharing tiles behind barriers, 103); one row of 257 keys in 32 bits: 18 us, three tiles of
-// products one after the other on each SIMD unit of one compute unit.
+// for the join (with the two maps' waves sharing tiles behind barriers, 103).
 template <typename T, int DB, int DVB, int NW>
 __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
@@ -944,6 +943,176 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
         store4<T>(po + c, y[0], y[1], y[2], y[3]);
       }
     }
+}
+
+// A row or a few of them in 32 bits: a matrix product of 32 rows takes as long for one (6 144 cycles for 32 keys at 32, 64), so these are
+// vector instructions.  A wave load is whole rows of K, 16 bytes a lane, LK lanes to the two maps of a key, KPL keys; sums of q . k over the
+// lanes of a map by DPP; the same lanes then take VE channels of the key's row of V.  Every key slot of a wave keeps a softmax of its own (no
+// exchange between slots, nothing in LDS), joined at the end.  Bound: latency at one row of 257 keys (6.0 us; the tiles below took 18.3), HBM on
+// long caches: 4 tokens over 8 192 keys, 4 heads, 64, 128: 24 us, 5.6 TB/s from the caches (52 by tiles); 128, 256: 49 us (155).
+// dpp: lanes of a row of 16; swap: the pair (rows or halves of the first map, of the second), each in both places
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+// the values of the first and the second map's lanes of a key, LK lanes to a key
+template <int LK>
+__device__ __forceinline__ void both(float x, bool second, float& one, float& two) {
+  if constexpr (LK == 16) {
+    const float o = dpp<0x128>(x);  // row_ror:8
+    one = second ? o : x, two = second ? x : o;
+  } else {
+    const auto w = LK == 32 ? __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)
+                            : __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    one = __uint_as_float(w[0]), two = __uint_as_float(w[1]);
+  }
+}
+template <int DB, int DVB, int R>
+__global__ __launch_bounds__(512) void fwd_rows_kernel(Args a) {
+  constexpr int NW = 8, U = 8, LK = DB / 2, KPL = 64 / LK, VE = DVB / LK, BN = U * KPL, W = 2 * DVB + 4;
+  static_assert((VE == 2 || VE == 4) && R <= NW, "values of a lane, a row to a wave at the end");
+  __shared__ __attribute__((aligned(16))) float box[NW][R][W];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slot = lane / LK, in_slot = lane % LK, map = in_slot / (LK / 2), chunk = in_slot % (LK / 2);
+  const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
+  const Seq s = find_seq<R, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
+  if (s.tile < 0) {
+    zero_rows<float>(a, s, kvh, NW * 64);
+    return;
+  }
+  const int row_base = s.tile * R, i0 = row_base >> a.gsh, off = s.m - s.n;
+  if (i0 >= (a.stacked ? s.n : a.n)) return;
+  const auto rq = buffer((const float*)a.q.data + s.b * a.q.batch_stride + ((a.stacked ? s.q0 : 0) + i0) * a.q.row_stride +
+                         (int64_t)kvh * 2 * a.g * a.q.head_stride);
+  f32x4 q[R];
+  float m[R], l[R], acc1[R][VE], acc2[R][VE];
+  int limit[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const Row row = row_of(a, s, row_base + r);
+    q[r] = load_frag<float>(rq, row.in && 4 * chunk < a.d ? (int)(((row.i - i0) * a.q.row_stride + (2 * row.h + map) * a.q.head_stride + 4 * chunk) * 4) : kOutside);
+    limit[r] = a.causal ? row.i + off : 0x7fffffff;
+    m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc1[r][e] = acc2[r][e] = 0.f;
+  }
+  const float* const kp = (const float*)a.k.data + s.b * a.k.batch_stride + (a.stacked ? s.k0 : 0) * a.k.row_stride + (int64_t)kvh * 2 * a.k.head_stride;
+  const float* const vp = (const float*)a.v.data + s.b * a.v.batch_stride + (a.stacked ? s.k0 : 0) * a.v.row_stride + (int64_t)kvh * a.v.head_stride;
+  int begin = 0, end = s.m;
+  if (a.causal) end = min(end, max(0, min((row_base + R - 1) >> a.gsh, s.n - 1) + off + 1));  // no key beyond the last row's limit
+  if (a.splits > 1) split_keys(a, begin, end);
+  const int krs = (int)(a.k.row_stride * 4), vrs = (int)(a.v.row_stride * 4);
+  const int ko = 4 * chunk < a.d ? (int)(map * a.k.head_stride + 4 * chunk) * 4 : kOutside, vo = VE * in_slot < a.dv ? VE * in_slot * 4 : kOutside;
+  using Vec = __attribute__((ext_vector_type(VE))) float;
+  for (int key0 = begin + wave * BN; key0 < end; key0 += NW * BN) {
+    const uint64_t bits = key_bits(a, s, key0, end, lane) >> slot;
+    const auto rk = buffer(kp + (int64_t)key0 * a.k.row_stride), rv = buffer(vp + (int64_t)key0 * a.v.row_stride);
+    f32x4 k[U];
+    Vec v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) k[u] = load_frag<float>(rk, (bits >> (u * KPL)) & 1 && ko != kOutside ? (u * KPL + slot) * krs + ko : kOutside);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int o = (bits >> (u * KPL)) & 1 && vo != kOutside ? (u * KPL + slot) * vrs + vo : kOutside;
+      if constexpr (VE == 4) v[u] = load_frag<float>(rv, o);
+      else v[u] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, 0));
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float x[U], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float t = q[r][0] * k[u][0];
+#pragma unroll
+        for (int e = 1; e < 4; ++e) t = fmaf(q[r][e], k[u][e], t);
+        t += dpp<0xB1>(t);   // quad_perm [1,0,3,2]
+        t += dpp<0x4E>(t);   // quad_perm [2,3,0,1]
+        t += dpp<0x141>(t);  // row_half_mirror: the sum of 8 lanes
+        if constexpr (LK >= 32) t += dpp<0x140>(t);  // row_mirror: of 16
+        if constexpr (LK == 64) {
+          const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+          t = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+        }
+        const bool seen = (bits >> (u * KPL)) & 1 && key0 + u * KPL + slot <= limit[r];
+        x[u] = seen ? t * a.scale_log2 : -INFINITY, top = fmaxf(top, x[u]);
+      }
+      const float n = fmaxf(m[r], top), from = n == -INFINITY ? 0.f : n, c = __builtin_amdgcn_exp2f(m[r] - from);
+      float c1, c2;
+      both<LK>(c, map, c1, c2);
+      m[r] = n, l[r] *= c;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc1[r][e] *= c1, acc2[r][e] *= c2;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float p = __builtin_amdgcn_exp2f(x[u] - from);
+        float p1, p2;
+        both<LK>(p, map, p1, p2);
+        l[r] += p;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc1[r][e] = fmaf(p1, v[u][e], acc1[r][e]), acc2[r][e] = fmaf(p2, v[u][e], acc2[r][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int o = LK; o < 64; o *= 2) {  // the wave's key slots
+      const float om = __shfl_xor(m[r], o, 64), n = fmaxf(m[r], om), from = n == -INFINITY ? 0.f : n;
+      const float c = __builtin_amdgcn_exp2f(m[r] - from), d = __builtin_amdgcn_exp2f(om - from);
+      float c1, c2, d1, d2;
+      both<LK>(c, map, c1, c2), both<LK>(d, map, d1, d2);
+      m[r] = n, l[r] = l[r] * c + __shfl_xor(l[r], o, 64) * d;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        acc1[r][e] = acc1[r][e] * c1 + __shfl_xor(acc1[r][e], o, 64) * d1;
+        acc2[r][e] = acc2[r][e] * c2 + __shfl_xor(acc2[r][e], o, 64) * d2;
+      }
+    }
+    if (lane < LK) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) box[wave][r][VE * in_slot + e] = acc1[r][e], box[wave][r][DVB + VE * in_slot + e] = acc2[r][e];
+      if (chunk == 0) box[wave][r][2 * DVB + map] = m[r], box[wave][r][2 * DVB + 2 + map] = l[r];
+    }
+  }
+  __syncthreads();
+  if (wave >= R) return;
+  const Row row = row_of(a, s, row_base + wave);
+  const int c = 4 * lane;
+  if (!row.out) return;
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, y[2][4] = {};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top[x] = fmaxf(top[x], box[w][wave][2 * DVB + x]);
+    const float from = top[x] == -INFINITY ? 0.f : top[x];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(box[w][wave][2 * DVB + x] - from);
+      sum[x] = fmaf(box[w][wave][2 * DVB + 2 + x], f, sum[x]);
+      if (c < DVB) {
+        const f32x4 t = *(const f32x4*)&box[w][wave][x * DVB + c];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[x][e] = fmaf(t[e], f, y[x][e]);
+      }
+    }
+    if (!row.in) top[x] = -INFINITY, sum[x] = 0.f;
+  }
+  const int64_t at = s.q0 + row.i;
+  const int head = kvh * a.g + row.h;
+  if (a.splits > 1) {  // unnormalised, with its maximum and sum: (split, row, head, 2, 4 + dv)
+    float* const p = a.part + (((int64_t)blockIdx.z * a.nq + at) * a.hk * a.g + head) * 2 * (a.dv + 4);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (lane == 0) p[x * (a.dv + 4)] = top[x], p[x * (a.dv + 4) + 1] = sum[x];
+      if (c < a.dv) store4<float>(p + x * (a.dv + 4) + 4 + c, y[x][0], y[x][1], y[x][2], y[x][3]);
+    }
+    return;
+  }
+  const float lam = a.lam[head], f1 = 1.f / sum[0], f2 = 1.f / sum[1];
+  const bool some = sum[0] != 0.f;  // false: no key, zero rows; a NaN stays one
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[0][e] = some ? fmaf(-lam, y[1][e] * f2, y[0][e] * f1) : 0.f;
+  if (c < a.dv) store4<float>((float*)a.out + (at * a.hk * a.g + head) * a.dv + c, y[0][0], y[0][1], y[0][2], y[0][3]);
 }
 
 // ---- backward: query rows (dQ, sum of P2 dP) --------------------------------------------------------------------------------------------
@@ -1542,6 +1711,11 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
     } else {
       return keys_of(std::integral_constant<int, kBoth>{});
     }
+  }
+  if constexpr (sizeof(T) == 4) {
+    const int64_t rows = (a.stacked ? (a.nq + a.batch - 1) / std::max(a.batch, 1) : a.n) << a.gsh;
+    if (which == kForwardKeys && rows <= 4 && tiles_of(a, false, rows == 1 ? 1 : 4) <= 65535)
+      return rows == 1 ? run(fwd_rows_kernel<DB, DVB, 1>, 1, 512) : run(fwd_rows_kernel<DB, DVB, 4>, 4, 512);
   }
   if (keys) {
     if constexpr (kNarrow) return run(fwd_keys_kernel<T, DB, DVB, 4>, 32, 256);

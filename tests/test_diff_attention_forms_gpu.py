@@ -219,3 +219,27 @@ def test_the_same_tensor_in_several_places():
     want[:, :4] += a + b
     want[:, :2] += c
     assert float((whole - want).abs().max()) <= 4 * 2.0 ** -24 * float((a.abs() + b.abs()).max() + c.abs().max())
+
+
+@pytest.mark.parametrize('d,dv', [(8, 8), (32, 32), (24, 56), (64, 64), (40, 120), (128, 128), (128, 256)])
+@pytest.mark.parametrize('heads,kv', [(2, 2), (3, 1), (4, 1)])
+def test_one_to_four_rows_in_fp32(d, dv, heads, kv):
+    """Rows by vector instructions: one to four packed rows, ends inside a step of a wave, keys dealt over blocks, a causal last row, masks."""
+    for n, m, causal in ((1, 1, False), (1, 7, True), (1, 257, False), (2, 64, True), (1, 2600, False), (4 if kv == 2 else 1, 1029, True)):
+        q, k, v, lam, _ = _make('f32', (2, n), (2, m), heads, kv, d, dv)
+        _check(q, k, v, lam, None, None, [m, m // 2], causal=causal, train=False)
+        masks = torch.rand(2, m, generator=torch.Generator('cuda').manual_seed(m), device='cuda') < 0.6
+        with torch.no_grad():
+            clean = (k.clone(), v.clone())
+            k[masks], v[masks] = float('nan'), float('inf')
+        from geotransformer_amd.modules.transformer import differential_attention
+        got = differential_attention(q, k, v, lam, key_masks=masks, causal=causal)
+        oracle.assert_within('out', got, *oracle.differential_attention(q, *clean, lam, key_masks=masks, causal=causal)['out'])
+    ql, kl = [1, 0, 3, 1, 9] + [1] * 80, [300, 5, 0, 41, 64] + [3] * 80
+    q, k, v, lam, _ = _make('f32', (sum(ql) + 2,), (sum(kl) + 2,), heads, kv, d, dv)
+    _check(q, k, v, lam, None, ql, kl, train=False)
+    with torch.no_grad():
+        q, k = torch.full_like(q[:1], 200.0), torch.full_like(k[:70], -200.0)  # scores beyond 2^20, all the same: the mean of v
+        mean = v[:70].double().mean(0).repeat_interleave(heads // kv, 0)
+        got = differential_attention(q, k, v[:70], lam, scale=1.0)[0].double()
+    assert float((got - (1 - lam.double())[:, None] * mean).abs().max()) <= 2 * 90 * 2.0 ** -23 * float(v[:70].abs().max())
