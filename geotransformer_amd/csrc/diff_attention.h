@@ -7,8 +7,8 @@
 //   Joining the weights first would need the sums before the pass: one V product less, but every score and exponential twice.
 // Backward, from lse_a = log2 of the sums and del_a = dO . O_a (attention output of map a):
 //   dP = dO V^T;  dS1 = P1 (dP - del1);  dS2 = -lam P2 (dP - del2);  dQa = s dSa Ka;  dKa = s dSa^T Qa;  dV = (P1 - lam P2)^T dO;
-//   dlam = - sum_ij P2 dP.  Two kernels, one that owns query rows (dQ, dlam) and one that owns keys (dK, dV): the scores are computed
-//   twice, and no sum depends on the order of atomics.
+//   dlam = - sum_ij P2 dP.  Blocks that own query rows (dQ, dlam) and blocks that own keys (dK, dV): the scores are computed twice, and no sum
+//   depends on the order of atomics.
 //
 // Layout of the matrix work (32 x 32 MFMA, a wave = 32 rows of one kind): scores are computed TRANSPOSED to how they are consumed, so the
 // accumulator a lane holds (16 of 32 contraction indices of ONE row) is the B operand of the next product as it stands: no exchange
@@ -196,14 +196,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p) {
 }
 // 16 bytes per lane from byte offset + scalar into 1 024 bytes of LDS.  Issued by asm (it writes no register): the compiler takes a
 // transposed LDS read for one that may depend on every such load in flight and would wait for the next tile before this one's products
-// (causal 8 192: 489 us with the builtin).  The loops wait themselves (tile_ready).
+// (causal 8 192: 489 us with the builtin).  The loops wait themselves (tile_ready).  The descriptor may come from v_readfirstlane, whose result a
+// buffer load may read after five wait states; the compiler does not look into the asm for that.
 using i32x4 = __attribute__((ext_vector_type(4))) int;
 __device__ __forceinline__ i32x4 words(const void* p) {
   const uint64_t u = (uint64_t)p;
   return i32x4{__builtin_amdgcn_readfirstlane((int)u), __builtin_amdgcn_readfirstlane((int)(u >> 32)) & 0xffff, kNumRecords, 0x00020000};
 }
 __device__ __forceinline__ void load_lds(i32x4 d, unsigned lds, int offset, int scalar = 0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(d), "s"(scalar)
                : "memory");
@@ -225,7 +226,8 @@ __device__ __forceinline__ void arrived(V& x) {
   asm volatile("" : "+v"(x));
 }
 // x lies in accumulation registers here: without it the compiler takes the same ones for the scores, 64 moves a tile (dK/dV 327 -> 276 us at
-// 2 x 4 096 causal rows and 8 heads; 128/128 at 2 x 2 048 and 4: 222 -> 129)
+// 2 x 4 096 causal rows and 8 heads; 128/128 at 2 x 2 048 and 4: 222 -> 129).  Not for dQ of 32-bit heads of 128, whose 432 registers of
+// fragments and accumulators are spilled: there the compiler loses the first map's accumulators over this.
 __device__ __forceinline__ void held(f32x16& x) { asm volatile("" : "+a"(x)); }
 template <typename T>
 __device__ __forceinline__ typename Ops<T>::Frag load_frag(__amdgpu_buffer_rsrc_t r, int offset) {
@@ -1133,18 +1135,24 @@ __device__ __forceinline__ float grad_scale(const Args& a) {
 template <typename T, int DB, int DVB>
 constexpr int kKeyGroups = 128 * (2 * DB + DVB) * (int)sizeof(T) <= 131072 ? 2 : 1;
 template <typename T, int DB, int DVB, int NW>
-__global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args a) {
+constexpr int kSmemQ() {
+  constexpr int KG = kKeyGroups<T, DB, DVB>, kTile = 32 * KG * (2 * DB + DVB) * (int)sizeof(T), NB = 2 * kTile <= 131072 ? 2 : 1;
+  constexpr int kJoin = KG == 1 ? 0 : NW / KG * (2 * DB / 32 * 16 + 1) * 64 * 4;
+  return NB * kTile > kJoin ? NB * kTile : kJoin;
+}
+// block `y` of `blocks` of a head
+template <typename T, int DB, int DVB, int NW>
+__device__ __forceinline__ void dq_block(const Args& a, char* smem, int y, int blocks) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CK = 2 * DB * (int)sizeof(T) / 16, CV = DVB * (int)sizeof(T) / 16, ND = DB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
   constexpr int KG = kKeyGroups<T, DB, DVB>, RG = NW / KG, BN = 32 * KG, TILE = 32 * RG;
-  constexpr int kTile = BN * (CK + CV) * 16, NB = 2 * kTile <= 131072 ? 2 : 1, kJoin = KG == 1 ? 0 : RG * (2 * ND * 16 + 1) * 64 * 4;
+  constexpr int kTile = BN * (CK + CV) * 16, NB = 2 * kTile <= 131072 ? 2 : 1;
   constexpr uint64_t kAll = BN == 64 ? ~0ull : 0xffffffffull;
-  __shared__ __attribute__((aligned(1024))) char smem[NB * kTile > kJoin ? NB * kTile : kJoin];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
   const int rg = wave % RG, kg = wave / RG;
-  const int t = tile_order(a, blockIdx.y, gridDim.y, gridDim.x, 256 * kWaves<T, DB, DVB>);
-  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
+  const int t = tile_order(a, y, blocks, gridDim.x, 256 * kWaves<T, DB, DVB>);
+  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, blocks);
   T* const dq = (T*)a.gq;
   if (s.tile < 0) {
     const int64_t rows = s.q_end < a.nq ? a.nq - s.q_end : 0, per = (int64_t)a.g * 2 * a.d;
@@ -1234,7 +1242,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       Ops<T>::mma(s1, krow.get(tile, 0, i), q1[i]);
       Ops<T>::mma(s2, krow.get(tile, 0, CK / 4 + i), q2[i]);
     }
-    if constexpr (kWaves<T, DB, DVB> == 1) {
+    if constexpr (kWaves<T, DB, DVB> == 1 && !(sizeof(T) == 4 && DB == 128)) {
 #pragma unroll
       for (int i = 0; i < ND; ++i) held(acc1[i]), held(acc2[i]);
     }
@@ -1338,6 +1346,11 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
       }
     }
 }
+template <typename T, int DB, int DVB, int NW>
+__global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) char smem[kSmemQ<T, DB, DVB, NW>()];
+  dq_block<T, DB, DVB, NW>(a, smem, blockIdx.y, gridDim.y);
+}
 
 // ---- backward: keys (dK, dV) --------------------------------------------------------------------------------------------------------------
 // A wave owns 32 keys; K and V are the B operands (lane = key).  16-bit K and V stay in registers, V of wide heads in LDS; in 32 bits they are
@@ -1361,20 +1374,25 @@ constexpr int kRowTile = 32 * (2 * DB + DVB) * (int)sizeof(T) + 1024;
 template <typename T, int DB, int DVB, int PART>
 constexpr int kRowGroups = 4 * kRowTile<T, DB, DVB> + (kLdsV<T, DB, PART> ? 64 * DVB * (int)sizeof(T) : 0) <= 160 * 1024 ? 2 : 1;
 template <typename T, int DB, int DVB, int NW, int PART, int QG>
-__global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_kernel(Args a) {
+constexpr int kSmemKV() {
+  constexpr int kBuf = QG * kRowTile<T, DB, DVB>, NB = 2 * kBuf <= 140000 ? 2 : 1, kV = kLdsV<T, DB, PART> ? 32 * NW / QG * DVB * (int)sizeof(T) : 0;
+  constexpr int kJoin = QG == 1 ? 0 : NW / QG * ((PART != kValuesOnly ? 2 * DB / 32 : 0) + (PART != kKeysOnly ? DVB / 32 : 0)) * 16 * 64 * 4;
+  return NB * kBuf + kV > kJoin ? NB * kBuf + kV : kJoin;
+}
+template <typename T, int DB, int DVB, int NW, int PART, int QG>
+__device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int blocks) {
   using Frag = typename Ops<T>::Frag;
   constexpr int CQ = 2 * DB * (int)sizeof(T) / 16, CO = DVB * (int)sizeof(T) / 16, ND = DB / 32, NV = DVB / 32, QS = DB / kStep<T>, VS = DVB / kStep<T>;
   constexpr bool kHold = sizeof(T) == 2, kInLds = kLdsV<T, DB, PART>, kHoldV = PART != kValuesOnly && kHold && !kInLds;
   constexpr bool DK = PART != kValuesOnly, DV = PART != kKeysOnly;
   constexpr int KG = NW / QG, TILE = 32 * KG, BN = 32 * QG;
   constexpr int kRowBytes = 32 * (CQ + CO) * 16, kTile = kRowTile<T, DB, DVB>, kBuf = QG * kTile;
-  constexpr int NB = 2 * kBuf <= 140000 ? 2 : 1, kV = kInLds ? TILE * CO * 16 : 0;
+  constexpr int NB = 2 * kBuf <= 140000 ? 2 : 1;
   constexpr int kJoin = QG == 1 ? 0 : KG * ((DK ? 2 * ND : 0) + (DV ? NV : 0)) * 16 * 64 * 4;
-  __shared__ __attribute__((aligned(1024))) char smem[NB * kBuf + kV > kJoin ? NB * kBuf + kV : kJoin];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int kg = wave % KG, qg = wave / KG;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const Seq s = find_seq<TILE, true>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
+  const Seq s = find_seq<TILE, true>(a, a.stacked ? 0 : blockIdx.x / a.hk, y, blocks);
   T* const dk = (T*)a.gk;
   T* const dv = (T*)a.gv;
   if (s.tile < 0) {
@@ -1482,7 +1500,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
     // rows that do not exist: zeros, and their products are zero because q and dout are
     for (int x = wave; x < 4; x += NW) {
       const i32x4 rs = words(sp + ((int64_t)(2 * x) * a.nq + i0) * a.g + h0);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
                    :
                    : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) && 2 * x + half < 7 ? so : kOutside), "s"(rs)
                    : "memory");
@@ -1661,9 +1679,23 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
     }
   }
 }
+template <typename T, int DB, int DVB, int NW, int PART, int QG>
+__global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) char smem[kSmemKV<T, DB, DVB, NW, PART, QG>()];
+  dkv_block<T, DB, DVB, NW, PART, QG>(a, smem, blockIdx.y, gridDim.y);
+}
+// Both in one launch where both take two waves to a SIMD unit, the first key_blocks of a head for the keys: the last blocks of one fill what the
+// other's leave empty (32 clouds of 295 in 32 bits, 32, 64: 215 -> 172 us; 2 x 2 048 rows, 4 heads, bf16: 81 -> 63).
+template <typename T, int DB, int DVB, int NW, int QG>
+__global__ __launch_bounds__(NW * 64, 2) void backward_kernel(Args a, int key_blocks) {
+  constexpr int kQ = kSmemQ<T, DB, DVB, NW>(), kKV = kSmemKV<T, DB, DVB, NW, kBoth, QG>();
+  __shared__ __attribute__((aligned(1024))) char smem[kQ > kKV ? kQ : kKV];
+  if ((int)blockIdx.y < key_blocks) dkv_block<T, DB, DVB, NW, kBoth, QG>(a, smem, blockIdx.y, key_blocks);
+  else dq_block<T, DB, DVB, NW>(a, smem, blockIdx.y - key_blocks, gridDim.y - key_blocks);
+}
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------------------
-enum Which { kForward, kForwardKeys, kBackwardQ, kBackwardKV };
+enum Which { kForward, kForwardKeys, kBackward };
 
 // stack mode: every sequence may end inside a tile, and one block more takes the rows behind the last
 inline int64_t tiles_of(const Args& a, bool keys, int tile) {
@@ -1677,39 +1709,49 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
   // few rows: narrow heads stream a tile per wave; wide ones share tiles of 64 keys, where two buffers of them fit
   constexpr bool kNarrow = (int)sizeof(T) * DB < 256, kFew = !kNarrow && 2 * kWide <= 160 * 1024;
   const bool keys = which == kForwardKeys && (kNarrow || kFew);
-  auto grid = [&](int tile) {
-    const int64_t tiles = tiles_of(a, which == kBackwardKV, tile), x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
-    return dim3((unsigned)std::min<int64_t>(x, 0x80000000ll), (unsigned)std::min<int64_t>(tiles, 65536),
-                which == kForward || which == kForwardKeys ? (unsigned)a.splits : 1u);
-  };
-  auto run = [&](auto kernel, int tile, int threads) -> int {
-    const dim3 d = grid(tile);
-    if (d.x == 0 || d.y == 0) return GEOTR_OK;
-    if (d.x > 0x7fffffffu || d.y > 65535u) return fail(GEOTR_E_INVALID, "differential attention: too many rows in one call (65 535 tiles of %d)", tile);
-    hipLaunchKernelGGL(kernel, d, dim3(threads), 0, s, a);
+  const int64_t x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
+  auto go = [&](auto kernel, int64_t blocks, int threads, auto... more) -> int {
+    if (x == 0 || blocks == 0) return GEOTR_OK;
+    if (x > 0x7fffffff || blocks > 65535) return fail(GEOTR_E_INVALID, "differential attention: too many rows in one call (65 535 tiles of a head)");
+    hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)blocks, which == kBackward ? 1u : (unsigned)a.splits), dim3(threads), 0, s, a, more...);
     GEOTR_CHECK_LAUNCH("differential attention");
     return GEOTR_OK;
   };
-  if (which == kBackwardQ) return run(dq_kernel<T, DB, DVB, NWB>, 32 * NWB / kKeyGroups<T, DB, DVB>, 64 * NWB);
-  if (which == kBackwardKV) {
+  auto run = [&](auto kernel, int tile, int threads) -> int { return go(kernel, tiles_of(a, false, tile), threads); };
+  if (which == kBackward) {
     // Two query groups halve a block's keys and its steps, but load every query row twice as often.  They win while all their blocks run at
     // once (2 x 2 048 rows and 4 heads, 128 against 64 blocks: 64/64 139 against 246 us, 128/128 220 against 308) and lose with more
     // (2 x 4 096 causal rows and 8 heads: 404 against 316).  32-bit products take 16 times as long as the loads: always (32 clouds of 295
     // rows: 119 against 128 us; 4 x 2 048 rows, 4 heads: 368 against 481).
     const int64_t tiles = a.stacked ? (a.nk / (32 * NWB) + a.batch / 2) : (int64_t)a.batch * ((a.m + 32 * NWB - 1) / (32 * NWB));
     const bool small = tiles * a.hk <= 128 * kWavesKV<T, DB, DVB, kBoth>;
-    auto keys_of = [&](auto part) -> int {
+    const int64_t rows = tiles_of(a, false, 32 * NWB / kKeyGroups<T, DB, DVB>);
+    auto keys_of = [&](auto part, auto use) -> int {  // use(query groups, blocks)
       constexpr int PART = decltype(part)::value, QG = kRowGroups<T, DB, DVB, PART>;
       if constexpr (QG == 2)
-        if (sizeof(T) == 4 || small) return run(dkv_kernel<T, DB, DVB, NWB, PART, 2>, 16 * NWB, 64 * NWB);
-      if constexpr (QG == 1 || sizeof(T) == 2) return run(dkv_kernel<T, DB, DVB, NWB, PART, 1>, 32 * NWB, 64 * NWB);
+        if (sizeof(T) == 4 || small) return use(std::integral_constant<int, 2>{}, tiles_of(a, true, 16 * NWB));
+      if constexpr (QG == 1 || sizeof(T) == 2) return use(std::integral_constant<int, 1>{}, tiles_of(a, true, 32 * NWB));
       return GEOTR_OK;
     };
-    if constexpr (kSplitKV<T, DVB>) {
-      if (const int r = keys_of(std::integral_constant<int, kKeysOnly>{})) return r;
-      return keys_of(std::integral_constant<int, kValuesOnly>{});
+    if constexpr (kWaves<T, DB, DVB> == 2 && kWavesKV<T, DB, DVB, kBoth> == 2) {
+      return keys_of(std::integral_constant<int, kBoth>{}, [&](auto qg, int64_t blocks) {
+        return go(backward_kernel<T, DB, DVB, NWB, decltype(qg)::value>, blocks + rows, 64 * NWB, (int)blocks);
+      });
     } else {
-      return keys_of(std::integral_constant<int, kBoth>{});
+      if (a.nq)
+        if (const int r = go(dq_kernel<T, DB, DVB, NWB>, rows, 64 * NWB)) return r;
+      if (a.nk == 0) return GEOTR_OK;
+      auto keys = [&](auto part) {
+        return keys_of(part, [&](auto qg, int64_t blocks) {
+          return go(dkv_kernel<T, DB, DVB, NWB, decltype(part)::value, decltype(qg)::value>, blocks, 64 * NWB);
+        });
+      };
+      if constexpr (kSplitKV<T, DVB>) {
+        if (const int r = keys(std::integral_constant<int, kKeysOnly>{})) return r;
+        return keys(std::integral_constant<int, kValuesOnly>{});
+      } else {
+        return keys(std::integral_constant<int, kBoth>{});
+      }
     }
   }
   if constexpr (sizeof(T) == 4) {

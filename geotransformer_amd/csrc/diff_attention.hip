@@ -330,10 +330,8 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
     else if (op->dtype == GEOTR_BF16) hipLaunchKernelGGL((del_kernel<__bf16>), grid, dim3(256), 0, s, a, amax);
     else hipLaunchKernelGGL((del_kernel<_Float16>), grid, dim3(256), 0, s, a, amax);
     GEOTR_CHECK_LAUNCH("geotr_diff_attn_backward");
-    if (const int r = launch(op->dtype, a, kBackwardQ, s)) return r;
   }
-  if (a.nk)
-    if (const int r = launch(op->dtype, a, kBackwardKV, s)) return r;
+  if (const int r = launch(op->dtype, a, kBackward, s)) return r;
   hipLaunchKernelGGL(dlam_kernel, dim3((unsigned)(a.hk * a.g)), dim3(1024), 0, s, a.drow, a.nq, a.g, dlam);
   GEOTR_CHECK_LAUNCH("geotr_diff_attn_backward");
   return GEOTR_OK;
