@@ -196,15 +196,17 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p) {
 }
 // 16 bytes per lane from byte offset + scalar into 1 024 bytes of LDS.  Issued by asm (it writes no register): the compiler takes a
 // transposed LDS read for one that may depend on every such load in flight and would wait for the next tile before this one's products
-// (causal 8 192: 489 us with the builtin).  The loops wait themselves (tile_ready).  The descriptor may come from v_readfirstlane, whose result a
-// buffer load may read after five wait states; the compiler does not look into the asm for that.
+// (causal 8 192: 489 us with the builtin).  The loops wait themselves (tile_ready).
 using i32x4 = __attribute__((ext_vector_type(4))) int;
 __device__ __forceinline__ i32x4 words(const void* p) {
   const uint64_t u = (uint64_t)p;
-  return i32x4{__builtin_amdgcn_readfirstlane((int)u), __builtin_amdgcn_readfirstlane((int)(u >> 32)) & 0xffff, kNumRecords, 0x00020000};
+  int lo = __builtin_amdgcn_readfirstlane((int)u), hi = __builtin_amdgcn_readfirstlane((int)(u >> 32)) & 0xffff;
+  // a buffer load may read what v_readfirstlane wrote after five wait states, and the compiler does not look into the asm for that
+  asm volatile("s_nop 4" : "+s"(lo), "+s"(hi));
+  return i32x4{lo, hi, kNumRecords, 0x00020000};
 }
 __device__ __forceinline__ void load_lds(i32x4 d, unsigned lds, int offset, int scalar = 0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(d), "s"(scalar)
                : "memory");
@@ -1500,7 +1502,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int 
     // rows that do not exist: zeros, and their products are zero because q and dout are
     for (int x = wave; x < 4; x += NW) {
       const i32x4 rs = words(sp + ((int64_t)(2 * x) * a.nq + i0) * a.g + h0);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                    :
                    : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) && 2 * x + half < 7 ? so : kOutside), "s"(rs)
                    : "memory");
