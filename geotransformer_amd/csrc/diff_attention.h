@@ -1737,7 +1737,10 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
     };
     if constexpr (kWaves<T, DB, DVB> == 2 && kWavesKV<T, DB, DVB, kBoth> == 2) {
       return keys_of(std::integral_constant<int, kBoth>{}, [&](auto qg, int64_t blocks) {
-        return go(backward_kernel<T, DB, DVB, NWB, decltype(qg)::value>, blocks + rows, 64 * NWB, (int)blocks);
+        const auto kernel = backward_kernel<T, DB, DVB, NWB, decltype(qg)::value>;
+        if (blocks + rows <= 65535) return go(kernel, blocks + rows, 64 * NWB, (int)blocks);
+        if (const int r = go(kernel, rows, 64 * NWB, 0)) return r;
+        return go(kernel, blocks, 64 * NWB, (int)blocks);
       });
     } else {
       if (a.nq)

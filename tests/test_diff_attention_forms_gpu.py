@@ -243,3 +243,21 @@ def test_one_to_four_rows_in_fp32(d, dv, heads, kv):
         mean = v[:70].double().mean(0).repeat_interleave(heads // kv, 0)
         got = differential_attention(q, k, v[:70], lam, scale=1.0)[0].double()
     assert float((got - (1 - lam.double())[:, None] * mean).abs().max()) <= 2 * 90 * 2.0 ** -23 * float(v[:70].abs().max())
+
+
+def test_more_blocks_of_both_gradients_than_one_grid():
+    """2.1 million rows and keys, all but 300 behind the last cloud: the gradients' blocks (64 rows each) take two launches."""
+    from geotransformer_amd.modules.transformer import differential_attention
+    clouds, rows = 33, 65024
+    q, k, v, lam, dout = _make('f32', (clouds * rows,), (clouds * rows,), 1, 1, 8, 8)
+    lens = torch.zeros(clouds, dtype=torch.int64, device='cuda')
+    lens[0] = 300  # the rest lies behind the last cloud
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    y = differential_attention(*leaves, q_lengths=lens, k_lengths=lens)
+    grads = torch.autograd.grad(y, leaves, dout)
+    small = [t[:300].detach().requires_grad_() for t in (q, k, v)] + [lam.detach().requires_grad_()]
+    want = oracle.differential_attention(*small, dout=dout[:300])
+    for name, got in zip(('out', 'dq', 'dk', 'dv'), (y,) + grads):
+        oracle.assert_within(name, got[:300], *want[name])
+        assert not got[300:].any()
+    oracle.assert_within('dlam', grads[3], *want['dlam'])
