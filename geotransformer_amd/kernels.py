@@ -8,6 +8,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -818,6 +819,13 @@ def _call(device, fn, name, *args):
             code = fn(*args, stream)
     if code:
         _lib.check(code, name)
+
+
+def refuse_tangents(name, *tensors):
+    """Refuses inputs of forward-mode differentiation (torch.autograd.forward_ad): they require no grad, and a kernel reads their values alone,
+    so that the result would silently have no tangent."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f'{name} has no forward-mode derivative: an input carries a tangent')
 
 
 def check_rotary_heads(q, k):

@@ -43,8 +43,9 @@ def differential_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_mas
     lam: float32 tensor, one value or one per head; key_masks: truth values of the key rows, True = ignored (what an ignored row, or one
     beyond its length, holds is never read into a result); causal: query i sees keys j <= i + keys - queries of its cloud; scale: default
     1 / sqrt(d).  Rows without any key, beyond their length or behind the last cloud give zeros.
-    Returns (rows, H, d_v) / (batch, rows, H, d_v).  Differentiable in q, k, v and lam (once); gradients do not depend on scheduling."""
+    Returns (rows, H, d_v) / (batch, rows, H, d_v).  Differentiable in q, k, v and lam (once, in reverse mode); gradients do not depend on scheduling."""
     kernels.check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
+    kernels.refuse_tangents('differential_attention', q, k, v, lam)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
         lam = lam.expand(q.shape[-2] // 2)  # the gradient of a shared value is the sum over its heads
         return _DifferentialAttention.apply(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)

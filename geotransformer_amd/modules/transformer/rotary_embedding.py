@@ -64,7 +64,7 @@ class _Rotary(torch.autograd.Function):
 class RotaryPositionalEmbedding(nn.Module):
     """q, k = rope(q, k, positions): q (rows, H, head_dim) or (batch, rows, H, head_dim), k likewise with its own number of heads (or None),
     float32, bfloat16 or float16; positions (rows,) / (batch, rows) integers or floats, for num_axes > 1 with a last dimension of num_axes.
-    Differentiable in q and k.  The angles are taken in 64 bits, the rotation in 32, and the result is rounded once.
+    Differentiable in q and k (in reverse mode).  The angles are taken in 64 bits, the rotation in 32, and the result is rounded once.
 
     rotary_dim: channels that are turned (the first ones; default: the largest multiple of 2 num_axes); interleaved: pairs (2i, 2i + 1)
     instead of (i, i + rotary_dim / 2).  Axis a turns the pairs a F .. (a + 1) F - 1, F = rotary_dim / (2 num_axes).
@@ -94,6 +94,7 @@ class RotaryPositionalEmbedding(nn.Module):
             raise ValueError(f'positions {tuple(positions.shape)} of rows {tuple(q.shape[:lead])}, built for {self.num_axes} axes')
         if positions.requires_grad:
             raise NotImplementedError('rotary positions are not differentiable in the positions: pass positions.detach()')
+        kernels.refuse_tangents('RotaryPositionalEmbedding', q, k, positions)
         how, turns = (self.rotary_dim, self.interleaved, self.gain), self.turn_bits
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             return _Rotary.apply(q, k, positions, turns, self.axis, how, False)

@@ -1,0 +1,40 @@
+"""CPU: calls of the rotary positions and the differential attention that are refused, or have to be answered, away from the common forms."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from geotransformer_amd import kernels
+from geotransformer_amd.modules.transformer import RotaryPositionalEmbedding, differential_attention
+
+
+def _heads(rows=5, keys=7, heads=4, kv=2, d=16, dv=32, lead=()):
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    return r(*lead, rows, 2 * heads, d), r(*lead, keys, 2 * kv, d), r(*lead, keys, kv, dv), torch.rand(heads, generator=g)
+
+
+@pytest.mark.parametrize('which', range(4))
+@pytest.mark.parametrize('grad', [False, True])
+def test_attention_refuses_tangents(monkeypatch, which, grad):
+    """A dual tensor requires no grad: without the refusal the kernel call returns a result that has silently no tangent."""
+    monkeypatch.setattr(kernels, 'diff_attention', lambda q, k, v, *a, **kw: q.new_zeros(5, 4, 32))
+    inputs = list(_heads())
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        assert differential_attention(*inputs).shape == (5, 4, 32)  # no tangent: an ordinary call
+        inputs[which] = forward_ad.make_dual(inputs[which], torch.ones_like(inputs[which]))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            differential_attention(*inputs)
+
+
+@pytest.mark.parametrize('which', range(3))
+@pytest.mark.parametrize('grad', [False, True])
+def test_rotary_refuses_tangents(monkeypatch, which, grad):
+    monkeypatch.setattr(kernels, 'rotary', lambda q, k, *a, **kw: (torch.zeros_like(q), k))
+    q, k, _, _ = _heads(keys=5)
+    inputs = [q, k, torch.arange(5, dtype=torch.float32)]
+    rope = RotaryPositionalEmbedding(16)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        assert rope(*inputs)[0].shape == q.shape
+        inputs[which] = forward_ad.make_dual(inputs[which], torch.ones_like(inputs[which]))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            rope(*inputs)
