@@ -38,7 +38,7 @@ struct Args {
   void *out, *gq, *gk, *gv;              // contiguous (rows, heads, channels)
   float* maps;                           // (rows, heads, 2, dv): the maps' outputs, for the backward pass
   float *lse, *part, *drow;              // (hk, 4, nq, g): see store_sums; split partials; (hk, nq, g)
-  float* rows;                           // backward, (hk, 7, nq, g): lse1, lse2 - log2 |lam|, del1, del2, sign of lam, rest of lse1, of lse2
+  float* rows;                           // backward, (hk, 4, nq, g, 2): lse1, lse2 - log2 |lam|; del1, del2; sign of lam, rest of lse1; of lse2, -
   const float* amax;                     // 16-bit floats of narrow range: largest |dout| and |v| (backward)
   const float* lam;
   const int64_t *q_len, *k_len;
@@ -409,8 +409,9 @@ __device__ __forceinline__ int64_t stat_at(const Args& a, int kvh, int map, int6
   return (((int64_t)kvh * 4 + map) * a.nq + row) * a.g + h;
 }
 
-__device__ __forceinline__ int64_t row_stat_at(const Args& a, int kvh, int which, int64_t row, int h) {
-  return (((int64_t)kvh * 7 + which) * a.nq + row) * a.g + h;
+// pairs of the numbers of a row lie side by side: what a wave reads of them stays near one address however many rows there are
+__device__ __forceinline__ int64_t row_stat_at(const Args& a, int kvh, int pair, int64_t row, int h) {
+  return ((((int64_t)kvh * 4 + pair) * a.nq + row) * a.g + h) * 2;
 }
 
 // What the backward pass takes weights from: log2 of the sum, m + log2 l.  Beyond 2^20 that would round log2 l away (weights off by 4 % at
@@ -1200,8 +1201,8 @@ __device__ __forceinline__ void dq_block(const Args& a, char* smem, int y, int b
   if (row.in) {
     const int64_t st = stat_at(a, kvh, 0, at, row.h);
     lse1 = a.lse[st], lse2 = a.lse[st + a.nq * a.g], rest1 = a.lse[st + 2 * a.nq * a.g], rest2 = a.lse[st + 3 * a.nq * a.g], lam = a.lam[head];
-    const int64_t rs = row_stat_at(a, kvh, 2, at, row.h);
-    del1 = a.rows[rs], del2 = a.rows[rs + a.nq * a.g];
+    const int64_t rs = row_stat_at(a, kvh, 1, at, row.h);
+    del1 = a.rows[rs], del2 = a.rows[rs + 1];
   }
   arrived(lse1), arrived(lse2), arrived(rest1), arrived(rest2), arrived(del1), arrived(del2), arrived(lam);
 #pragma unroll
@@ -1486,8 +1487,8 @@ __device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int 
   const int group = 1 << a.gsh, q16 = group <= 16 ? (16 >> a.gsh) * qrs : 32 * qhs, o16 = group <= 16 ? (16 >> a.gsh) * ors : 16 * ohs;
   const Stage<T, 32, 2, DB, NW> qst(a.d, qhs, wave, lane, [&](int x) { return (x >> a.gsh) * qrs + (x & (group - 1)) * 2 * qhs; });
   const Stage<T, 32, 1, DVB, NW> ost(a.dv, 0, wave, lane, [&](int x) { return (x >> a.gsh) * ors + (x & (group - 1)) * ohs; });
-  // numbers of the rows: a wave load takes two of the seven kinds, lane = kind and row
-  const int so = (int)((half * a.nq + (col >> a.gsh)) * a.g + (col & (group - 1))) * 4;
+  // numbers of the rows: a wave load takes a pair of the kinds, lane = kind and row
+  const int so = (((col >> a.gsh) * a.g + (col & (group - 1))) * 2 + half) * 4;
   auto fill32 = [&](unsigned tile, int r0) GEOTR_INLINE {
     const int i0 = r0 >> a.gsh, h0 = r0 & (group - 1);
     const i32x4 rq = words(qp + i0 * a.q.row_stride + 2 * h0 * a.q.head_stride), ro = words(op + i0 * a.dout.row_stride + h0 * a.dout.head_stride);
@@ -1501,10 +1502,10 @@ __device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int 
     }
     // rows that do not exist: zeros, and their products are zero because q and dout are
     for (int x = wave; x < 4; x += NW) {
-      const i32x4 rs = words(sp + ((int64_t)(2 * x) * a.nq + i0) * a.g + h0);
+      const i32x4 rs = words(sp + (((int64_t)x * a.nq + i0) * a.g + h0) * 2);
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                    :
-                   : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) && 2 * x + half < 7 ? so : kOutside), "s"(rs)
+                   : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) ? so : kOutside), "s"(rs)
                    : "memory");
     }
   };

@@ -82,61 +82,70 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
 }
 
 // What the backward pass reads of a row: the sums, del_a = dout . O_a in 32 bits (16 lanes per (row, head)), |lam| folded into the second
-// sum.  fp16: the largest |dout| of the rows that exist (an order-free maximum).  Bound: HBM.
+// sum.  fp16: the largest |dout| of the rows that exist (an order-free maximum).  Bound: HBM.  The blocks take the rows in turn: a grid holds
+// 2^32 threads, 16 of them to a (row, head).
 template <typename T>
 __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
   using Frag = typename Ops<T>::Frag;
   const int lane = threadIdx.x & 63, heads = a.hk * a.g, c0 = lane & 15;
-  const int64_t e = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
-  const bool in = e < a.nq * heads;
-  float x = 0.f, z = 0.f, top = 0.f;
-  const int64_t row = in ? e / heads : 0;
-  const int head = in ? (int)(e - row * heads) : 0;
-  if (in) {
+  const int64_t all = a.nq * heads;
+  float most = 0.f;
+  int64_t exist = a.nq;  // stack mode: rows behind the last sequence say nothing
+  if constexpr (Narrow<T>::value) {
+    if (a.stacked && a.q_len) {
+      exist = 0;
+      for (int b = lane; b < a.batch; b += 64) exist += clamp_len(a.q_len[b], a.nq);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) exist += __shfl_xor(exist, o, 64);
+    }
+  }
+  for (int64_t e0 = (int64_t)blockIdx.x * 16; e0 < all; e0 += (int64_t)gridDim.x * 16) {
+    const int64_t e = e0 + 4 * (threadIdx.x >> 6) + (lane >> 4);
+    const bool in = e < all;
+    float x = 0.f, z = 0.f, top = 0.f;
+    const int64_t row = in ? e / heads : 0;
+    const int head = in ? (int)(e - row * heads) : 0;
     const int64_t b = a.stacked ? 0 : row / a.n, i = a.stacked ? row : row - b * a.n;
-    const T* g = (const T*)a.dout.data + b * a.dout.batch_stride + i * a.dout.row_stride + head * a.dout.head_stride;
-    const float* y = a.maps + 2 * e * a.dv;
-    for (int c = c0 * kE<T>; c < a.dv; c += 16 * kE<T>) {
-      const Frag fg = *(const Frag*)(g + c);
+    if (in) {
+      const T* g = (const T*)a.dout.data + b * a.dout.batch_stride + i * a.dout.row_stride + head * a.dout.head_stride;
+      const float* y = a.maps + 2 * e * a.dv;
+      for (int c = c0 * kE<T>; c < a.dv; c += 16 * kE<T>) {
+        const Frag fg = *(const Frag*)(g + c);
 #pragma unroll
-      for (int j = 0; j < kE<T>; j += 4) {
-        const f32x4 y1 = *(const f32x4*)(y + c + j), y2 = *(const f32x4*)(y + a.dv + c + j);
+        for (int j = 0; j < kE<T>; j += 4) {
+          const f32x4 y1 = *(const f32x4*)(y + c + j), y2 = *(const f32x4*)(y + a.dv + c + j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = (float)fg[j + i];
-          x = fmaf(v, y1[i], x), z = fmaf(v, y2[i], z);
-          if constexpr (Narrow<T>::value) top = fmaxf(top, fabsf(v));
+          for (int i = 0; i < 4; ++i) {
+            const float v = (float)fg[j + i];
+            x = fmaf(v, y1[i], x), z = fmaf(v, y2[i], z);
+            if constexpr (Narrow<T>::value) top = fmaxf(top, fabsf(v));
+          }
         }
       }
     }
-  }
 #pragma unroll
-  for (int o = 8; o; o >>= 1) x += __shfl_xor(x, o, 64), z += __shfl_xor(z, o, 64);
-  if (in && c0 == 0) {
-    const int kvh = head / a.g;
-    const int64_t at = stat_at(a, kvh, 0, row, head - kvh * a.g);
-    const int64_t to = row_stat_at(a, kvh, 0, row, head - kvh * a.g), step = a.nq * a.g;
-    const float lam = a.lam[head], e2 = a.lse[at + step], r2 = a.lse[at + 3 * step], log = log2f(fabsf(lam));
-    const bool far = fabsf(e2) > kHuge && e2 < INFINITY;
-    a.rows[to] = a.lse[at], a.rows[to + step] = lam == 0.f ? INFINITY : far ? e2 : e2 - log;
-    a.rows[to + 5 * step] = a.lse[at + 2 * step], a.rows[to + 6 * step] = far && lam != 0.f ? r2 - log : 0.f;
-    a.rows[to + 2 * step] = x, a.rows[to + 3 * step] = z, a.rows[to + 4 * step] = lam < 0.f ? -1.f : 1.f;
+    for (int o = 8; o; o >>= 1) x += __shfl_xor(x, o, 64), z += __shfl_xor(z, o, 64);
+    if (in && c0 == 0) {
+      const int kvh = head / a.g;
+      const int64_t at = stat_at(a, kvh, 0, row, head - kvh * a.g);
+      const int64_t to = row_stat_at(a, kvh, 0, row, head - kvh * a.g), step = a.nq * a.g;
+      const float lam = a.lam[head], e2 = a.lse[at + step], r2 = a.lse[at + 3 * step], log = log2f(fabsf(lam));
+      const bool far = fabsf(e2) > kHuge && e2 < INFINITY;
+      float2* const p = (float2*)(a.rows + to);
+      p[0] = float2{a.lse[at], lam == 0.f ? INFINITY : far ? e2 : e2 - log};
+      p[step] = float2{x, z};
+      p[2 * step] = float2{lam < 0.f ? -1.f : 1.f, a.lse[at + 2 * step]};
+      p[3 * step] = float2{far && lam != 0.f ? r2 - log : 0.f, 0.f};
+    }
+    if constexpr (Narrow<T>::value) {  // gradients of rows that do not exist say nothing
+      if (a.stacked ? row >= exist : in && a.q_len && i >= a.q_len[b]) top = 0.f;
+      most = fmaxf(most, top);
+    }
   }
   if constexpr (Narrow<T>::value) {
-    if (a.q_len) {  // gradients of rows that do not exist say nothing
-      if (a.stacked) {
-        int64_t end = 0;
-        for (int b = lane; b < a.batch; b += 64) end += clamp_len(a.q_len[b], a.nq);
 #pragma unroll
-        for (int o = 32; o; o >>= 1) end += __shfl_xor(end, o, 64);
-        if (row >= end) top = 0.f;
-      } else if (in && row % a.n >= a.q_len[row / a.n]) {
-        top = 0.f;
-      }
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if (lane == 0 && top > 0.f) atomicMax((int*)amax, __float_as_int(top));
+    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    if (lane == 0 && most > 0.f) atomicMax((int*)amax, __float_as_int(most));
   }
 }
 
@@ -296,7 +305,7 @@ size_t geotr_diff_attn_backward_workspace_bytes(const geotr_diff_attn* op) {
   Args a;
   if (make_args(op, a) != GEOTR_OK) return 0;
   const size_t rows = (size_t)a.nq * a.hk * a.g;
-  return align_up(7 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(2 * sizeof(float));
+  return align_up(8 * rows * sizeof(float)) + align_up(rows * sizeof(float)) + align_up(2 * sizeof(float));
 }
 
 int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout, const float* maps, const float* lse,
@@ -313,7 +322,7 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
   const size_t rows = (size_t)a.nq * a.hk * a.g, need = geotr_diff_attn_backward_workspace_bytes(op);
   if (!ws || ws_bytes < need) return fail(GEOTR_E_WORKSPACE, "geotr_diff_attn_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   Carver c(ws);
-  a.rows = c.take<float>(7 * rows), a.drow = c.take<float>(rows);
+  a.rows = c.take<float>(8 * rows), a.drow = c.take<float>(rows);
   float* amax = c.take<float>(2);
   a.dout = *dout, a.maps = const_cast<float*>(maps), a.lse = const_cast<float*>(lse);
   a.gq = dq, a.gk = dk, a.gv = dv, a.amax = amax;
@@ -325,7 +334,7 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
     GEOTR_CHECK_LAUNCH("geotr_diff_attn_backward");
   }
   if (a.nq) {
-    const dim3 grid((unsigned)((rows + 15) / 16));
+    const dim3 grid((unsigned)std::min<size_t>(1 << 20, (rows + 15) / 16));
     if (op->dtype == GEOTR_F32) hipLaunchKernelGGL((del_kernel<float>), grid, dim3(256), 0, s, a, amax);
     else if (op->dtype == GEOTR_BF16) hipLaunchKernelGGL((del_kernel<__bf16>), grid, dim3(256), 0, s, a, amax);
     else hipLaunchKernelGGL((del_kernel<_Float16>), grid, dim3(256), 0, s, a, amax);
