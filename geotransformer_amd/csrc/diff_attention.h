@@ -46,6 +46,7 @@ struct Args {
   int64_t nq, nk;                        // all rows
   int batch, stacked, n, m;              // batch mode: n, m rows per sequence
   int hk, g, gsh, d, dv, causal, splits; // query heads to a key head; packed rows r = (i << gsh) + h, h < g <= 1 << gsh
+  int tiles, tile0, seq0;                // tiles of a head; a launch's first tile and (batch mode) first sequence: a grid may not hold them all
   float scale, scale_log2;
 };
 
@@ -492,8 +493,8 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int map = wave & 1, group = wave >> 1, rows_at = FEW ? 0 : 32 * group;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const int t = tile_order(a, blockIdx.y, gridDim.y, gridDim.x);
-  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, gridDim.y);
+  const int t = tile_order(a, a.tile0 + blockIdx.y, a.tiles, gridDim.x);
+  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : a.seq0 + blockIdx.x / a.hk, t, a.tiles);
   if (s.tile < 0) {
     zero_rows<T>(a, s, kvh, 128 * G);
     return;
@@ -752,7 +753,7 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel
   __shared__ __attribute__((aligned(1024))) char smem[kSmem];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
+  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : a.seq0 + blockIdx.x / a.hk, a.tile0 + blockIdx.y, a.tiles);
   T* const out = (T*)a.out;
   if (s.tile < 0) {
     zero_rows<T>(a, s, kvh, NW * 64);
@@ -980,7 +981,7 @@ __global__ __launch_bounds__(512) void fwd_rows_kernel(Args a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slot = lane / LK, in_slot = lane % LK, map = in_slot / (LK / 2), chunk = in_slot % (LK / 2);
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const Seq s = find_seq<R, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, blockIdx.y, gridDim.y);
+  const Seq s = find_seq<R, false>(a, a.stacked ? 0 : a.seq0 + blockIdx.x / a.hk, a.tile0 + blockIdx.y, a.tiles);
   if (s.tile < 0) {
     zero_rows<float>(a, s, kvh, NW * 64);
     return;
@@ -1155,7 +1156,7 @@ __device__ __forceinline__ void dq_block(const Args& a, char* smem, int y, int b
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
   const int rg = wave % RG, kg = wave / RG;
   const int t = tile_order(a, y, blocks, gridDim.x, 256 * kWaves<T, DB, DVB>);
-  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : blockIdx.x / a.hk, t, blocks);
+  const Seq s = find_seq<TILE, false>(a, a.stacked ? 0 : a.seq0 + blockIdx.x / a.hk, t, blocks);
   T* const dq = (T*)a.gq;
   if (s.tile < 0) {
     const int64_t rows = s.q_end < a.nq ? a.nq - s.q_end : 0, per = (int64_t)a.g * 2 * a.d;
@@ -1352,7 +1353,7 @@ __device__ __forceinline__ void dq_block(const Args& a, char* smem, int y, int b
 template <typename T, int DB, int DVB, int NW>
 __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) char smem[kSmemQ<T, DB, DVB, NW>()];
-  dq_block<T, DB, DVB, NW>(a, smem, blockIdx.y, gridDim.y);
+  dq_block<T, DB, DVB, NW>(a, smem, a.tile0 + blockIdx.y, a.tiles);
 }
 
 // ---- backward: keys (dK, dV) --------------------------------------------------------------------------------------------------------------
@@ -1395,7 +1396,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int kg = wave % KG, qg = wave / KG;
   const int kvh = a.stacked ? blockIdx.x : blockIdx.x % a.hk;
-  const Seq s = find_seq<TILE, true>(a, a.stacked ? 0 : blockIdx.x / a.hk, y, blocks);
+  const Seq s = find_seq<TILE, true>(a, a.stacked ? 0 : a.seq0 + blockIdx.x / a.hk, y, blocks);
   T* const dk = (T*)a.gk;
   T* const dv = (T*)a.gv;
   if (s.tile < 0) {
@@ -1685,7 +1686,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int 
 template <typename T, int DB, int DVB, int NW, int PART, int QG>
 __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) char smem[kSmemKV<T, DB, DVB, NW, PART, QG>()];
-  dkv_block<T, DB, DVB, NW, PART, QG>(a, smem, blockIdx.y, gridDim.y);
+  dkv_block<T, DB, DVB, NW, PART, QG>(a, smem, a.tile0 + blockIdx.y, a.tiles);
 }
 // Both in one launch where both take two waves to a SIMD unit, the first key_blocks of a head for the keys: the last blocks of one fill what the
 // other's leave empty (32 clouds of 295 in 32 bits, 32, 64: 215 -> 172 us; 2 x 2 048 rows, 4 heads, bf16: 81 -> 63).
@@ -1693,8 +1694,9 @@ template <typename T, int DB, int DVB, int NW, int QG>
 __global__ __launch_bounds__(NW * 64, 2) void backward_kernel(Args a, int key_blocks) {
   constexpr int kQ = kSmemQ<T, DB, DVB, NW>(), kKV = kSmemKV<T, DB, DVB, NW, kBoth, QG>();
   __shared__ __attribute__((aligned(1024))) char smem[kQ > kKV ? kQ : kKV];
-  if ((int)blockIdx.y < key_blocks) dkv_block<T, DB, DVB, NW, kBoth, QG>(a, smem, blockIdx.y, key_blocks);
-  else dq_block<T, DB, DVB, NW>(a, smem, blockIdx.y - key_blocks, gridDim.y - key_blocks);
+  const int y = a.tile0 + blockIdx.y;
+  if (y < key_blocks) dkv_block<T, DB, DVB, NW, kBoth, QG>(a, smem, y, key_blocks);
+  else dq_block<T, DB, DVB, NW>(a, smem, y - key_blocks, a.tiles - key_blocks);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------------------
@@ -1712,12 +1714,18 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
   // few rows: narrow heads stream a tile per wave; wide ones share tiles of 64 keys, where two buffers of them fit
   constexpr bool kNarrow = (int)sizeof(T) * DB < 256, kFew = !kNarrow && 2 * kWide <= 160 * 1024;
   const bool keys = which == kForwardKeys && (kNarrow || kFew);
-  const int64_t x = a.stacked ? a.hk : (int64_t)a.batch * a.hk;
+  // A grid holds 65 535 tiles of a head and 2^32 threads over the heads and sequences: what is more takes further launches
+  const int seqs = a.stacked ? 1 : a.batch, most_seqs = std::max(1, (1 << 22) / a.hk), most_tiles = 65535;
   auto go = [&](auto kernel, int64_t blocks, int threads, auto... more) -> int {
-    if (x == 0 || blocks == 0) return GEOTR_OK;
-    if (x > 0x7fffffff || blocks > 65535) return fail(GEOTR_E_INVALID, "differential attention: too many rows in one call (65 535 tiles of a head)");
-    hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)blocks, which == kBackward ? 1u : (unsigned)a.splits), dim3(threads), 0, s, a, more...);
-    GEOTR_CHECK_LAUNCH("differential attention");
+    for (int seq0 = 0; seq0 < seqs; seq0 += most_seqs)
+      for (int64_t tile0 = 0; tile0 < blocks; tile0 += most_tiles) {
+        Args part = a;
+        part.tiles = (int)blocks, part.tile0 = (int)tile0, part.seq0 = seq0;
+        const dim3 grid((unsigned)(std::min(most_seqs, seqs - seq0) * a.hk), (unsigned)std::min<int64_t>(most_tiles, blocks - tile0),
+                        which == kBackward ? 1u : (unsigned)a.splits);
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, part, more...);
+        GEOTR_CHECK_LAUNCH("differential attention");
+      }
     return GEOTR_OK;
   };
   auto run = [&](auto kernel, int tile, int threads) -> int { return go(kernel, tiles_of(a, false, tile), threads); };
@@ -1738,10 +1746,7 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
     };
     if constexpr (kWaves<T, DB, DVB> == 2 && kWavesKV<T, DB, DVB, kBoth> == 2) {
       return keys_of(std::integral_constant<int, kBoth>{}, [&](auto qg, int64_t blocks) {
-        const auto kernel = backward_kernel<T, DB, DVB, NWB, decltype(qg)::value>;
-        if (blocks + rows <= 65535) return go(kernel, blocks + rows, 64 * NWB, (int)blocks);
-        if (const int r = go(kernel, rows, 64 * NWB, 0)) return r;
-        return go(kernel, blocks, 64 * NWB, (int)blocks);
+        return go(backward_kernel<T, DB, DVB, NWB, decltype(qg)::value>, blocks + rows, 64 * NWB, (int)blocks);
       });
     } else {
       if (a.nq)
@@ -1762,7 +1767,7 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
   }
   if constexpr (sizeof(T) == 4) {
     const int64_t rows = (a.stacked ? (a.nq + a.batch - 1) / std::max(a.batch, 1) : a.n) << a.gsh;
-    if (which == kForwardKeys && rows <= 4 && tiles_of(a, false, rows == 1 ? 1 : 4) <= 65535)
+    if (which == kForwardKeys && rows <= 4)
       return rows == 1 ? run(fwd_rows_kernel<DB, DVB, 1>, 1, 512) : run(fwd_rows_kernel<DB, DVB, 4>, 4, 512);
   }
   if (keys) {

@@ -236,7 +236,7 @@ int make_args(const geotr_diff_attn* op, Args& a) {
   a.out = a.gq = a.gk = a.gv = nullptr, a.maps = a.lse = a.part = a.drow = a.rows = nullptr, a.amax = nullptr;
   a.lam = op->lam, a.q_len = op->q_lengths, a.k_len = op->k_lengths, a.masks = op->key_masks;
   a.batch = (int)op->batch, a.stacked = op->stacked != 0, a.n = (int)op->n, a.m = (int)op->m;
-  a.hk = (int)hk, a.g = (int)g, a.d = (int)op->dim, a.dv = (int)op->v_dim, a.causal = op->causal != 0, a.splits = 1;
+  a.hk = (int)hk, a.g = (int)g, a.d = (int)op->dim, a.dv = (int)op->v_dim, a.causal = op->causal != 0, a.splits = 1, a.tiles = a.tile0 = a.seq0 = 0;
   a.scale = op->scale, a.scale_log2 = (float)((double)op->scale * 1.4426950408889634);
   return GEOTR_OK;
 }

@@ -641,9 +641,10 @@ int geotr_rotary(const geotr_heads* q, const geotr_heads* q_out, const geotr_hea
 
 /* out[i, h] = sum_j (softmax_j(scale q[i, 2h] . k[j, 2c]) - lam[h] softmax_j(scale q[i, 2h+1] . k[j, 2c+1])) v[j, c],  c = h / (H / Hk).
  * q: 2 H heads of dim channels, k: 2 Hk heads, v: Hk heads of v_dim; H a multiple of Hk; dim <= 128, v_dim <= 256, multiples of 8; 16-byte
- * aligned views.  Two layouts: stacked = 0: (batch, n, ...) and (batch, m, ...), lengths NULL or (batch); stacked = 1: n and m are the
- * rows of ALL `batch` sequences one behind the other (stack mode), both lengths given.  Lengths are read on the device and held to the
- * rows that exist.  key_masks: bytes (batch, m) or (m), contiguous, nonzero = ignored.  causal: query i sees keys j <= i + (keys - queries) of its sequence.
+ * aligned views.  Up to 2^30 query rows (times H / Hk, rounded up to a power of two), 2^30 keys and 2^20 sequences, with gradients or without.
+ * Two layouts: stacked = 0: (batch, n, ...) and (batch, m, ...), lengths NULL or (batch); stacked = 1: n and m are the rows of ALL `batch`
+ * sequences one behind the other (stack mode), both lengths given.  Lengths are read on the device and held to the rows that exist.
+ * key_masks: bytes (batch, m) or (m), contiguous, nonzero = ignored.  causal: query i sees keys j <= i + (keys - queries) of its sequence.
  * Results of rows without a key, beyond their length or behind the last sequence are zero; what such key rows hold is never used.
  * out: contiguous (rows, H, v_dim).  For the gradients, both or none: maps (rows, H, 2, v_dim) fp32, the output of each map before lam, and
  * lse (Hk, 4, rows, H / Hk) fp32, the logarithms (base 2) of their sums in two parts. */

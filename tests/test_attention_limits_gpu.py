@@ -31,3 +31,62 @@ def test_gradients_of_2_28_query_rows():
     assert float((dlam.cpu().double() / batch - value).abs().max()) <= float((bound + 2.0 ** -23 * value.abs()).max())
     del out, state, dq, dk, dv
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('train', [False, True])
+@pytest.mark.parametrize('dtype,n,m,heads,kv,d,dv', [(torch.float32, 1, 5, 1, 1, 8, 8), (torch.float32, 3, 62, 1, 1, 8, 8), (torch.bfloat16, 3, 62, 2, 1, 64, 128),
+                                                     (torch.bfloat16, 20, 9, 2, 1, 32, 64), (torch.float16, 20, 9, 1, 1, 128, 256),
+                                                     (torch.float32, 20, 9, 2, 1, 64, 64)])
+def test_stacks_of_more_sequences_than_a_grid_holds_tiles(dtype, n, m, heads, kv, d, dv, train):
+    """70 000 times the same sequence, and rows behind the last: forward and both gradients, every form."""
+    from geotransformer_amd import kernels
+    batch = 70000
+    one, _, lam = _repeated(1, n, m, heads, kv, d, dv, dtype)
+    q, k, v, dout = (torch.cat([t.repeat(batch, 1, 1), t[:1]]) for t in one)
+    lens = [torch.full((batch,), x, dtype=torch.int64, device='cuda') for x in (n, m)]
+    want = oracle.differential_attention(one[0], one[1], one[2], lam, dout=one[3])
+    if train:
+        out, state = kernels.diff_attention(q, k, v, lam, *lens, want_state=True)
+        dq, dk, dv_, _ = kernels.diff_attention_backward(dout, q, k, v, lam, state, *lens)
+        results = (('out', out, n), ('dq', dq, n), ('dk', dk, m), ('dv', dv_, m))
+    else:
+        results = (('out', kernels.diff_attention(q, k, v, lam, *lens), n),)
+    for name, got, rows in results:
+        each = got[:batch * rows].unflatten(0, (batch, rows))
+        oracle.assert_within(name, each[0], *want[name])
+        assert bool((each == each[:1]).all()), name
+        assert not got[batch * rows:].any(), name
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_more_tiles_of_a_head_than_a_grid_holds(dtype):
+    """70 000 rows of 64 query heads to a key head in one sequence: 70 000 tiles of 64 packed rows."""
+    from geotransformer_amd import kernels
+    one, _, lam = _repeated(1, 70000, 5, 64, 1, 8, 8, dtype)
+    q, k, v, dout = one
+    out, state = kernels.diff_attention(q, k, v, lam, want_state=True)
+    assert torch.equal(out, kernels.diff_attention(q, k, v, lam)) or dtype != torch.float32
+    dq = kernels.diff_attention_backward(dout, q, k, v, lam, state)[0]
+    some = torch.cat([torch.arange(40), torch.arange(65500, 65560), torch.arange(69960, 70000)]).cuda()  # rows do not depend on each other
+    want = oracle.differential_attention(q[some], k, v, lam, dout=dout[some])
+    oracle.assert_within('out', out[some], *want['out'])
+    oracle.assert_within('dq', dq[some], *want['dq'])
+    half = [kernels.diff_attention(q[a:b], k, v, lam, want_state=True) for a, b in ((0, 35000), (35000, 70000))]
+    assert torch.equal(out, torch.cat([half[0][0], half[1][0]]))
+
+
+@pytest.mark.parametrize('train', [False, True])
+def test_more_heads_of_sequences_than_a_grid_holds(train):
+    """2^20 sequences of 8 key heads: 2^23 blocks of 512 threads are 2^32 threads along one axis."""
+    from geotransformer_amd import kernels
+    batch = 1 << 20
+    one, (q, k, v, dout), lam = _repeated(batch, 1, 2, 8, 8, 8, 8, torch.float32)
+    want = oracle.differential_attention(one[0], one[1], one[2], lam, dout=one[3])
+    if train:
+        out, state = kernels.diff_attention(q, k, v, lam, want_state=True)
+        results = (('out', out),) + tuple(zip(('dq', 'dk', 'dv'), kernels.diff_attention_backward(dout, q, k, v, lam, state)))
+    else:
+        results = (('out', kernels.diff_attention(q, k, v, lam)),)
+    for name, got in results:
+        oracle.assert_within(name, got[0], *want[name])
+        assert bool((got == got[:1]).all()), name
