@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void del_kernel(Args a, float* amax) {
   float most = 0.f;
   int64_t exist = a.nq;  // stack mode: rows behind the last sequence say nothing
   if constexpr (Narrow<T>::value) {
-    if (a.stacked && a.q_len) {
+    if (a.stacked) {
       exist = 0;
       for (int b = lane; b < a.batch; b += 64) exist += clamp_len(a.q_len[b], a.nq);
 #pragma unroll
@@ -220,7 +220,7 @@ int make_args(const geotr_diff_attn* op, Args& a) {
                   "differential attention: %lld query, %lld key and %lld value heads", (long long)op->q.heads, (long long)op->k.heads, (long long)hk);
   GEOTR_CHECK_ARG(op->scale > 0.f && op->scale < 1e30f, "differential attention: scale %g", (double)op->scale);
   GEOTR_CHECK_ARG(op->lam, "differential attention: lam is a null pointer");
-  GEOTR_CHECK_ARG(!op->stacked || (op->q_lengths && op->k_lengths), "differential attention: stack mode needs both lengths");
+  GEOTR_CHECK_ARG(!op->stacked || op->batch == 0 || (op->q_lengths && op->k_lengths), "differential attention: stack mode needs both lengths");
   const int size = op->dtype == GEOTR_F32 ? 4 : 2;
   const int64_t g = h / hk;
   a.gsh = 0;

@@ -38,3 +38,15 @@ def test_rotary_refuses_tangents(monkeypatch, which, grad):
         inputs[which] = forward_ad.make_dual(inputs[which], torch.ones_like(inputs[which]))
         with pytest.raises(NotImplementedError, match='forward-mode'):
             rope(*inputs)
+
+
+def test_a_stack_of_no_sequence_needs_no_lengths():
+    """An empty tensor of lengths has no address: the entry point takes it (no rows here, so nothing is launched)."""
+    import ctypes
+    from geotransformer_amd import _lib
+    lib, one = _lib.load(), 1 << 20  # a non-null, aligned address that is never read
+    view = lambda heads, d: kernels.Heads(one, heads, 0, heads * d, d)  # noqa: E731
+    op = kernels.DiffAttn(q=view(8, 16), k=view(4, 16), v=view(2, 32), dtype=0, stacked=1, batch=0, n=0, m=7, dim=16, v_dim=32, lam=one, scale=0.25)
+    assert lib.geotr_diff_attn_forward(ctypes.byref(op), one, None, None, None, 0, None) == 0
+    op.batch = 1
+    assert lib.geotr_diff_attn_forward(ctypes.byref(op), one, None, None, None, 0, None) == -1 and b'both lengths' in lib.geotr_last_error()

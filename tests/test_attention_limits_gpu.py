@@ -90,3 +90,20 @@ def test_more_heads_of_sequences_than_a_grid_holds(train):
     for name, got in results:
         oracle.assert_within(name, got[0], *want[name])
         assert bool((got == got[:1]).all()), name
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('d,dv', [(32, 64), (64, 128), (128, 256)])
+@pytest.mark.parametrize('n,m', [(5, 7), (100, 600), (1, 3), (0, 4)])
+def test_a_stack_of_no_sequence(dtype, d, dv, n, m):
+    """Lengths of no cloud at all: every row lies behind the last one."""
+    from geotransformer_amd.modules.transformer import differential_attention
+    one, _, lam = _repeated(1, n, m, 2, 1, d, dv, dtype)
+    none = torch.zeros(0, dtype=torch.int64, device='cuda')
+    with torch.no_grad():
+        assert not differential_attention(*one[:3], lam, none, none).any()
+    leaves = [t.requires_grad_() for t in (*one[:3], lam)]
+    y = differential_attention(*leaves, none, none)
+    assert y.shape == (n, 2, dv) and not y.any()
+    for g, t in zip(torch.autograd.grad(y, leaves, torch.full_like(y, float('nan'))), leaves):
+        assert g.shape == t.shape and not g.any()
