@@ -971,22 +971,27 @@ def diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks=None,
     return (out, (maps, lse)) if want_state else out
 
 
-def diff_attention_backward(dout, q, k, v, lam, state, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None):
+def diff_attention_backward(dout, q, k, v, lam, state, q_lengths=None, k_lengths=None, key_masks=None, causal=False, scale=None, checked=False):
     """(dq, dk, dv, dlam (H)) for dout from the state of diff_attention(..., want_state=True) (geotr_diff_attn_backward)."""
+    if not checked:
+        check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
+    lead, heads, kv_heads, v_dim = q.shape[:-2], q.shape[-2] // 2, v.shape[-2], v.shape[-1]
+    if dout.shape != lead + (heads, v_dim) or dout.dtype != q.dtype:
+        raise ValueError(f'dout is {q.dtype} of the output\'s shape {tuple(lead) + (heads, v_dim)}: got {dout.dtype} {tuple(dout.shape)}')
+    maps, lse = state
+    if maps.shape != lead + (heads, 2, v_dim) or lse.shape != (kv_heads, 4) + lead + (heads // kv_heads,):
+        raise ValueError(f'the state of another call: outputs of the maps {tuple(maps.shape)}, sums {tuple(lse.shape)}')
+    if maps.dtype != torch.float32 or lse.dtype != torch.float32 or not maps.is_contiguous() or not lse.is_contiguous():
+        raise ValueError(f'the state is passed on as diff_attention left it, float32 and contiguous: got {maps.dtype} and {lse.dtype}')
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
-    shape = q.shape[:-2] + (q.shape[-2] // 2, v.shape[-1])
-    if dout.shape != shape or dout.dtype != q.dtype:
-        raise ValueError(f'dout is {q.dtype} of the output\'s shape {tuple(shape)}: got {dout.dtype} {tuple(dout.shape)}')
-    if state[0].shape != shape[:-1] + (2, v.shape[-1]):
-        raise ValueError(f'the state of another call: outputs of the maps {tuple(state[0].shape)}')
-    _same_device(q, dout, *state)
+    _same_device(q, dout, maps, lse)
     lib = _lib.load()
     dout, dout_view = _aligned_heads(dout, 4 if dout.dtype == torch.float32 else 8)
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-    dlam = torch.empty(q.shape[-2] // 2, dtype=torch.float32, device=device)
+    dlam = torch.empty(heads, dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_backward_workspace_bytes(op)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _call(device, lib.geotr_diff_attn_backward, 'geotr_diff_attn_backward', op, _HEADS.pack(*dout_view), state[0].data_ptr(),
-          state[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), need)
+    _call(device, lib.geotr_diff_attn_backward, 'geotr_diff_attn_backward', op, _HEADS.pack(*dout_view), maps.data_ptr(),
+          lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), need)
     del keep
     return dq, dk, dv, dlam

@@ -28,7 +28,7 @@ class _DifferentialAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, lam, maps, lse, q_lengths, k_lengths, key_masks = ctx.saved_tensors
-        grads = kernels.diff_attention_backward(dout, q, k, v, lam, (maps, lse), q_lengths, k_lengths, key_masks, ctx.causal, ctx.scale)
+        grads = kernels.diff_attention_backward(dout, q, k, v, lam, (maps, lse), q_lengths, k_lengths, key_masks, ctx.causal, ctx.scale, checked=True)
         return grads + (None,) * 5
 
 

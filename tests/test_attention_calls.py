@@ -50,3 +50,32 @@ def test_a_stack_of_no_sequence_needs_no_lengths():
     assert lib.geotr_diff_attn_forward(ctypes.byref(op), one, None, None, None, 0, None) == 0
     op.batch = 1
     assert lib.geotr_diff_attn_forward(ctypes.byref(op), one, None, None, None, 0, None) == -1 and b'both lengths' in lib.geotr_last_error()
+
+
+def _state(q, v):
+    lead, heads, kv = q.shape[:-2], q.shape[-2] // 2, v.shape[-2]
+    return torch.zeros(*lead, heads, 2, v.shape[-1]), torch.zeros(kv, 4, *lead, heads // kv)
+
+
+@pytest.mark.parametrize('change,error,text', [
+    (dict(v=torch.zeros(6, 2, 32)), ValueError, 'do not fit'),            # a row less than k: rows behind v would be read
+    (dict(k=torch.zeros(7, 4, 24)), ValueError, 'multiples of 8'),
+    (dict(lam=torch.zeros(3)), ValueError, 'lam is'),
+    (dict(q_lengths=torch.tensor([5], dtype=torch.int32), k_lengths=torch.tensor([7], dtype=torch.int32)), TypeError, 'int64'),
+    (dict(q_lengths=torch.tensor([5])), ValueError, 'both lengths'),
+    (dict(key_masks=torch.zeros(6, dtype=torch.bool)), ValueError, 'truth values'),
+    (dict(scale=-1.0), ValueError, 'scale'),
+    (dict(dout=torch.zeros(4, 4, 32)), ValueError, 'dout is'),
+    (dict(state=(torch.zeros(4, 4, 2, 32), torch.zeros(2, 4, 5, 2))), ValueError, 'another call'),
+    (dict(state=(torch.zeros(5, 4, 2, 32), torch.zeros(4, 4, 5, 1))), ValueError, 'another call'),   # the sums of other groups of heads
+    (dict(state=(torch.zeros(5, 4, 2, 32), torch.zeros(2, 4, 4, 2))), ValueError, 'another call'),
+    (dict(state=(torch.zeros(5, 4, 2, 32), torch.zeros(2, 4, 5, 2, dtype=torch.float16))), ValueError, 'as diff_attention left it'),
+    (dict(state=(torch.zeros(5, 4, 32, 2).transpose(2, 3), torch.zeros(2, 4, 5, 2))), ValueError, 'as diff_attention left it'),
+])
+def test_the_gradient_entry_checks_its_arguments(change, error, text):
+    """Also what reaches it without the function: shapes that do not fit would be read past their ends."""
+    q, k, v, lam = _heads()
+    args = dict(dout=torch.zeros(5, 4, 32), q=q, k=k, v=v, lam=lam, state=_state(q, v))
+    args.update(change)
+    with pytest.raises(error, match=text):
+        kernels.diff_attention_backward(**args)
