@@ -229,9 +229,11 @@ __device__ __forceinline__ void arrived(V& x) {
   asm volatile("" : "+v"(x));
 }
 // x lies in accumulation registers here: without it the compiler takes the same ones for the scores, 64 moves a tile (dK/dV 327 -> 276 us at
-// 2 x 4 096 causal rows and 8 heads; 128/128 at 2 x 2 048 and 4: 222 -> 129).  Not for dQ of 32-bit heads of 128, whose 432 registers of
-// fragments and accumulators are spilled: there the compiler loses the first map's accumulators over this.
-__device__ __forceinline__ void held(f32x16& x) { asm volatile("" : "+a"(x)); }
+// 2 x 4 096 causal rows and 8 heads).  Only in kernels that spill nothing: in dQ of 32-bit heads of 128
+// (432 registers of fragments and accumulators) the compiler, out of registers, takes apart the four registers of a Q fragment around the pinned
+// accumulators and loses the copy of one: the first product read an accumulator in its place, and dQ of the first map was wrong.  The marker is
+// what a test finds pinned kernels by; it also looks for accumulators among the factors of every product.
+__device__ __forceinline__ void held(f32x16& x) { asm volatile("; held" : "+a"(x)); }
 template <typename T>
 __device__ __forceinline__ typename Ops<T>::Frag load_frag(__amdgpu_buffer_rsrc_t r, int offset) {
   return __builtin_bit_cast(typename Ops<T>::Frag, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
@@ -1374,9 +1376,11 @@ constexpr bool kLdsV = PART != kValuesOnly && sizeof(T) == 2 && (int)sizeof(T) *
 // bytes of 32 query rows, of dout's, and of 8 x 32 numbers of the rows
 template <typename T, int DB, int DVB>
 constexpr int kRowTile = 32 * (2 * DB + DVB) * (int)sizeof(T) + 1024;
-// QG = 2: the waves are two groups of keys x two of the query rows
+// QG = 2: the waves are two groups of keys x two of the query rows.  Not for 16-bit heads of 128 whose dK and dV are one launch: the tiles' second
+// addresses spill 17 registers there, and accumulators are pinned only where nothing spills (held, above; 232 instead of 212 us at 2 x 2 048
+// rows and 4 heads; spilled without the pins 312, dK and dV apart 252).
 template <typename T, int DB, int DVB, int PART>
-constexpr int kRowGroups = 4 * kRowTile<T, DB, DVB> + (kLdsV<T, DB, PART> ? 64 * DVB * (int)sizeof(T) : 0) <= 160 * 1024 ? 2 : 1;
+constexpr int kRowGroups = sizeof(T) == 2 && DB == 128 && PART == kBoth ? 1 : 4 * kRowTile<T, DB, DVB> + (kLdsV<T, DB, PART> ? 64 * DVB * (int)sizeof(T) : 0) <= 160 * 1024 ? 2 : 1;
 template <typename T, int DB, int DVB, int NW, int PART, int QG>
 constexpr int kSmemKV() {
   constexpr int kBuf = QG * kRowTile<T, DB, DVB>, NB = 2 * kBuf <= 140000 ? 2 : 1, kV = kLdsV<T, DB, PART> ? 32 * NW / QG * DVB * (int)sizeof(T) : 0;
@@ -1731,7 +1735,7 @@ int launch_dims(const Args& a, Which which, hipStream_t s) {
   auto run = [&](auto kernel, int tile, int threads) -> int { return go(kernel, tiles_of(a, false, tile), threads); };
   if (which == kBackward) {
     // Two query groups halve a block's keys and its steps, but load every query row twice as often.  They win while all their blocks run at
-    // once (2 x 2 048 rows and 4 heads, 128 against 64 blocks: 64/64 139 against 246 us, 128/128 220 against 308) and lose with more
+    // once (2 x 2 048 rows and 4 heads, 128 against 64 blocks: 64/64 139 against 246 us) and lose with more
     // (2 x 4 096 causal rows and 8 heads: 404 against 316).  32-bit products take 16 times as long as the loads: always (32 clouds of 295
     // rows: 119 against 128 us; 4 x 2 048 rows, 4 heads: 368 against 481).
     const int64_t tiles = a.stacked ? (a.nk / (32 * NWB) + a.batch / 2) : (int64_t)a.batch * ((a.m + 32 * NWB - 1) / (32 * NWB));

@@ -2,7 +2,9 @@
 
 * no instruction touches a register that an asm read may still be filling (scripts/check_inflight_regs.py: gemm_packed, gse_embed);
 * a buffer load issued by asm may read a scalar register that a vector instruction (v_readfirstlane, v_readlane, a compare) wrote only after
-  five wait states, along every path of the control flow, branches and loop back edges included."""
+  five wait states, along every path of the control flow, branches and loop back edges included;
+* no kernel that pins accumulators (its assembly carries the marker of `held`) spills vector registers, and no kernel multiplies by an
+  accumulator that stands in the place of a lost copy."""
 import os
 import re
 import subprocess
@@ -145,3 +147,82 @@ def test_tile_loads_wait_for_their_descriptors_on_every_path(assembly, name):
     assert len(kernels) >= 20 and sum('offen lds' in ln for _, lines, _ in kernels for ln in lines) > 100
     found = {kernel: early[:3] for kernel, early in ((k, too_early(lines)) for k, lines, _ in kernels) if early}
     assert not found, found
+
+
+# ---- accumulators -----------------------------------------------------------------------------------------------------------------------
+def _vectors(token):
+    m = re.match(r'([av])\[(\d+):(\d+)\]$', token)
+    if m:
+        return [m[1] + str(i) for i in range(int(m[2]), int(m[3]) + 1)]
+    return [token] if re.match(r'[av]\d+$', token) else []
+
+
+COPIES = ('v_accvgpr_read', 'v_accvgpr_write', 'v_accvgpr_mov', 'v_mov_b32', 'v_mov_b64', 'scratch_store', 'scratch_load')
+
+
+def sums_as_factors(lines):
+    """The matrix products of a kernel one of whose factors (not the sum that it adds to) may be another product's sum as it stands.  No kernel
+    here multiplies a sum before vector instructions worked on it, so such a factor is a register that a copy was lost for: fp32 dQ of heads
+    of 128 with pinned accumulators and spills multiplied K by an accumulator in place of one element of Q.  State at a point: the registers and
+    spill slots that may hold a sum; copies pass it on."""
+    code, labels = _parse(lines)
+    code = [(op, [_vectors(x) for x in args], args, int((re.search(r'offset:(\d+)', text) or [0, 0])[1]), text) for op, args, text in code]
+    ends = ('s_endpgm', 's_setpc_b64', 's_branch')
+    leaders = {0, *labels.values(), *(i + 1 for i, c in enumerate(code) if c[0].startswith('s_cbranch') or c[0] in ends)}
+    found, before, todo = set(), {0: frozenset()}, [0]
+    while todo:
+        at = todo.pop()
+        sums, following = set(before[at]), []
+        while at < len(code):
+            op, vec, args, slot, text = code[at]
+            if op.startswith('v_mfma'):
+                if any(r in sums for r in vec[1] + vec[2]):
+                    found.add((at, text))
+                sums.update(vec[0])
+            elif op.startswith(COPIES):  # pairs (to, from); a spill slot is its byte offset
+                if op.startswith('scratch_store'):
+                    pairs = [(slot + 4 * i, r) for i, r in enumerate(vec[1])]
+                elif op.startswith('scratch_load'):
+                    pairs = [(r, slot + 4 * i) for i, r in enumerate(vec[0])]
+                else:
+                    pairs = list(zip(vec[0], vec[1] or [None] * len(vec[0])))
+                for to, held in [(to, source in sums) for to, source in pairs]:
+                    (sums.add if held else sums.discard)(to)
+            elif vec and ' lds' not in text and not op.startswith(('s_', 'ds_write', 'buffer_store', 'global_store', 'v_cmp', 'v_read')):
+                sums.difference_update(vec[0], *(vec[1:2] if op.startswith(('v_permlane', 'v_swap')) else []))
+            if op.startswith('s_cbranch') or op == 's_branch':
+                following.append(labels[args[0]])
+            if op in ends:
+                break
+            at += 1
+            if at in leaders:
+                following.append(at)
+                break
+        for nxt in following:
+            if nxt < len(code) and (nxt not in before or not sums <= before[nxt]):
+                before[nxt] = before.get(nxt, frozenset()) | sums
+                todo.append(nxt)
+    return [text for _, text in sorted(found)]
+
+
+def test_the_check_finds_a_sum_in_the_place_of_a_factor():
+    product, zero = 'v_mfma_f32_32x32x2_f32 a[0:15], v1, {}, a[0:15]', 'v_accvgpr_write_b32 a1, v0'
+    assert not sums_as_factors([product.format('v2'), product.format('v2')])
+    assert sums_as_factors([product.format('v2'), product.format('a1')])
+    assert sums_as_factors([zero, '.L1:', 'v_mfma_f32_32x32x2_f32 a[16:31], v1, a1, 0', product.format('v2'), 's_cbranch_scc1 .L1', 's_endpgm'])
+    copied = [product.format('v2'), 'v_accvgpr_read_b32 v9, a3', 'scratch_store_dword off, v9, off offset:8', 'v_mov_b32_e32 v9, 0',
+              'scratch_load_dword v8, off, off offset:8']
+    assert sums_as_factors(copied + [product.format('v8')]) and not sums_as_factors(copied + ['v_exp_f32_e32 v8, v8', product.format('v8')])
+
+
+@pytest.mark.parametrize('name', ATTENTION)
+def test_no_product_takes_an_accumulator_for_a_factor(assembly, name):
+    found = {kernel: bad[:3] for kernel, bad in ((k, sums_as_factors(lines)) for k, lines, _ in kernels_of(assembly[name])) if bad}
+    assert not found, found
+
+
+@pytest.mark.parametrize('name', ATTENTION)
+def test_no_kernel_with_pinned_accumulators_spills(assembly, name):
+    kernels = kernels_of(assembly[name])
+    pinned = {k: scratch for k, lines, scratch in kernels if any('; held' in ln for ln in lines)}
+    assert len(pinned) >= 4 and not any(pinned.values()), pinned
