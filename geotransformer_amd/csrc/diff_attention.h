@@ -210,7 +210,7 @@ __device__ __forceinline__ void load_lds(i32x4 d, unsigned lds, int offset, int 
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(d), "s"(scalar)
-               : "memory");
+               : "m0", "memory");
 }
 // the descriptor `bytes` further on
 __device__ __forceinline__ i32x4 advance(i32x4 d, unsigned bytes) {
@@ -1511,7 +1511,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int 
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                    :
                    : "s"(__builtin_amdgcn_readfirstlane(tile + kRowBytes + x * 256)), "v"(there(col) ? so : kOutside), "s"(rs)
-                   : "memory");
+                   : "m0", "memory");
     }
   };
   auto fill = [&](unsigned tile, int r0) GEOTR_INLINE {

@@ -4,7 +4,8 @@
 * a buffer load issued by asm may read a scalar register that a vector instruction (v_readfirstlane, v_readlane, a compare) wrote only after
   five wait states, along every path of the control flow, branches and loop back edges included;
 * no kernel that pins accumulators (its assembly carries the marker of `held`) spills vector registers, and no kernel multiplies by an
-  accumulator that stands in the place of a lost copy."""
+  accumulator that stands in the place of a lost copy;
+* the asm that writes m0 says so."""
 import os
 import re
 import subprocess
@@ -226,3 +227,14 @@ def test_no_kernel_with_pinned_accumulators_spills(assembly, name):
     kernels = kernels_of(assembly[name])
     pinned = {k: scratch for k, lines, scratch in kernels if any('; held' in ln for ln in lines)}
     assert len(pinned) >= 4 and not any(pinned.values()), pinned
+
+
+def test_asm_that_writes_m0_says_so():
+    """A compiler that used m0 itself (indexed registers, messages) would otherwise find it changed."""
+    found = 0
+    for name in sorted(f for f in os.listdir(CSRC) if f.endswith(('.h', '.hip'))):
+        for m in re.finditer(r'asm\s*(?:volatile)?\s*\((.*?)\);', open(os.path.join(CSRC, name)).read(), re.S):
+            if re.search(r'\bm0\s*,', m[1]):
+                found += 1
+                assert '"m0"' in m[1].rsplit(':', 1)[1], (name, m[0])
+    assert found >= 2
