@@ -30,6 +30,7 @@ struct RotaryArgs {
   const int32_t* axis;
   float gain, sign;
   int pos_type, dim, rot, tiles, tokens, heads, heads_per_block, copy_rest;
+  unsigned block0;  // a launch's first block: a grid holds 2^32 threads along an axis
 };
 
 __device__ __forceinline__ double position_at(const void* p, int type, int64_t i) {
@@ -71,8 +72,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   constexpr int NP = kTwo ? E : E / 2;            // pairs per thread
   const int half = a.rot / 2;
   const int n_rot = half / NP, n_all = n_rot + (a.copy_rest ? (a.dim - a.rot) / E : 0);
-  const int b = blockIdx.x / (unsigned)a.tiles;
-  const int64_t row0 = (int64_t)(blockIdx.x - b * (unsigned)a.tiles) * a.tokens;
+  const unsigned block = a.block0 + blockIdx.x, b = block / (unsigned)a.tiles;
+  const int64_t row0 = (int64_t)(block - b * (unsigned)a.tiles) * a.tokens;
   const int h0 = blockIdx.y * a.heads_per_block, h1 = min(h0 + a.heads_per_block, a.heads);
   const int hq = (int)a.q.heads;
   for (int u = threadIdx.x; u < a.tokens * n_all; u += 256) {
@@ -202,11 +203,15 @@ extern "C" int geotr_rotary(const geotr_heads* q, const geotr_heads* q_out, cons
   // all heads in one thread once the tokens alone give 2 048 blocks (the angles are computed once); fewer tokens: heads over more blocks
   const int64_t want = std::min<int64_t>(a.heads, (2048 + blocks - 1) / blocks);
   a.heads_per_block = (int)((a.heads + want - 1) / want);
-  const dim3 grid((unsigned)blocks, (unsigned)((a.heads + a.heads_per_block - 1) / a.heads_per_block));
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == GEOTR_F32) rotary_dispatch<float>(a, e, interleaved, grid, s);
-  else if (dtype == GEOTR_BF16) rotary_dispatch<__bf16>(a, e, interleaved, grid, s);
-  else rotary_dispatch<_Float16>(a, e, interleaved, grid, s);
-  GEOTR_CHECK_LAUNCH("geotr_rotary");
+  constexpr int64_t kMost = 1 << 23;
+  for (int64_t first = 0; first < blocks; first += kMost) {
+    a.block0 = (unsigned)first;
+    const dim3 grid((unsigned)std::min(kMost, blocks - first), (unsigned)((a.heads + a.heads_per_block - 1) / a.heads_per_block));
+    if (dtype == GEOTR_F32) rotary_dispatch<float>(a, e, interleaved, grid, s);
+    else if (dtype == GEOTR_BF16) rotary_dispatch<__bf16>(a, e, interleaved, grid, s);
+    else rotary_dispatch<_Float16>(a, e, interleaved, grid, s);
+    GEOTR_CHECK_LAUNCH("geotr_rotary");
+  }
   return GEOTR_OK;
 }

@@ -107,3 +107,15 @@ def test_a_stack_of_no_sequence(dtype, d, dv, n, m):
     assert y.shape == (n, 2, dv) and not y.any()
     for g, t in zip(torch.autograd.grad(y, leaves, torch.full_like(y, float('nan'))), leaves):
         assert g.shape == t.shape and not g.any()
+
+
+def test_rotary_of_more_sequences_than_a_grid_holds_blocks():
+    """2^24 + 3 sequences of one token are 2^32 threads: the same as one sequence of as many tokens."""
+    from geotransformer_amd.modules.transformer import RotaryPositionalEmbedding
+    rows = (1 << 24) + 3
+    rope = RotaryPositionalEmbedding(8).cuda()
+    g = torch.Generator('cuda').manual_seed(0)
+    q, pos = torch.randn(rows, 1, 8, generator=g, device='cuda').bfloat16(), torch.arange(rows, device='cuda')
+    want = rope(q, None, pos)[0]
+    got = rope(q[:, None], None, pos[:, None])[0]
+    assert torch.equal(got[:, 0], want)
