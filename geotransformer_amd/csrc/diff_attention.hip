@@ -195,16 +195,20 @@ int launch(int dtype, const Args& a, Which which, hipStream_t s) {
   return dtype == GEOTR_F32 ? launch_f32(a, which, s) : dtype == GEOTR_BF16 ? launch_bf16(a, which, s) : launch_f16(a, which, s);
 }
 
-int check_view(const geotr_heads& v, int64_t heads, int size, int64_t batch, int64_t rows, const char* what) {
+// near: rows and heads that a tile reaches by 32-bit offsets from its first element, below the 1 GiB a buffer descriptor here covers; other
+// heads and rows have 64-bit addresses of their own
+int check_view(const geotr_heads& v, int64_t heads, int size, int64_t batch, int64_t rows, int64_t near_rows, int64_t near_heads, const char* what) {
   GEOTR_CHECK_ARG(v.heads == heads, "differential attention: %s has %lld heads, expected %lld", what, (long long)v.heads, (long long)heads);
   if (batch * rows == 0) return GEOTR_OK;
   GEOTR_CHECK_ARG(v.data, "differential attention: %s is a null pointer", what);
   const int e = 16 / size;
   GEOTR_CHECK_ARG((uintptr_t)v.data % 16 == 0 && v.batch_stride % e == 0 && v.row_stride % e == 0 && v.head_stride % e == 0,
                   "differential attention: %s is not a 16-byte aligned view", what);
-  // a tile of 128 rows is addressed by 32-bit offsets from its first row, below the 1 GiB a buffer descriptor here covers
-  GEOTR_CHECK_ARG(v.row_stride >= 0 && v.head_stride >= 0 && (128 * v.row_stride + 128 * v.head_stride + 512) * size < kNumRecords,
-                  "differential attention: strides of %s (rows %lld, heads %lld elements)", what, (long long)v.row_stride, (long long)v.head_stride);
+  const int64_t most = 1ll << 40;  // no product below passes 64 bits
+  GEOTR_CHECK_ARG(v.row_stride >= 0 && v.head_stride >= 0 && v.row_stride < most && v.head_stride < most &&
+                      (near_rows * v.row_stride + near_heads * v.head_stride + 512) * size < kNumRecords,
+                  "differential attention: strides of %s (rows %lld, heads %lld elements): %lld rows and %lld heads on have to lie within 1 GiB, "
+                  "which a contiguous tensor's do", what, (long long)v.row_stride, (long long)v.head_stride, (long long)near_rows, (long long)near_heads);
   return GEOTR_OK;
 }
 
@@ -229,8 +233,8 @@ int make_args(const geotr_diff_attn* op, Args& a) {
   GEOTR_CHECK_ARG((a.nq << a.gsh) <= kMostRows && a.nk <= kMostRows, "differential attention: %lld query rows (x %lld heads) and %lld keys in one call",
                   (long long)a.nq, (long long)g, (long long)a.nk);
   int rc;
-  if ((rc = check_view(op->q, 2 * h, size, op->batch, op->n, "q")) || (rc = check_view(op->k, 2 * hk, size, op->batch, op->m, "k")) ||
-      (rc = check_view(op->v, hk, size, op->batch, op->m, "v")))
+  if ((rc = check_view(op->q, 2 * h, size, op->batch, op->n, 64, 2ll << a.gsh, "q")) || (rc = check_view(op->k, 2 * hk, size, op->batch, op->m, 128, 1, "k")) ||
+      (rc = check_view(op->v, hk, size, op->batch, op->m, 128, 0, "v")))
     return rc;
   a.q = op->q, a.k = op->k, a.v = op->v, a.dout = geotr_heads{nullptr, 0, 0, 0, 0};
   a.out = a.gq = a.gk = a.gv = nullptr, a.maps = a.lse = a.part = a.drow = a.rows = nullptr, a.amax = nullptr;
@@ -315,7 +319,7 @@ int geotr_diff_attn_backward(const geotr_diff_attn* op, const geotr_heads* dout,
   if (rc != GEOTR_OK) return rc;
   GEOTR_CHECK_ARG(dout && dlam, "geotr_diff_attn_backward: null pointer");
   const int size = op->dtype == GEOTR_F32 ? 4 : 2;
-  if (const int r = check_view(*dout, (int64_t)a.hk * a.g, size, op->batch, op->n, "dout")) return r;
+  if (const int r = check_view(*dout, (int64_t)a.hk * a.g, size, op->batch, op->n, 64, 1ll << a.gsh, "dout")) return r;
   GEOTR_CHECK_ARG((a.nq == 0 || (maps && lse && dq)) && (a.nk == 0 || (dk && dv)), "geotr_diff_attn_backward: null pointer");
   GEOTR_CHECK_ARG((uintptr_t)maps % 16 == 0 && (uintptr_t)dq % 16 == 0 && (uintptr_t)dk % 16 == 0 && (uintptr_t)dv % 16 == 0,
                   "geotr_diff_attn_backward: results are not 16-byte aligned");

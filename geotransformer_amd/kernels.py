@@ -866,9 +866,9 @@ def rotary(q, k, positions, turns, axis, rotary_dim, interleaved=False, gain=1.0
     return q_out, k_out
 
 
-def _aligned_heads(t, e):
+def _aligned_heads(t, e, near_rows, near_heads):
     """(t, words of geotr_heads) with channels contiguous, addresses and strides multiples of 16 bytes (e elements: what the tiles are loaded
-    in); a contiguous copy where t's are not."""
+    in), and the rows and heads that one tile reaches within 1 GiB; a contiguous copy where t's are not."""
     size, stride = t.shape, t.stride()
     if len(size) == 4:
         batch, rows, heads, _ = size
@@ -884,8 +884,8 @@ def _aligned_heads(t, e):
     if heads == 1:
         h = 0
     address = t.data_ptr()
-    if c != 1 or address & 15 or (b | r | h) & (e - 1):
-        return _aligned_heads(t.clone(memory_format=torch.contiguous_format), e)
+    if c != 1 or address & 15 or (b | r | h) & (e - 1) or ((near_rows * r + near_heads * h + 512) * 16 >= e << 30 and not t.is_contiguous()):
+        return _aligned_heads(t.clone(memory_format=torch.contiguous_format), e, near_rows, near_heads)
     return t, (address, heads, b, r, h)
 
 
@@ -931,7 +931,8 @@ def _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale):
     device = _same_device(q, k, v, lam, q_lengths, k_lengths, key_masks)
     qs, dtype = q.shape, q.dtype
     e = 4 if dtype == torch.float32 else 8
-    (q, q_view), (k, k_view), (v, v_view) = _aligned_heads(q, e), _aligned_heads(k, e), _aligned_heads(v, e)
+    group = 1 << (qs[-2] // (2 * v.shape[-2]) - 1).bit_length()
+    (q, q_view), (k, k_view), (v, v_view) = _aligned_heads(q, e, 64, 2 * group), _aligned_heads(k, e, 128, 1), _aligned_heads(v, e, 128, 0)
     if lam.dim() == 0 or lam.shape[0] * 2 != qs[-2] or lam.stride(0) != 1:
         lam = lam.expand(qs[-2] // 2).contiguous()
     ql = kl = masks = 0
@@ -986,7 +987,7 @@ def diff_attention_backward(dout, q, k, v, lam, state, q_lengths=None, k_lengths
     op, keep, device = _diff_attn(q, k, v, lam, q_lengths, k_lengths, key_masks, causal, scale)
     _same_device(q, dout, maps, lse)
     lib = _lib.load()
-    dout, dout_view = _aligned_heads(dout, 4 if dout.dtype == torch.float32 else 8)
+    dout, dout_view = _aligned_heads(dout, 4 if dout.dtype == torch.float32 else 8, 64, 1 << (heads // kv_heads - 1).bit_length())
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     dlam = torch.empty(heads, dtype=torch.float32, device=device)
     need = lib.geotr_diff_attn_backward_workspace_bytes(op)

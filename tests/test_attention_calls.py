@@ -79,3 +79,22 @@ def test_the_gradient_entry_checks_its_arguments(change, error, text):
     args.update(change)
     with pytest.raises(error, match=text):
         kernels.diff_attention_backward(**args)
+
+
+def test_strides_are_held_to_what_a_tile_reaches():
+    """A cache laid out by heads, (heads, keys, channels) seen as (keys, heads, channels): heads may lie as far apart as the offsets of one tile
+    allow, 1 GiB for the two maps of a key, any distance for values."""
+    import ctypes
+    from geotransformer_amd import _lib
+    lib, one = _lib.load(), 1 << 20
+
+    def call(**strides):
+        view = lambda name, heads, d: kernels.Heads(one, heads, 0, *strides.get(name, (heads * d, d)))  # noqa: E731
+        op = kernels.DiffAttn(q=view('q', 8, 16), k=view('k', 4, 16), v=view('v', 2, 32), dtype=0, batch=1, n=0, m=7, dim=16, v_dim=32, lam=one, scale=0.25)
+        code = lib.geotr_diff_attn_forward(ctypes.byref(op), one, None, None, None, 0, None)
+        return code, lib.geotr_last_error() if code else b''
+
+    assert call(k=(16, 1 << 27), v=(32, 1 << 34), q=(16, 1 << 25)) == (0, b'')
+    assert b'strides of k' in call(k=(16, 1 << 28))[1]
+    assert b'strides of k' in call(k=(1 << 22, 16))[1] and b'strides of v' in call(v=(1 << 22, 32))[1]
+    assert b'strides of v' in call(v=(32, 1 << 62))[1] and b'strides of v' in call(v=(1 << 62, 32))[1]  # their products would pass 64 bits

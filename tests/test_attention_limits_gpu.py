@@ -119,3 +119,23 @@ def test_rotary_of_more_sequences_than_a_grid_holds_blocks():
     want = rope(q, None, pos)[0]
     got = rope(q[:, None], None, pos[:, None])[0]
     assert torch.equal(got[:, 0], want)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n,heads,kv', [(1, 4, 2), (5, 4, 2), (90, 4, 2), (3, 64, 1)])
+@pytest.mark.parametrize('d,dv', [(32, 64), (64, 128), (128, 256)])
+def test_a_cache_laid_out_by_heads(dtype, n, heads, kv, d, dv):
+    """(heads, keys, channels) seen as (keys, heads, channels), heads tens of megabytes apart: the same as contiguous tensors."""
+    from geotransformer_amd.modules.transformer import differential_attention
+    room, m = 140000 * 32 // d + 8, 333
+    g = torch.Generator('cuda').manual_seed(0)
+    by_heads = [torch.empty(h, room, c, dtype=dtype, device='cuda').transpose(0, 1) for h, c in ((2 * heads, d), (2 * kv, d), (kv, dv))]
+    q, k, v = (t[:r].copy_(torch.randn(r, *t.shape[1:], generator=g, device='cuda')) for t, r in zip(by_heads, (n, m, m)))
+    lam = torch.rand(heads, generator=g, device='cuda')
+    assert q.stride(1) >= 2 ** 22 and torch.equal(differential_attention(q, k, v, lam), differential_attention(*(t.contiguous() for t in (q, k, v)), lam))
+    dout = torch.empty(heads, room, dv, dtype=dtype, device='cuda').transpose(0, 1)[:n].copy_(torch.randn(n, heads, dv, generator=g, device='cuda'))
+    grads = []
+    for copy in (False, True):
+        leaves = [(t.contiguous() if copy else t).detach().requires_grad_() for t in (q, k, v, lam)]
+        grads.append(torch.autograd.grad(differential_attention(*leaves), leaves, dout.contiguous() if copy else dout))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
