@@ -908,6 +908,8 @@ def check_diff_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_masks
         raise ValueError(f'channels of a head are multiples of 8, q and k alike up to 128, v up to 256: got {dim}, {ks[-1]}, {v_dim}')
     if lam.dtype != torch.float32 or lam.dim() > 1 or lam.numel() not in (1, heads):
         raise ValueError(f'lam is a float32 tensor of 1 or {heads} values: got {lam.dtype} {tuple(lam.shape)}')
+    if torch.is_tensor(scale) and scale.requires_grad:
+        raise NotImplementedError('differential attention is not differentiable in scale: pass a number, or scale q')
     if scale is not None and not 0.0 < float(scale) < 1e30:
         raise ValueError(f'scale is a positive number, not {scale}')
     if dims == 3 and (q_lengths is None) != (k_lengths is None):

@@ -98,3 +98,11 @@ def test_strides_are_held_to_what_a_tile_reaches():
     assert b'strides of k' in call(k=(16, 1 << 28))[1]
     assert b'strides of k' in call(k=(1 << 22, 16))[1] and b'strides of v' in call(v=(1 << 22, 32))[1]
     assert b'strides of v' in call(v=(32, 1 << 62))[1] and b'strides of v' in call(v=(1 << 62, 32))[1]  # their products would pass 64 bits
+
+
+def test_a_scale_that_wants_a_gradient_is_refused():
+    """It would be taken for a number, and its gradient would silently be missing."""
+    scale = torch.tensor(0.25, requires_grad=True)
+    with pytest.raises(NotImplementedError, match='scale'):
+        differential_attention(*_heads(), scale=scale)
+    kernels.check_diff_attention(*_heads(), scale=scale.detach())
