@@ -229,8 +229,9 @@ int make_args(const geotr_diff_attn* op, Args& a) {
   const int64_t g = h / hk;
   a.gsh = 0;
   while ((1 << a.gsh) < g) ++a.gsh;
-  a.nq = op->stacked ? op->n : op->batch * op->n, a.nk = op->stacked ? op->m : op->batch * op->m;
-  GEOTR_CHECK_ARG((a.nq << a.gsh) <= kMostRows && a.nk <= kMostRows, "differential attention: %lld query rows (x %lld heads) and %lld keys in one call",
+  const int64_t most = 1ll << 40;  // the products stay below 2^63
+  a.nq = std::min(op->n, most) * (op->stacked ? 1 : op->batch), a.nk = std::min(op->m, most) * (op->stacked ? 1 : op->batch);
+  GEOTR_CHECK_ARG(op->n <= kMostRows && op->m <= kMostRows && (a.nq << a.gsh) <= kMostRows && a.nk <= kMostRows, "differential attention: %lld query rows (x %lld heads) and %lld keys in one call",
                   (long long)a.nq, (long long)g, (long long)a.nk);
   int rc;
   if ((rc = check_view(op->q, 2 * h, size, op->batch, op->n, 64, 2ll << a.gsh, "q")) || (rc = check_view(op->k, 2 * hk, size, op->batch, op->m, 128, 1, "k")) ||

@@ -197,8 +197,9 @@ extern "C" int geotr_rotary(const geotr_heads* q, const geotr_heads* q_out, cons
   const int pairs = interleaved && e > 1 ? e / 2 : e;
   const int n_all = (int)(rotary_dim / 2) / pairs + (a.copy_rest ? (int)(dim - rotary_dim) / e : 0);
   a.tokens = std::max(1, 256 / n_all);
-  const int64_t tiles = (rows + a.tokens - 1) / a.tokens, blocks = tiles * batch;
-  GEOTR_CHECK_ARG(blocks <= 0x7fffffff, "geotr_rotary: %lld x %lld tokens in one call", (long long)batch, (long long)rows);
+  const int64_t tiles = rows / a.tokens + (rows % a.tokens != 0);
+  GEOTR_CHECK_ARG(tiles <= 0x7fffffff / batch, "geotr_rotary: %lld x %lld tokens in one call", (long long)batch, (long long)rows);
+  const int64_t blocks = tiles * batch;
   a.tiles = (int)tiles, a.heads = (int)(a.q.heads + a.k.heads);
   // all heads in one thread once the tokens alone give 2 048 blocks (the angles are computed once); fewer tokens: heads over more blocks
   const int64_t want = std::min<int64_t>(a.heads, (2048 + blocks - 1) / blocks);

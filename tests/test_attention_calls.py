@@ -106,3 +106,18 @@ def test_a_scale_that_wants_a_gradient_is_refused():
     with pytest.raises(NotImplementedError, match='scale'):
         differential_attention(*_heads(), scale=scale)
     kernels.check_diff_attention(*_heads(), scale=scale.detach())
+
+
+def test_numbers_of_rows_that_pass_64_bits_are_refused():
+    """Their products with the number of sequences came out small, and the call went on with them."""
+    import ctypes
+    from geotransformer_amd import _lib
+    lib, one = _lib.load(), 1 << 20
+    view = lambda heads, d: kernels.Heads(one, heads, 0, heads * d, d)  # noqa: E731
+    for n, m in ((1 << 62, 7), (5, 1 << 62), ((1 << 62) + 1, 1 << 62), (1 << 31, 7), (5, 1 << 31)):
+        op = kernels.DiffAttn(q=view(8, 16), k=view(4, 16), v=view(2, 32), dtype=0, batch=4, n=n, m=m, dim=16, v_dim=32, lam=one, scale=0.25)
+        assert lib.geotr_diff_attn_forward(ctypes.byref(op), None, None, None, None, 0, None) == -1 and b'query rows' in lib.geotr_last_error(), (n, m)
+        assert lib.geotr_diff_attn_workspace_bytes(ctypes.byref(op)) == lib.geotr_diff_attn_backward_workspace_bytes(ctypes.byref(op)) == 0
+    for batch, rows in ((4, 1 << 62), (1 << 62, 4), (1 << 40, 1 << 40), (1 << 32, 1)):
+        code = lib.geotr_rotary(ctypes.byref(view(4, 16)), ctypes.byref(view(4, 16)), None, None, 0, batch, rows, 16, 16, 0, one, 1, 0, 1, 0, one, one, 1.0, 0, None)
+        assert code == -1 and b'tokens in one call' in lib.geotr_last_error(), (batch, rows)
