@@ -10,6 +10,9 @@
 //   dlam = - sum_ij P2 dP.  Blocks that own query rows (dQ, dlam) and blocks that own keys (dK, dV): the scores are computed twice, and no sum
 //   depends on the order of atomics.
 //
+// Buckets of widths (32, 64, 128; values one or two times that) and groups of heads rounded up to a power of two pad what lies between: a head
+// of 80 or 96 takes the time of 128 (52 and 53 us against 56, causal 2 x 2 048 rows, 4 heads, bf16), a group of 5 or 7 nearly that of 8 (62, 65 and
+// 68 us, 2 key heads, 64, 128).
 // Layout of the matrix work (32 x 32 MFMA, a wave = 32 rows of one kind): scores are computed TRANSPOSED to how they are consumed, so the
 // accumulator a lane holds (16 of 32 contraction indices of ONE row) is the B operand of the next product as it stands: no exchange
 // between lanes and no LDS round trip for P and dS.  The other operand of that product is read transposed from LDS (ds_read_b64_tr_b16;
@@ -477,9 +480,13 @@ __device__ __forceinline__ void zero_rows(const Args& a, const Seq& s, int kvh, 
 
 // Many rows: the waves are two maps x G groups of 32 packed rows; a wave owns 32 rows of ONE map, so it needs half the accumulators (three
 // waves to a SIMD unit at d = 64, v 128, where both maps in a wave leave one) and the maps meet in LDS at the end.  Tiles of 32 keys in two
-// buffers: the next one loads while this one is consumed.  Bound: matrix and vector instructions of a SIMD unit issue one after the other
-// (12 products of 32 cycles and 58 vector instructions for 32 x 32 weights at 64, 128).  8 192 causal rows, 16 heads, 64, 128, bf16: 433 us,
-// 0.95 PFLOP/s of the four products where a large library product of this card reaches 1.2; 32 bits, 2 048 rows: 112 of 138 TFLOP/s.
+// buffers: the next one loads while this one is consumed.  8 192 causal rows, 16 heads on 4, 64, 128, bf16: 416 us, 0.99 PFLOP/s of the four
+// products where a large library product of this card reaches 1.2.  Counters of that call: matrix core busy 0.51 of the cycles, vector
+// instructions 0.50, LDS 0.42 (and 0.17 in conflicts), 2.5 waves to a SIMD unit that wait for an issue slot 0.36 of their life and for data 0.30:
+// the two kinds of work take about their sum; what keeps them from overlapping is not established.  32 bits, 2 048 rows: 112 of 138 TFLOP/s.
+// P is rounded to the type before its product (outputs in 16 bits are off by 1.2 to 1.4 times what rounding the exact ones gives): a 32-bit
+// product takes 16 times as long.  EXACT (below) keeps the rest as well, so a training call's output differs from the same call without
+// gradients in the last bits.
 // The accumulators are rescaled only when a row's maximum grew by more than 2^8: weights stay below 2^8, sums are exact either way.
 // FEW (a token over a cache, wide heads): the G groups share 32 rows and take 32 keys each of every tile, joined at the end.
 // EXACT (16-bit, for training): what rounding P to 16 bits takes away goes through a second product, because the gradients subtract
@@ -742,10 +749,11 @@ __global__ __launch_bounds__(128 * G, (kWavesRows<T, DB, DVB>)) void fwd_kernel(
     }
 }
 
-// Few rows (a token over a cache; in 32 bits five rows and more): the NW waves own the same 32 packed rows, both maps, and every wave streams key tiles of its own (no
-// barrier), joined at the end; with a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next launch.
-// Bound: HBM.  8 tokens over caches of up to 32 768 keys, 16 heads on 4, 64, 128, bf16: 83 us, 4.9 of the 5.1 TB/s of a large copy, and 6 us
-// for the join (with the two maps' waves sharing tiles behind barriers, 103).
+// Few rows (a token over a cache; in 32 bits five rows and more): the NW waves own the same 32 packed rows, both maps, and every wave streams
+// key tiles of its own (no barrier), joined at the end; with a.splits > 1 the keys are dealt over blockIdx.z and the partials joined by the next
+// launch.  Bound: HBM.  8 tokens over caches of up to 32 768 keys, 16 heads on 4, 64, 128, bf16: 81 us, 4.9 of the 5.1 TB/s of a large copy, and
+// 6 us for the join (with the two maps' waves sharing tiles behind barriers, 103).  4 tokens of 32 heads on 4 over 8 192 keys, 32, 64, 32 bits:
+// 26 us, 13 at the copy's rate.  P is rounded to the type before its product.
 template <typename T, int DB, int DVB, int NW>
 __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void fwd_keys_kernel(Args a) {
   using Frag = typename Ops<T>::Frag;
@@ -1137,7 +1145,8 @@ __device__ __forceinline__ float grad_scale(const Args& a) {
 
 // A wave owns 32 packed rows.  Where two tiles of 64 keys fit into LDS the four waves are two groups of rows x two of the keys, joined at the
 // end: blocks of 64 rows fill the chip at half the rows, and the longest causal block ends after half the steps (2 x 4 096 causal rows, 8
-// heads, 64, 128: 175 -> 157 us; 128, 256 at 2 x 2 048 and 4 heads: 187 -> 116).  Bound: latency of two waves to a SIMD unit, 0.65 PFLOP/s.
+// heads, 64, 128: 175 -> 157 us, 147 by now; 128, 256 at 2 x 2 048 and 4 heads: 187 -> 116).  Bound: latency of 1.6 waves to a SIMD unit (matrix
+// core busy 0.31, vector instructions 0.46, 0.30 of a wave's life in waits for data), 0.70 PFLOP/s.  dS is rounded to the type before its product.
 template <typename T, int DB, int DVB>
 constexpr int kKeyGroups = 128 * (2 * DB + DVB) * (int)sizeof(T) <= 131072 ? 2 : 1;
 template <typename T, int DB, int DVB, int NW>
@@ -1361,10 +1370,11 @@ __global__ __launch_bounds__(NW * 64, (kWaves<T, DB, DVB>)) void dq_kernel(Args 
 // ---- backward: keys (dK, dV) --------------------------------------------------------------------------------------------------------------
 // A wave owns 32 keys; K and V are the B operands (lane = key).  16-bit K and V stay in registers, V of wide heads in LDS; in 32 bits they are
 // read again from memory for every tile of 32 packed query rows (a product takes 16 times as long as the load; held: 136 against 129 us at
-// 32 clouds of 295, spilled).  Bound: latency of one wave to a SIMD unit, 0.5 PFLOP/s at 2 x 4 096 causal rows, 8 heads, 64, 128 (270 us);
-// two waves spill (989 us).  Where both gradients' accumulators leave no registers (16-bit heads of 128, values of 256) dK and dV are two launches, the scores twice:
-// 20 instead of 16 products of d, 334 instead of 462 us at 2 x 2 048 rows and 4 heads (260 by now).  Narrower heads lose by it (64, 128: 370 against
-// 274 us at 2 x 4 096 causal rows and 8 heads).
+// 32 clouds of 295, spilled).  Bound: latency of one wave to a SIMD unit (matrix core busy 0.24, vector instructions 0.36), 0.55 PFLOP/s at
+// 2 x 4 096 causal rows, 8 heads, 64, 128 (251 us); two waves spill (989 us).  Where both gradients' accumulators leave no registers (16-bit heads
+// of 128, values of 256) dK and dV are two launches, the scores twice: 20 instead of 16 products of d, 334 instead of 462 us at 2 x 2 048 rows and
+// 4 heads (255 by now).  Narrower heads lose by it (64, 128: 370 against 274 us at 2 x 4 096 causal rows and 8 heads; 128, 128 at 2 x 2 048 and 4:
+// 162 against 142).  P1 - lam P2 and dS are rounded to the type before their products.
 enum Part { kBoth, kKeysOnly, kValuesOnly };
 template <typename T, int DVB>
 constexpr bool kSplitKV = sizeof(T) == 2 && DVB == 256;
@@ -1693,7 +1703,7 @@ __global__ __launch_bounds__(NW * 64, (kWavesKV<T, DB, DVB, PART>)) void dkv_ker
   dkv_block<T, DB, DVB, NW, PART, QG>(a, smem, a.tile0 + blockIdx.y, a.tiles);
 }
 // Both in one launch where both take two waves to a SIMD unit, the first key_blocks of a head for the keys: the last blocks of one fill what the
-// other's leave empty (32 clouds of 295 in 32 bits, 32, 64: 215 -> 172 us; 2 x 2 048 rows, 4 heads, bf16: 81 -> 63).
+// other's leave empty (32 clouds of 295 in 32 bits, 32, 64: 215 -> 169 us, 25 registers spilled in 32 bits; 2 x 2 048 rows, 4 heads, bf16: 81 -> 60).
 template <typename T, int DB, int DVB, int NW, int QG>
 __global__ __launch_bounds__(NW * 64, 2) void backward_kernel(Args a, int key_blocks) {
   constexpr int kQ = kSmemQ<T, DB, DVB, NW>(), kKV = kSmemKV<T, DB, DVB, NW, kBoth, QG>();

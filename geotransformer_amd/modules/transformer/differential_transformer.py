@@ -43,6 +43,8 @@ def differential_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_mas
     lam: float32 tensor, one value or one per head; key_masks: truth values of the key rows, True = ignored (what an ignored row, or one
     beyond its length, holds is never read into a result); causal: query i sees keys j <= i + keys - queries of its cloud; scale: default
     1 / sqrt(d).  Rows without any key, beyond their length or behind the last cloud give zeros.
+    In 16-bit types the weights are rounded to the type before their product with v; a call that keeps what a gradient needs adds the rest in a
+    second product, so its output differs from the same call without gradients in the last bits.
     Returns (rows, H, d_v) / (batch, rows, H, d_v).  Differentiable in q, k, v and lam (once, in reverse mode); gradients do not depend on scheduling."""
     kernels.check_diff_attention(q, k, v, lam, q_lengths, k_lengths, key_masks, scale)
     kernels.refuse_tangents('differential_attention', q, k, v, lam)
@@ -55,7 +57,10 @@ def differential_attention(q, k, v, lam, q_lengths=None, k_lengths=None, key_mas
 class DifferentialMultiHeadAttention(nn.Module):
     """num_heads pairs of maps of d_model / num_heads / 2 channels each, values of d_model / num_heads.  lam = exp(a1 . b1) - exp(a2 . b2) +
     lambda_init with learned vectors; the heads are normalised one by one and scaled by 1 - lambda_init.  positions_* (1, N, 3): points
-    whose coordinates turn the heads (None: no positions)."""
+    whose coordinates turn the heads (None: no positions).
+
+    The heads' norm is this package's LayerNorm, with a mean and a bias; the published layer divides each head by its root mean square alone.
+    Weights trained with that layer are not this module's: use differential_attention and their own norm."""
 
     def __init__(self, d_model, num_heads, dropout=None, lambda_init=0.5, rotary_base=10000.0):
         super().__init__()

@@ -18,7 +18,8 @@ def rotary_frequencies(pairs, base=10000.0, scaling=None, scaling_factor=1.0, or
     'linear': every frequency divided by scaling_factor;
     'ntk':    a larger base, such that the slowest pair slows down by scaling_factor and the fastest keeps its rate;
     'yarn':   by parts (YaRN, Peng et al. 2023): pairs that turn beta_fast times or more within original_length keep their rate, pairs that
-              turn beta_slow times or less are divided by scaling_factor, a linear ramp between; factor 0.1 ln(scaling_factor) + 1."""
+              turn beta_slow times or less are divided by scaling_factor, a linear ramp between; factor 0.1 ln(scaling_factor) + 1.  The ramp
+              is in turns, as the formula is published; a program that ramps in the pair's index has other frequencies inside the ramp."""
     if scaling not in SCALINGS:
         raise ValueError(f'Unsupported scaling of rotary positions: {scaling}.')
     if not scaling_factor >= 1.0 or not base > 1.0:
