@@ -1490,7 +1490,8 @@ __device__ __forceinline__ void dkv_block(const Args& a, char* smem, int y, int 
   int first = 0;
   if (a.causal) first = (min(s.n, max(0, key_base - off)) << a.gsh) / 32 * 32;  // rows before see none of these keys
   // key j is seen by query i iff j <= i + off, by packed row r iff (j - off) << gsh <= r
-  const int from = a.causal ? min(key - off, s.n) * (1 << a.gsh) : 0, last = a.causal ? min(key_base + TILE - 1 - off, s.n) * (1 << a.gsh) : 0;
+  auto sees = [&](int j) GEOTR_INLINE { return a.causal ? max(0, min(j - off, s.n)) << a.gsh : 0; };  // below zero it would pass 32 bits
+  const int from = sees(key), last = sees(key_base + TILE - 1);
   for (int h = 0; h < a.g; ++h) minus |= a.lam[kvh * a.g + h] < 0.f;
 
   const T* const qp = (const T*)a.q.data + s.b * a.q.batch_stride + (a.stacked ? s.q0 : 0) * a.q.row_stride + (int64_t)kvh * 2 * a.g * a.q.head_stride;

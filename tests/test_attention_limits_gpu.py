@@ -139,3 +139,27 @@ def test_a_cache_laid_out_by_heads(dtype, n, heads, kv, d, dv):
         leaves = [(t.contiguous() if copy else t).detach().requires_grad_() for t in (q, k, v, lam)]
         grads.append(torch.autograd.grad(differential_attention(*leaves), leaves, dout.contiguous() if copy else dout))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_causal_gradients_of_many_more_keys_than_rows(dtype):
+    """2 rows of 64 heads to a key head over 50 million equal keys: (keys - rows) x heads passes 2^31.  All scores of a row are the same, so that the
+    weights are 1 / keys (sums of equal powers of two are exact) and dv is the same for all keys but the last, which row 0 does not see.
+    Bound: each weight rounded to the type and its factors to 32 bits, products and sums in 32 bits, the result rounded once."""
+    from geotransformer_amd import kernels
+    n, m, heads = 2, 3 * 2 ** 24 + 64, 64
+    one, _, lam = _repeated(1, n, 1, heads, 1, 8, 8, dtype)
+    q, k, v, dout = one[0], one[1].expand(m, -1, -1), one[2].expand(m, -1, -1), one[3]
+    out, state = kernels.diff_attention(q, k, v, lam, causal=True, want_state=True)
+    dv = kernels.diff_attention_backward(dout, q, k, v, lam, state, causal=True)[2]
+    seen = [torch.tensor([m - 1, m]).double(), torch.tensor([float('inf'), m]).double()]  # keys that the two rows see: of any key, of the last
+    u = oracle.U[dtype]
+    alike = bool((dv[:-1] == dv[:1]).all())
+    assert alike
+    for got, count in zip((dv[0], dv[-1]), seen):
+        weights = (1 - lam.cpu().double())[None, :, None] / count[:, None, None]
+        terms = weights.expand(n, heads, 8) * dout.cpu().double()
+        size = ((1 + lam.cpu().double())[None, :, None] / count[:, None, None] * dout.cpu().double().abs()).sum((0, 1))
+        value = terms.sum((0, 1))
+        bound = u * terms.abs().sum((0, 1)) + 2.0 ** -24 * (n * heads + 16) * size
+        oracle.assert_within('dv', got[0], value, bound + u * (value.abs() + bound))
